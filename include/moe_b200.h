@@ -189,6 +189,81 @@ int moe_b200_fused_experts_fp8_tp_reduce(const void* x, const void* w13_q, const
  * that keep quantised activations). */
 int moe_b200_quant_fp8_per_token_group(const void* x, int rows, int cols, void* q, float* scales, void* stream);
 
+/* fused_experts_fp8_tp from activations that are quantised already (what moe_b200_rms_norm_quant_fp8 with groups of 128
+ * writes): x_q e4m3 [T, H], x_scale fp32 [T, H/128]; the call's own quantisation of x falls away, the rest and the workspace
+ * are the same. */
+int moe_b200_fused_experts_fp8_quantized(const void* x_q, const float* x_scale, const void* w13_q, const float* w13_scale,
+                                         const void* w2_q, const float* w2_scale, const float* topk_weights,
+                                         const int32_t* topk_ids, void* out, int T, int E, int top_k, int H, int I,
+                                         int i_offset, int i_total, void* workspace, size_t workspace_bytes,
+                                         int32_t* status_word, void* stream);
+
+/*
+ * RMS norm whose output is e4m3 with scales, optionally with the residual's addition in front and with the bf16 norm next
+ * to it. No reference counterpart (its norm ops write bf16, csrc/ops.cpp:16-27).
+ *   r = bf16(input + residual), written to residual_out (residual == NULL: r = input, residual_out unused);
+ *   residual_out may be residual itself
+ *   y = r * rsqrt(mean(r^2) + eps) * weight in fp32;  s = max(max |y| over the group, 1e-10) / 448;  q = e4m3(y / s)
+ *   normed_out = bf16(y) unless NULL (rounded once: moe_b200_rms_norm rounds before the weight too, as the reference does)
+ *   q e4m3 [T, H]; scales fp32 [T, H/128] for group_size 128 (H % 128 == 0), [T] for group_size H or -1
+ * A NaN in a group makes its scale and codes NaN. bf16 [T, H] contiguous, pointers on 16 bytes (q on 8); H % 8 == 0,
+ * H <= 32768. Outputs must not overlap inputs except residual_out == residual.
+ */
+int moe_b200_rms_norm_quant_fp8(void* q, float* scales, void* normed_out, void* residual_out, const void* residual,
+                                const void* input, const void* weight, float eps, int T, int H, int group_size,
+                                void* stream);
+
+/*
+ * Balance loss, z loss and per-expert counts of a router, and the gradient with respect to its logits. No reference
+ * counterpart (it only serves); stands next to moe_b200_topk_softmax, whose topk_ids it takes.
+ *   gating [T, E] fp32 or bf16; topk_ids int32 [T, k] (entries outside [0, E) are not counted);
+ *   token_mask one byte a token, 0 = padding that is neither read nor counted (NULL: all count);
+ *   n = counted tokens, p = softmax(gating), c_e = counts, P_e = sum_t p_te / n (n = 1 in divisions when none counts)
+ *   losses fp32 [2] = { E * sum_e (c_e / n) P_e, sum_t logsumexp(gating_t)^2 / n };  counts int32 [E];
+ *   num_tokens int32 [1] = n;  mean_probs fp32 [E] = P
+ * Balanced routing gives a balance loss of k. Same bits on every run. E <= 1024.
+ */
+size_t moe_b200_router_loss_workspace_bytes(int T, int E);
+int moe_b200_router_loss(float* losses, int32_t* counts, int32_t* num_tokens, float* mean_probs, const void* gating,
+                         int gating_is_bf16, const int32_t* topk_ids, const uint8_t* token_mask, int T, int E, int k,
+                         void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * grad_logits [T, E] (type of gating) = gradient of
+ *   grad_losses[0] * balance + grad_losses[1] * z + sum grad_topk_weights * topk_weights
+ * with respect to gating; counts and num_tokens as moe_b200_router_loss wrote them (or summed over the ranks of a
+ * data-parallel job). topk_weights = the picked p, divided by their sum when renormalize != 0, as
+ * moe_b200_topk_softmax returns them. grad_losses fp32 [2] and grad_topk_weights fp32 [T, k] may be NULL. Rows of
+ * tokens that the mask leaves out are zero. grad_logits must not overlap gating.
+ */
+int moe_b200_router_backward(void* grad_logits, const void* gating, int gating_is_bf16, const int32_t* topk_ids,
+                             const int32_t* counts, const int32_t* num_tokens, const float* grad_losses,
+                             const float* grad_topk_weights, const uint8_t* token_mask, int T, int E, int k,
+                             int renormalize, void* stream);
+
+/*
+ * Products with 4-bit weights and group scales, built for few tokens (decode). No reference counterpart (its
+ * fused_moe asserts that no scales or zero points are passed, nanovllm/layers/for_moe/fused_moe.py:248-249; its
+ * linears are bf16).
+ *   W[n, k] = (code - zero) * scale;  codes [N, K/2], two a byte, the low nibble is the even k;
+ *   scale bf16 [N, K/group_size];  zero one byte 0..15 per scale, NULL = 8 throughout;  bias bf16 [N] or NULL
+ *   out bf16 [M, N] = x @ W^T + bias;  x bf16, rows x_row_stride elements apart (a multiple of 8)
+ * group_size 32, 64 or 128 and K % group_size == 0; any N. fp32 sums, one rounding. qweight and x on 16 bytes.
+ */
+int moe_b200_w4_linear(void* out, const void* x, int64_t x_row_stride, const void* qweight, const void* scale,
+                       const void* zero, const void* bias, int M, int N, int K, int group_size, void* stream);
+/*
+ * fused_experts with such weights: w13 codes [E, 2*I, H/2] (gate rows then up rows, interleaved for
+ * MOE_B200_ACT_SWIGLUOAI), w2 codes [E, H, I/2], scales [E, 2*I, H/g] and [E, H, I/g], zeros alike or NULL, biases bf16
+ * [E, 2*I] and [E, H] or NULL. H % group_size == 0, I % group_size == 0. Slots whose id is outside [0, E) add
+ * nothing. The intermediate and the slots' results are not rounded to bf16. out may be x.
+ */
+size_t moe_b200_fused_experts_w4_workspace_bytes(int T, int E, int top_k, int H, int I);
+int moe_b200_fused_experts_w4(const void* x, const void* w13_q, const void* w13_scale, const void* w13_zero,
+                              const void* w13_bias, const void* w2_q, const void* w2_scale, const void* w2_zero,
+                              const void* w2_bias, const float* topk_weights, const int32_t* topk_ids, void* out, int T,
+                              int E, int top_k, int H, int I, int group_size, int activation, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
 /*
  * The two grouped GEMM passes on their own, for callers that keep the permutation (block size
  * moe_b200_block_m()) and the intermediates themselves. Each replaces one invoke_fused_moe_kernel call

@@ -122,6 +122,21 @@ int check_block_shapes(int T, int E, int top_k, int H, int I) {
   return kStatusOk;
 }
 
+bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+int check_w4_group(const char* what, int group_size, int K) {
+  if (group_size != 32 && group_size != 64 && group_size != 128)
+    return set_error(kStatusInvalidArgument, "%s: group_size must be 32, 64 or 128 (got %d)", what, group_size);
+  if (K <= 0 || K % group_size != 0)
+    return set_error(kStatusInvalidArgument, "%s: %d columns are not a whole number of groups of %d", what, K, group_size);
+  return kStatusOk;
+}
+
+W4Matrix w4_matrix(const void* q, const void* scale, const void* zero, const void* bias, int group_size) {
+  return W4Matrix{static_cast<const uint8_t*>(q), static_cast<const __nv_bfloat16*>(scale), static_cast<const uint8_t*>(zero),
+                  static_cast<const __nv_bfloat16*>(bias), group_size};
+}
+
 }  // namespace
 
 // Everything of fused_experts up to (not including) the k-slot sum; leaves C3 in the workspace.
@@ -353,7 +368,8 @@ size_t moe_b200_fused_experts_fp8_workspace_bytes(int T, int E, int top_k, int H
 }
 
 // Everything of the fp8 experts up to (not including) the k-slot sum; returns the C3 slot tensor in the workspace.
-static int run_experts_fp8_until_c3(const void* x, const void* w13_q, const float* w13_scale, const void* w2_q,
+// x_scale == nullptr: x is bf16 and quantised here; otherwise x is e4m3 with these scales.
+static int run_experts_fp8_until_c3(const void* x, const float* x_scale, const void* w13_q, const float* w13_scale, const void* w2_q,
                                     const float* w2_scale, const float* topk_weights, const int32_t* topk_ids, int T, int E,
                                     int top_k, int H, int I, int i_offset, int i_total, void* workspace,
                                     size_t workspace_bytes, int32_t* status_word, cudaStream_t s,
@@ -369,7 +385,13 @@ static int run_experts_fp8_until_c3(const void* x, const void* w13_q, const floa
     return set_error(kStatusWorkspaceTooSmall, "fused_experts_fp8: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
   const Fp8Workspace w = carve_fp8(workspace, T, E, top_k, H, I);
   const PermSizes ps = perm_sizes(T, E, top_k);
-  if (int st = launch_quant_rows_fp8(static_cast<const __nv_bfloat16*>(x), T, H, 0, w.x_q, w.x_s, nullptr, 0, nullptr, s)) return st;
+  const uint8_t* x_q = static_cast<const uint8_t*>(x);
+  const float* x_s = x_scale;
+  if (x_scale == nullptr) {
+    if (int st = launch_quant_rows_fp8(static_cast<const __nv_bfloat16*>(x), T, H, 0, w.x_q, w.x_s, nullptr, 0, nullptr, s)) return st;
+    x_q = w.x_q;
+    x_s = w.x_s;
+  }
   if (int st = launch_align_block_size(topk_ids, ps.numel, E, kBlockM, w.base.sorted_ids, ps.sorted_cap, w.base.expert_ids,
                                        ps.blocks_cap, w.base.num_post_pad, w.base.align_ws, w.base.align_ws_bytes, s))
     return st;
@@ -377,7 +399,7 @@ static int run_experts_fp8_until_c3(const void* x, const void* w13_q, const floa
   a.sorted_ids = w.base.sorted_ids; a.expert_ids = w.base.expert_ids; a.num_post_pad = w.base.num_post_pad;
   a.numel = ps.numel; a.top_k = top_k; a.max_m_blocks = ps.blocks_cap; a.num_experts = E;
   a.hidden = H; a.inter = I; a.activation = 0; a.status = status_word;
-  if (int st = launch_grouped_gemm1_fp8(a, w.x_q, w.x_s, static_cast<const uint8_t*>(w13_q), w13_scale, i_offset, i_total,
+  if (int st = launch_grouped_gemm1_fp8(a, x_q, x_s, static_cast<const uint8_t*>(w13_q), w13_scale, i_offset, i_total,
                                         w.base.h_sorted, s))
     return st;
   if (int st = launch_quant_rows_fp8(w.base.h_sorted, ps.sorted_cap, I, i_offset % 128, w.h_q, w.h_s, w.base.sorted_ids,
@@ -398,7 +420,7 @@ int moe_b200_fused_experts_fp8_tp(const void* x, const void* w13_q, const float*
   if (out == nullptr) return set_error(kStatusInvalidArgument, "fused_experts_fp8: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const __nv_bfloat16* c3 = nullptr;
-  if (int st = run_experts_fp8_until_c3(x, w13_q, w13_scale, w2_q, w2_scale, topk_weights, topk_ids, T, E, top_k, H, I,
+  if (int st = run_experts_fp8_until_c3(x, nullptr, w13_q, w13_scale, w2_q, w2_scale, topk_weights, topk_ids, T, E, top_k, H, I,
                                         i_offset, i_total, workspace, workspace_bytes, status_word, s, &c3))
     return st;
   return launch_moe_sum(c3, static_cast<__nv_bfloat16*>(out), T, top_k, H, s);
@@ -413,10 +435,26 @@ int moe_b200_fused_experts_fp8_tp_reduce(const void* x, const void* w13_q, const
   if (out == nullptr || ar_handle == 0) return set_error(kStatusInvalidArgument, "fused_experts_fp8_tp_reduce: null pointer or no communicator");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const __nv_bfloat16* c3 = nullptr;
-  if (int st = run_experts_fp8_until_c3(x, w13_q, w13_scale, w2_q, w2_scale, topk_weights, topk_ids, T, E, top_k, H, I,
+  if (int st = run_experts_fp8_until_c3(x, nullptr, w13_q, w13_scale, w2_q, w2_scale, topk_weights, topk_ids, T, E, top_k, H, I,
                                         i_offset, i_total, workspace, workspace_bytes, status_word, s, &c3))
     return st;
   return ar_moe_sum_all_reduce_impl(ar_handle, c3, out, T, top_k, H, reg_buffer, reg_buffer_bytes, ar_algo, status_word, s);
+}
+
+int moe_b200_fused_experts_fp8_quantized(const void* x_q, const float* x_scale, const void* w13_q, const float* w13_scale,
+                                         const void* w2_q, const float* w2_scale, const float* topk_weights,
+                                         const int32_t* topk_ids, void* out, int T, int E, int top_k, int H, int I,
+                                         int i_offset, int i_total, void* workspace, size_t workspace_bytes,
+                                         int32_t* status_word, void* stream) {
+  if (T == 0) return check_block_shapes(T, E, top_k, H, I);
+  if (out == nullptr || x_scale == nullptr) return set_error(kStatusInvalidArgument, "fused_experts_fp8_quantized: null pointer");
+  if (!aligned(x_q, 16)) return set_error(kStatusInvalidArgument, "fused_experts_fp8_quantized: x_q must start on 16 bytes");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const __nv_bfloat16* c3 = nullptr;
+  if (int st = run_experts_fp8_until_c3(x_q, x_scale, w13_q, w13_scale, w2_q, w2_scale, topk_weights, topk_ids, T, E, top_k,
+                                        H, I, i_offset, i_total, workspace, workspace_bytes, status_word, s, &c3))
+    return st;
+  return launch_moe_sum(c3, static_cast<__nv_bfloat16*>(out), T, top_k, H, s);
 }
 
 int moe_b200_fused_experts_fp8(const void* x, const void* w13_q, const float* w13_scale, const void* w2_q,
@@ -425,6 +463,99 @@ int moe_b200_fused_experts_fp8(const void* x, const void* w13_q, const float* w1
                                int32_t* status_word, void* stream) {
   return moe_b200_fused_experts_fp8_tp(x, w13_q, w13_scale, w2_q, w2_scale, topk_weights, topk_ids, out, T, E, top_k, H,
                                        I, 0, I, workspace, workspace_bytes, status_word, stream);
+}
+
+int moe_b200_rms_norm_quant_fp8(void* q, float* scales, void* normed_out, void* residual_out, const void* residual,
+                                const void* input, const void* weight, float eps, int T, int H, int group_size,
+                                void* stream) {
+  if (T < 0 || H <= 0 || H % 8 != 0 || H > 32768)
+    return set_error(kStatusInvalidArgument, "rms_norm_quant_fp8: the hidden size must be a multiple of 8 up to 32768 (T=%d H=%d)", T, H);
+  const bool per_token = group_size == -1 || (group_size == H && H != 128);
+  if (!per_token && group_size != 128)
+    return set_error(kStatusInvalidArgument, "rms_norm_quant_fp8: group_size must be 128, or -1 (or the hidden size) for one scale a token; got %d", group_size);
+  if (!per_token && H % 128 != 0)
+    return set_error(kStatusInvalidArgument, "rms_norm_quant_fp8: groups of 128 need a hidden size that is a multiple of 128 (got %d)", H);
+  if (T == 0) return kStatusOk;
+  if (q == nullptr || scales == nullptr || input == nullptr || weight == nullptr || (residual != nullptr && residual_out == nullptr))
+    return set_error(kStatusInvalidArgument, "rms_norm_quant_fp8: null pointer");
+  if (!aligned(input, 16) || !aligned(weight, 16) || !aligned(residual, 16) || !aligned(residual_out, 16) ||
+      !aligned(normed_out, 16) || !aligned(q, 8) || !aligned(scales, 4))
+    return set_error(kStatusInvalidArgument, "rms_norm_quant_fp8: bf16 tensors must start on 16 bytes, q on 8, scales on 4");
+  return launch_rms_norm_quant_fp8(static_cast<uint8_t*>(q), scales, static_cast<__nv_bfloat16*>(normed_out),
+                                   static_cast<__nv_bfloat16*>(residual_out), static_cast<const __nv_bfloat16*>(residual),
+                                   static_cast<const __nv_bfloat16*>(input), static_cast<const __nv_bfloat16*>(weight), eps, T,
+                                   H, per_token, static_cast<cudaStream_t>(stream));
+}
+
+size_t moe_b200_router_loss_workspace_bytes(int T, int E) {
+  if (T < 0 || E <= 0) return 0;
+  return router_loss_workspace_bytes(T, E);
+}
+
+int moe_b200_router_loss(float* losses, int32_t* counts, int32_t* num_tokens, float* mean_probs, const void* gating,
+                         int gating_is_bf16, const int32_t* topk_ids, const uint8_t* token_mask, int T, int E, int k,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+  if (losses == nullptr || counts == nullptr || num_tokens == nullptr || mean_probs == nullptr ||
+      (T > 0 && (gating == nullptr || topk_ids == nullptr)))
+    return set_error(kStatusInvalidArgument, "router_loss: null pointer");
+  return launch_router_loss(losses, counts, num_tokens, mean_probs, gating, gating_is_bf16, topk_ids, token_mask, T, E, k,
+                            workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int moe_b200_router_backward(void* grad_logits, const void* gating, int gating_is_bf16, const int32_t* topk_ids,
+                             const int32_t* counts, const int32_t* num_tokens, const float* grad_losses,
+                             const float* grad_topk_weights, const uint8_t* token_mask, int T, int E, int k,
+                             int renormalize, void* stream) {
+  if (T > 0 && (grad_logits == nullptr || gating == nullptr || (grad_topk_weights != nullptr && topk_ids == nullptr) ||
+                (grad_losses != nullptr && (counts == nullptr || num_tokens == nullptr))))
+    return set_error(kStatusInvalidArgument, "router_backward: null pointer");
+  return launch_router_backward(grad_logits, gating, gating_is_bf16, topk_ids, counts, num_tokens, grad_losses,
+                                grad_topk_weights, token_mask, T, E, k, renormalize, static_cast<cudaStream_t>(stream));
+}
+
+int moe_b200_w4_linear(void* out, const void* x, int64_t x_row_stride, const void* qweight, const void* scale,
+                       const void* zero, const void* bias, int M, int N, int K, int group_size, void* stream) {
+  if (M < 0 || N <= 0) return set_error(kStatusInvalidArgument, "w4_linear: bad sizes M=%d N=%d", M, N);
+  if (int st = check_w4_group("w4_linear", group_size, K)) return st;
+  if (M == 0) return kStatusOk;
+  if (out == nullptr || x == nullptr || qweight == nullptr || scale == nullptr)
+    return set_error(kStatusInvalidArgument, "w4_linear: null pointer");
+  if (!aligned(x, 16) || !aligned(qweight, 16) || (M > 1 && (x_row_stride % 8 != 0 || x_row_stride < K)))
+    return set_error(kStatusInvalidArgument, "w4_linear: x and qweight must start on 16 bytes and the rows of x lie a multiple of 8 elements, at least K, apart");
+  return launch_w4_linear(static_cast<__nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(x), x_row_stride,
+                          w4_matrix(qweight, scale, zero, bias, group_size), M, N, K, static_cast<cudaStream_t>(stream));
+}
+
+size_t moe_b200_fused_experts_w4_workspace_bytes(int T, int E, int top_k, int H, int I) {
+  if (T < 0 || E <= 0 || top_k <= 0 || H <= 0 || I <= 0) return 0;
+  return w4_experts_workspace_bytes(T, top_k, H, I);
+}
+
+int moe_b200_fused_experts_w4(const void* x, const void* w13_q, const void* w13_scale, const void* w13_zero,
+                              const void* w13_bias, const void* w2_q, const void* w2_scale, const void* w2_zero,
+                              const void* w2_bias, const float* topk_weights, const int32_t* topk_ids, void* out, int T,
+                              int E, int top_k, int H, int I, int group_size, int activation, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  if (int st = check_block_shapes(T, E, top_k, H, I)) return st;
+  if (int st = check_w4_group("fused_experts_w4 (H)", group_size, H)) return st;
+  if (int st = check_w4_group("fused_experts_w4 (I)", group_size, I)) return st;
+  if (activation != MOE_B200_ACT_SILU && activation != MOE_B200_ACT_SWIGLUOAI)
+    return set_error(kStatusInvalidArgument, "fused_experts_w4: unsupported activation code %d", activation);
+  if (T == 0) return kStatusOk;
+  if (x == nullptr || w13_q == nullptr || w13_scale == nullptr || w2_q == nullptr || w2_scale == nullptr ||
+      topk_weights == nullptr || topk_ids == nullptr || out == nullptr)
+    return set_error(kStatusInvalidArgument, "fused_experts_w4: null pointer");
+  if ((w13_zero == nullptr) != (w2_zero == nullptr))
+    return set_error(kStatusInvalidArgument, "fused_experts_w4: zero points for both weights or for none");
+  if (!aligned(x, 16) || !aligned(w13_q, 16) || !aligned(w2_q, 16))
+    return set_error(kStatusInvalidArgument, "fused_experts_w4: x and the codes must start on 16 bytes");
+  const size_t need = moe_b200_fused_experts_w4_workspace_bytes(T, E, top_k, H, I);
+  if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16))
+    return set_error(kStatusWorkspaceTooSmall, "fused_experts_w4: workspace of %zu bytes on 16 needed, %zu given", need, workspace_bytes);
+  return launch_w4_experts(static_cast<__nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(x),
+                           w4_matrix(w13_q, w13_scale, w13_zero, w13_bias, group_size),
+                           w4_matrix(w2_q, w2_scale, w2_zero, w2_bias, group_size), topk_weights, topk_ids, T, E, top_k, H, I,
+                           activation, workspace, static_cast<cudaStream_t>(stream));
 }
 
 size_t moe_b200_fused_moe_workspace_bytes(int T, int E, int top_k, int H, int I) {

@@ -102,6 +102,36 @@ int launch_grouped_gemm1_fp8(const GroupedGemmArgs& a, const uint8_t* x_q, const
 int launch_grouped_gemm2_fp8(const GroupedGemmArgs& a, const uint8_t* h_q, const float* h_s, const uint8_t* w2_q,
                              const float* w2_s, int i_offset, int i_total, const float* topk_w, __nv_bfloat16* c3,
                              cudaStream_t stream);
+// ---- norm_quant.cu: (add +) RMS norm with an e4m3 output, one scale per 128 columns or per token
+int launch_rms_norm_quant_fp8(uint8_t* q, float* scales, __nv_bfloat16* normed, __nv_bfloat16* residual_out,
+                              const __nv_bfloat16* residual, const __nv_bfloat16* input, const __nv_bfloat16* weight,
+                              float eps, int T, int H, bool per_token, cudaStream_t stream);
+
+// ---- router_loss.cu
+size_t router_loss_workspace_bytes(int T, int E);
+int launch_router_loss(float* losses, int* counts, int* num_tokens, float* mean_probs, const void* gating, int gating_is_bf16,
+                       const int* topk_ids, const uint8_t* token_mask, int T, int E, int k, void* workspace,
+                       size_t workspace_bytes, cudaStream_t stream);
+int launch_router_backward(void* grad_logits, const void* gating, int gating_is_bf16, const int* topk_ids, const int* counts,
+                           const int* num_tokens, const float* grad_losses, const float* grad_topk_weights,
+                           const uint8_t* token_mask, int T, int E, int k, int renormalize, cudaStream_t stream);
+
+// ---- w4_gemv.cu: 4-bit weights [rows, K / 2] (two codes a byte, low nibble first) with a bf16 scale and, if zero is not
+// null, a zero point (one byte, 0..15; 8 otherwise) per row and group of `group` columns; bias [rows] or null
+struct W4Matrix {
+  const uint8_t* q;
+  const __nv_bfloat16* scale;
+  const uint8_t* zero;
+  const __nv_bfloat16* bias;
+  int group;
+};
+int launch_w4_linear(__nv_bfloat16* out, const __nv_bfloat16* x, long long x_ld, const W4Matrix& w, int M, int N, int K,
+                     cudaStream_t stream);
+size_t w4_experts_workspace_bytes(int T, int top_k, int H, int I);
+int launch_w4_experts(__nv_bfloat16* out, const __nv_bfloat16* x, const W4Matrix& w13, const W4Matrix& w2, const float* topk_w,
+                      const int* topk_ids, int T, int E, int top_k, int H, int I, int activation, void* workspace,
+                      cudaStream_t stream);
+
 // Tensor map of a dense bf16 (elem_bytes 2) or byte (elem_bytes 1) tensor, 128-byte swizzle; dims/box innermost first.
 int make_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint32_t* box, int elem_bytes);
 // Token blocks the permutation is expected to produce, and the share of SM-time a round-robin tile list keeps busy.

@@ -119,7 +119,13 @@ def fused_experts_impl(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.
                        block_shape=None, w1_bias: Optional[torch.Tensor] = None,
                        w2_bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """for_moe/fused_moe.py:461-633. With e4m3 weights, `w1_scale` / `w2_scale` and `block_shape=[128, 128]` (arguments
-    the reference declares and asserts unused) the block-scaled fp8 path runs instead."""
+    the reference declares and asserts unused) the block-scaled fp8 path runs instead; hidden_states may then be e4m3 with
+    `a1_scale` fp32 [T, H / 128] (what ops.rms_norm_quant_fp8 writes). With packed uint8 weights and `block_shape=[0, group]`
+    the 4-bit path runs (`w1_scale` / `w2_scale` bf16 per row and group, `w1_zp` / `w2_zp` zero points or None; see quant_w4)."""
+    if block_shape is not None and len(block_shape) == 2 and block_shape[0] == 0:
+        return _fused_experts_w4(hidden_states, w1, w2, topk_weights, topk_ids, inplace, activation, w1_scale, w2_scale, w1_zp,
+                                 w2_zp, block_shape[1], w1_bias, w2_bias, a1_scale, a2_scale, expert_map, global_num_experts,
+                                 apply_router_weight_on_input)
     if w1.dtype in (torch.float8_e4m3fn, torch.uint8):
         return _fused_experts_fp8(hidden_states, w1, w2, topk_weights, topk_ids, inplace, activation, w1_scale,
                                   w2_scale, block_shape, w1_bias, w2_bias, a1_scale, a2_scale, w1_zp, w2_zp,
@@ -192,18 +198,22 @@ def _fused_experts_fp8(hidden_states, w1, w2, topk_weights, topk_ids, inplace, a
                        apply_router_weight_on_input, out: Optional[torch.Tensor] = None,
                        intermediate_offset: int = 0, intermediate_size: Optional[int] = None, comm=None) -> torch.Tensor:
     """w8a8 e4m3: weights [E, 2I, H] / [E, H, I] with fp32 scales per 128 x 128 block, activations quantised per
-    token and 128 columns inside the library (dynamic, so a1_scale / a2_scale stay None)."""
+    token and 128 columns inside the library (a2_scale stays None), unless they come as e4m3 with a1_scale [T, H / 128]."""
     if not hidden_states.is_cuda:
         raise RuntimeError("fused_experts needs CUDA tensors; there is no CPU path")
-    if hidden_states.dtype != torch.bfloat16:
-        raise ValueError(f"Unsupported compute_type: {hidden_states.dtype} (activations enter as bfloat16)")
+    quantized = hidden_states.dtype == torch.float8_e4m3fn
+    if hidden_states.dtype != torch.bfloat16 and not quantized:
+        raise ValueError(f"Unsupported compute_type: {hidden_states.dtype} (activations enter as bfloat16, or as e4m3 with a1_scale)")
+    if quantized and (inplace or comm is not None):
+        raise NotImplementedError("e4m3 hidden states cannot take the bf16 result in place, nor go into the fused reduction")
     if w2.dtype != w1.dtype:
         raise ValueError("w1 and w2 must both be e4m3")
     if w1_scale is None or w2_scale is None or block_shape is None or list(block_shape) != [128, 128]:
         raise ValueError("fp8 weights need w1_scale, w2_scale and block_shape=[128, 128]")
     if activation != "silu" or w1_bias is not None or w2_bias is not None:
         raise NotImplementedError("the fp8 path is built for silu without expert biases")
-    for name, v in dict(a1_scale=a1_scale, a2_scale=a2_scale, w1_zp=w1_zp, w2_zp=w2_zp, expert_map=expert_map).items():
+    for name, v in dict(a1_scale=None if quantized else a1_scale, a2_scale=a2_scale, w1_zp=w1_zp, w2_zp=w2_zp,
+                        expert_map=expert_map).items():
         assert v is None, f"{name} is not supported"
     if apply_router_weight_on_input:
         raise NotImplementedError("apply_router_weight_on_input=True is not used by the reference's models")
@@ -222,8 +232,11 @@ def _fused_experts_fp8(hidden_states, w1, w2, topk_weights, topk_ids, inplace, a
     assert s1.shape == (E, 2 * i_total // 128, H // 128), f"w1_scale shape {tuple(s1.shape)}"
     assert s2.shape == (E, H // 128, i_total // 128), f"w2_scale shape {tuple(s2.shape)}"
     k = topk_ids.size(1)
+    if quantized and (a1_scale is None or a1_scale.dtype != torch.float32 or a1_scale.shape != (T, H // 128)
+                      or not a1_scale.is_contiguous() or a1_scale.device != hidden_states.device):
+        raise ValueError(f"e4m3 hidden states need a contiguous a1_scale fp32 [{T}, {H // 128}] on their device")
     if out is None:
-        out = hidden_states if inplace else torch.empty_like(hidden_states)
+        out = hidden_states if inplace else torch.empty_like(hidden_states, dtype=torch.bfloat16)
     assert out.shape == hidden_states.shape and out.dtype == torch.bfloat16 and out.is_contiguous()
     if T == 0:
         return out
@@ -235,7 +248,12 @@ def _fused_experts_fp8(hidden_states, w1, w2, topk_weights, topk_ids, inplace, a
     import ctypes
     fptr = ctypes.POINTER(ctypes.c_float)
     with torch.cuda.device(dev):
-        if comm is not None and not comm.disabled and comm.world_size > 1 and T * H * 2 <= comm.max_size:
+        if quantized:
+            check(lib.moe_b200_fused_experts_fp8_quantized(
+                hidden_states.data_ptr(), a1_scale.data_ptr(), w1.data_ptr(), s1.data_ptr(), w2.data_ptr(), s2.data_ptr(),
+                tw.data_ptr(), ti.data_ptr(), out.data_ptr(), T, E, k, H, inter, i_off, i_total, ws.data_ptr(), ws.numel(),
+                ops.status_word(dev).data_ptr(), torch.cuda.current_stream().cuda_stream))
+        elif comm is not None and not comm.disabled and comm.world_size > 1 and T * H * 2 <= comm.max_size:
             check(lib.moe_b200_fused_experts_fp8_tp_reduce(
                 hidden_states.data_ptr(), w1.data_ptr(), ctypes.cast(s1.data_ptr(), fptr), w2.data_ptr(),
                 ctypes.cast(s2.data_ptr(), fptr), tw.data_ptr(), ti.data_ptr(), out.data_ptr(), T, E, k, H, inter, i_off,
@@ -248,6 +266,83 @@ def _fused_experts_fp8(hidden_states, w1, w2, topk_weights, topk_ids, inplace, a
                 i_total, ws.data_ptr(), ws.numel(), ops.status_word(dev).data_ptr(),
                 torch.cuda.current_stream().cuda_stream))
     return out
+
+
+def _fused_experts_w4(hidden_states, w1, w2, topk_weights, topk_ids, inplace, activation, w1_scale, w2_scale, w1_zp, w2_zp,
+                      group_size, w1_bias, w2_bias, a1_scale, a2_scale, expert_map, global_num_experts,
+                      apply_router_weight_on_input) -> torch.Tensor:
+    """4-bit weights with group scales, bf16 activations: w1 uint8 [E, 2I, H / 2], w2 uint8 [E, H, I / 2] (quant_w4's layout)."""
+    if w1.dtype != torch.uint8 or w2.dtype != torch.uint8 or w1.dim() != 3 or w2.dim() != 3:
+        raise ValueError("block_shape=[0, group] needs packed uint8 weights [E, 2I, H / 2] and [E, H, I / 2]")
+    if w1_scale is None or w2_scale is None or (w1_zp is None) != (w2_zp is None):
+        raise ValueError("4-bit weights need w1_scale and w2_scale, and zero points for both or for none")
+    if group_size not in (32, 64, 128):
+        raise ValueError(f"4-bit weights come in groups of 32, 64 or 128, got {group_size}")
+    if activation not in ACT_CODES:
+        raise ValueError(f"Unsupported FusedMoe activation: {activation}")
+    for name, v in dict(a1_scale=a1_scale, a2_scale=a2_scale, expert_map=expert_map).items():
+        if v is not None:
+            raise ValueError(f"{name} is not supported with 4-bit weights")
+    if apply_router_weight_on_input or global_num_experts not in (-1, w1.size(0)):
+        raise NotImplementedError("apply_router_weight_on_input and expert parallelism are not used by the reference's models")
+    if hidden_states.dim() != 2 or topk_ids.dim() != 2 or topk_weights.shape != topk_ids.shape:
+        raise ValueError("hidden_states must be [T, H], topk_weights and topk_ids [T, k]")
+    T, H = hidden_states.shape
+    E, inter, k, g = w1.size(0), w1.size(1) // 2, topk_ids.size(1), group_size
+    if H % g or inter % g:
+        raise ValueError(f"H and I must be whole numbers of groups of {g} (H={H}, I={inter})")
+    tw = topk_weights if topk_weights.dtype == torch.float32 else topk_weights.float()
+    ti = topk_ids if topk_ids.dtype == torch.int32 else topk_ids.to(torch.int32)
+    tw, ti = tw.contiguous(), ti.contiguous()
+    bf16, u8, dev = torch.bfloat16, torch.uint8, hidden_states.device
+    ops._check("fused_experts (4-bit)", dev, hidden_states=(hidden_states, bf16, (T, H)), w1=(w1, u8, (E, 2 * inter, H // 2)),
+               w2=(w2, u8, (E, H, inter // 2)), w1_scale=(w1_scale, bf16, (E, 2 * inter, H // g)),
+               w2_scale=(w2_scale, bf16, (E, H, inter // g)), w1_zp=(w1_zp, u8, (E, 2 * inter, H // g)),
+               w2_zp=(w2_zp, u8, (E, H, inter // g)), w1_bias=(w1_bias, bf16, (E, 2 * inter)), w2_bias=(w2_bias, bf16, (E, H)),
+               topk_weights=(tw, torch.float32, (T, k)), topk_ids=(ti, torch.int32, (T, k)))
+    out = hidden_states if inplace else torch.empty_like(hidden_states)
+    nbytes = lib.moe_b200_fused_experts_w4_workspace_bytes(T, E, k, H, inter)
+    # not the shared scratch buffer: a tensor of the current stream (or of the capture's own pool), a few KB a slot
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    p = ops._ptr
+    ops._launch(lib.moe_b200_fused_experts_w4, dev, p(hidden_states), p(w1), p(w1_scale), p(w1_zp), p(w1_bias), p(w2), p(w2_scale),
+                p(w2_zp), p(w2_bias), p(tw), p(ti), p(out), T, E, k, H, inter, g, ACT_CODES[activation], p(ws), nbytes)
+    return out
+
+
+def quant_w4(weight: torch.Tensor, group_size: int = 128, zero_points: bool = False):
+    """Rounds weights [..., N, K] to 4-bit codes with a bf16 scale (and, with zero_points, a zero point) per row and group of
+    group_size columns: weight ~ (code - zero) * scale, zero = 8 without zero points. Returns (codes uint8 [..., N, K / 2], two a
+    byte with the even column in the low nibble, scales bf16 [..., N, K / group_size], zeros uint8 or None). Done once when
+    weights are loaded; works on any device."""
+    if group_size not in (32, 64, 128) or weight.size(-1) % group_size:
+        raise ValueError(f"group_size must be 32, 64 or 128 and divide the {weight.size(-1)} columns")
+    w = weight.float().unflatten(-1, (-1, group_size))
+    if zero_points:
+        lo, hi = w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)
+        scale = ((hi - lo) / 15).to(torch.bfloat16)
+        s = scale.float()
+        zero = torch.where(s > 0, (-lo / s).round(), torch.zeros_like(s)).clamp(0, 15)
+    else:
+        scale = (w.abs().amax(-1) / 7.5).to(torch.bfloat16)
+        s, zero = scale.float(), torch.full_like(scale, 8, dtype=torch.float32)
+    code = torch.where(s[..., None] > 0, w / s[..., None], torch.zeros_like(w)).add_(zero[..., None]).round_().clamp_(0, 15)
+    code = code.to(torch.uint8).flatten(-2)
+    return code[..., 0::2] | (code[..., 1::2] << 4), scale, zero.to(torch.uint8) if zero_points else None
+
+
+def shard_w4_expert_weights(w13, w2, tp_rank: int, tp_size: int, group_size: int):
+    """Slices 4-bit expert weights over the intermediate dimension the way FusedMoE.weight_loader slices bf16 ones
+    (nanovllm/layers/fused_moe.py:400-470). w13 and w2 are quant_w4's (codes, scales, zeros) of [E, 2I, H] and [E, H, I];
+    a rank's share of I has to be a whole number of groups. Returns the two triples of this rank. Works on any device."""
+    inter = w13[0].size(1) // 2
+    if inter % tp_size or (inter // tp_size) % group_size:
+        raise ValueError(f"a rank's share of I={inter} over {tp_size} ranks must be a whole number of groups of {group_size}")
+    ip = inter // tp_size
+    lo, hi = tp_rank * ip, (tp_rank + 1) * ip
+    rows = lambda t: None if t is None else torch.cat([t[:, lo:hi], t[:, inter + lo:inter + hi]], dim=1)  # noqa: E731
+    cols = lambda t, per: None if t is None else t[:, :, lo // per:hi // per].contiguous()  # noqa: E731
+    return tuple(rows(t) for t in w13), tuple(cols(t, per) for t, per in zip(w2, (2, group_size, group_size)))
 
 
 def shard_fp8_expert_weights(w13_q: torch.Tensor, w2_q: torch.Tensor, tp_rank: int, tp_size: int):
@@ -319,6 +414,64 @@ def fused_moe_forward_fp8(hidden_states: torch.Tensor, router_logits: torch.Tens
     tw, ti, _ = fused_topk(hidden_states, router_logits, top_k, renormalize)
     return _fused_experts_fp8(hidden_states, w13_q, w2_q, tw, ti, False, "silu", w13_scale, w2_scale, [128, 128], None,
                               None, None, None, None, None, None, False, out=out)
+
+
+def fused_moe_forward_w4(hidden_states: torch.Tensor, router_logits: torch.Tensor, w13, w2, top_k: int, group_size: int,
+                         renormalize: bool = True, activation: str = "silu", inplace: bool = False) -> torch.Tensor:
+    """Router + 4-bit experts: what FusedMoE.forward does (layers/fused_moe.py:590-612) with quant_w4's (codes, scales, zeros)
+    of w13 [E, 2I, H] and w2 [E, H, I]."""
+    tw, ti, _ = fused_topk(hidden_states, router_logits, top_k, renormalize)
+    return fused_experts_impl(hidden_states, w13[0], w2[0], tw, ti, inplace, activation, w1_scale=w13[1], w2_scale=w2[1],
+                              w1_zp=w13[2], w2_zp=w2[2], block_shape=[0, group_size])
+
+
+class _TopkWithLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gating_output, topk, renormalize, token_mask):
+        T, E = gating_output.shape
+        dev = gating_output.device
+        tw = torch.empty(T, topk, dtype=torch.float32, device=dev)
+        ti = torch.empty(T, topk, dtype=torch.int32, device=dev)
+        losses = torch.empty(2, dtype=torch.float32, device=dev)
+        counts = torch.empty(E, dtype=torch.int32, device=dev)
+        num = torch.empty(1, dtype=torch.int32, device=dev)
+        mean_probs = torch.empty(E, dtype=torch.float32, device=dev)
+        if T > 0:
+            ops.topk_softmax_renorm(tw, ti, gating_output, renormalize)
+        ops.router_loss(losses, counts, num, mean_probs, gating_output, ti, token_mask)
+        ctx.save_for_backward(gating_output, ti, counts, num, token_mask)
+        ctx.renormalize = renormalize
+        ctx.mark_non_differentiable(ti, counts)
+        ctx.set_materialize_grads(False)
+        return tw, ti, losses, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_tw, _g_ti, g_losses, _g_counts):
+        gating_output, ti, counts, num, token_mask = ctx.saved_tensors
+        if g_tw is None and g_losses is None:
+            return None, None, None, None
+        grad = torch.empty_like(gating_output)
+        ops.router_backward(grad, gating_output, ti, counts, num, None if g_losses is None else g_losses.contiguous(),
+                            None if g_tw is None else g_tw.contiguous(), ctx.renormalize, token_mask)
+        return grad, None, None, None
+
+
+def fused_topk_with_loss(gating_output: torch.Tensor, topk: int, renormalize: bool, token_mask: Optional[torch.Tensor] = None):
+    """`fused_topk` for training a router: returns (topk_weights fp32 [T, k], topk_ids int32 [T, k], balance_loss, z_loss,
+    counts int32 [E]). topk_weights and the losses (see ops.router_loss) are differentiable once with respect to
+    gating_output (fp32 or bf16 [T, E]); tokens that token_mask (bool [T]) leaves out do not count and get no gradient,
+    not through their routed weights either. Balanced routing has a balance loss of k. Weight the losses by their
+    coefficients and add them to the task's loss. A captured backward pass needs what torch asks for: a graph of its own, built
+    in the capture, whose leaves no eager graph holds."""
+    if gating_output.dim() != 2 or gating_output.dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError("fused_topk_with_loss: gating_output must be float32 or bfloat16 [T, E]")
+    if not gating_output.is_cuda:
+        raise RuntimeError("fused_topk_with_loss needs CUDA tensors; there is no CPU path")
+    if not 0 < topk <= gating_output.size(1):
+        raise RuntimeError(f"fused_topk_with_loss: need 0 < topk <= {gating_output.size(1)}, got {topk}")
+    tw, ti, losses, counts = _TopkWithLoss.apply(gating_output.contiguous(), int(topk), bool(renormalize), token_mask)
+    return tw, ti, losses[0], losses[1], counts
 
 
 def per_token_group_quant_fp8(x: torch.Tensor, group_size: int = 128):

@@ -55,13 +55,17 @@ class RowParallelLinear(nn.Module):
         shard_size = param.data.size(self.tp_dim)
         param.data.copy_(loaded_weight.narrow(self.tp_dim, self.tp_rank * shard_size, shard_size))
 
+    def _product(self, x: torch.Tensor, out: torch.Tensor) -> None:
+        """out = this rank's product, with the bias on rank 0."""
+        if self.bias is not None and self.tp_rank == 0:
+            torch.addmm(self.bias, x, self.weight.t(), out=out)
+        else:
+            torch.matmul(x, self.weight.t(), out=out)
+
     def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """linear.py:188-201."""
         if out is not None:
-            if self.bias is not None and self.tp_rank == 0:
-                torch.addmm(self.bias, x, self.weight.t(), out=out)
-            else:
-                torch.matmul(x, self.weight.t(), out=out)
+            self._product(x, out)
             if self.tp_size > 1:
                 red = tensor_model_parallel_all_reduce(out)
                 if red.data_ptr() != out.data_ptr():
@@ -90,9 +94,38 @@ class RowParallelLinear(nn.Module):
             ops.add_rms_norm(normed, res2, y, norm_weight, eps)
             return normed.view(*lead, self.output_size), residual
         staged = comm.staging_view((x2.shape[0], self.output_size), torch.bfloat16)
-        if self.bias is not None and self.tp_rank == 0:
-            torch.addmm(self.bias, x2, self.weight.t(), out=staged)
-        else:
-            torch.matmul(x2, self.weight.t(), out=staged)
+        self._product(x2, staged)
         normed, _ = comm.all_reduce_add_rms_norm(staged, res2, norm_weight, eps)
         return normed.view(*lead, self.output_size), residual
+
+
+class W4RowParallelLinear(RowParallelLinear):
+    """RowParallelLinear with 4-bit weights and group scales (fused_moe.quant_w4's layout; the product is ops.w4_linear, built for
+    decode batches): qweight uint8 [output_size, input_size / tp / 2], scales bf16 [output_size, input_size / tp / group], zeros
+    uint8 like scales or None. weight_loader takes the unsharded codes, scales and zeros and keeps this rank's columns, so
+    a rank's share of the input has to be a whole number of groups."""
+
+    def __init__(self, input_size: int, output_size: int, bias: bool = False, group_size: int = 128, zero_points: bool = False):
+        super().__init__(input_size, output_size, bias)
+        k = self.input_size_per_partition
+        if group_size not in (32, 64, 128) or k % group_size:
+            raise ValueError(f"group_size must be 32, 64 or 128 and divide this rank's {k} input columns")
+        del self.weight
+        self.group_size = group_size
+        shapes = {"qweight": (k // 2, torch.uint8), "scales": (k // group_size, torch.bfloat16),
+                  "zeros": (k // group_size, torch.uint8) if zero_points else None}
+        for name, spec in shapes.items():
+            if spec is None:
+                self.register_parameter(name, None)
+                continue
+            p = nn.Parameter(torch.empty(output_size, spec[0], dtype=spec[1]), requires_grad=False)
+            p.weight_loader = self.weight_loader
+            setattr(self, name, p)
+
+    def _product(self, x: torch.Tensor, out: torch.Tensor) -> None:
+        ops.w4_linear(out, x, self.qweight, self.scales, self.zeros, self.bias if self.tp_rank == 0 else None)
+
+    def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if out is None:
+            out = torch.empty(*x.shape[:-1], self.output_size, dtype=x.dtype, device=x.device)
+        return super().forward(x, out)

@@ -110,6 +110,135 @@ def topk_softmax_renorm(topk_weights: torch.Tensor, topk_indices: torch.Tensor, 
                                         topk_weights.size(-1), int(bool(renormalize)), _stream()))
 
 
+# ---------------------------------------------------------------- low-precision operators around the block, router losses
+def _launch(fn, device: torch.device, *args) -> None:
+    """check(fn(*args, current stream)) with `device` current."""
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch.cuda.current_stream().cuda_stream))
+
+
+def _check(op: str, device: torch.device, **tensors) -> None:
+    """name=(tensor, dtype, shape): CUDA tensor of that device, dtype and shape, contiguous. None tensors pass."""
+    for name, (t, dtype, shape) in tensors.items():
+        if t is None:
+            continue
+        if t.device != device or not t.is_cuda:
+            raise RuntimeError(f"{op}: {name} must be on the CUDA device of the other tensors (got {t.device}); there is no CPU path")
+        if t.dtype != dtype:
+            raise RuntimeError(f"{op}: {name} must be {dtype}, got {t.dtype}")
+        if t.shape != shape:
+            raise RuntimeError(f"{op}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+        if not t.is_contiguous():
+            raise RuntimeError(f"{op}: {name} must be contiguous")
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _norm_quant(op, out, scales, residual, input, weight, epsilon, group_size, normed_out, residual_out):  # noqa: A002
+    H = input.size(-1) if input.dim() else 0
+    T = input.numel() // H if H else 0
+    groups = 1 if group_size == -1 or (group_size == H and H != 128) else H // 128
+    bf16, shape = torch.bfloat16, input.shape
+    _check(op, input.device, input=(input, bf16, shape), out=(out, torch.float8_e4m3fn, shape), weight=(weight, bf16, (H,)),
+           residual=(residual, bf16, shape), residual_out=(residual_out, bf16, shape), normed_out=(normed_out, bf16, shape),
+           scales=(scales, torch.float32, (*shape[:-1], groups)))
+    _launch(lib.moe_b200_rms_norm_quant_fp8, input.device, out.data_ptr(), scales.data_ptr(), _ptr(normed_out),
+            _ptr(residual_out), _ptr(residual), input.data_ptr(), weight.data_ptr(), epsilon, T, H, group_size)
+
+
+def rms_norm_quant_fp8(out: torch.Tensor, scales: torch.Tensor, input: torch.Tensor, weight: torch.Tensor,  # noqa: A002
+                       epsilon: float, group_size: int = 128, normed_out: torch.Tensor | None = None) -> None:
+    """RMS norm with an e4m3 output: y = input * rsqrt(mean(input^2) + eps) * weight in fp32, scales = max(|y|, 1e-10) / 448 over
+    each group of 128 columns ([.., H / 128]) or, with group_size -1, over each token ([.., 1]), out = e4m3(y / scale).
+    normed_out, if given, gets bf16(y), rounded once (`rms_norm` also rounds before the weight). The pair (out, scales) with groups
+    of 128 is what `fused_experts` takes as hidden states and `a1_scale` next to e4m3 weights."""
+    _norm_quant("rms_norm_quant_fp8", out, scales, None, input, weight, epsilon, group_size, normed_out, None)
+
+
+def add_rms_norm_quant_fp8(out: torch.Tensor, scales: torch.Tensor, residual: torch.Tensor, input: torch.Tensor,  # noqa: A002
+                           weight: torch.Tensor, epsilon: float, group_size: int = 128,
+                           normed_out: torch.Tensor | None = None, residual_out: torch.Tensor | None = None) -> None:
+    """`rms_norm_quant_fp8` of residual <- bf16(input + residual): the sum is written to residual_out, or to residual itself."""
+    _norm_quant("add_rms_norm_quant_fp8", out, scales, residual, input, weight, epsilon, group_size, normed_out,
+                residual if residual_out is None else residual_out)
+
+
+def w4_linear(out: torch.Tensor, input: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,  # noqa: A002
+              zeros: torch.Tensor | None = None, bias: torch.Tensor | None = None) -> None:
+    """out[.., N] = input[.., K] @ W^T + bias for 4-bit weights W[n, k] = (code - zero) * scale, built for few tokens (any number
+    works). qweight uint8 [N, K / 2], two codes a byte, the low nibble is the even k; scales bf16 [N, K / group], groups of 32, 64 or
+    128; zeros uint8 0..15 like scales (8 without it); bias bf16 [N]. A two-dimensional input may have rows further than K apart
+    (a multiple of 8 elements). `fused_moe.quant_w4` makes such weights."""
+    K = input.size(-1) if input.dim() else 0
+    N, groups = (qweight.size(0), scales.size(-1)) if qweight.dim() == 2 and scales.dim() == 2 else (0, 0)
+    if N == 0 or groups == 0 or K == 0:
+        raise RuntimeError("w4_linear: qweight must be [N, K / 2], scales [N, K / group] and input [.., K]")
+    M = input.numel() // K
+    ld = K
+    if input.dim() == 2 and input.stride(1) == 1 and not input.is_contiguous():
+        ld = input.stride(0)
+        _check("w4_linear", qweight.device, input=(input[:1], torch.bfloat16, (min(M, 1), K)))
+    else:
+        _check("w4_linear", qweight.device, input=(input, torch.bfloat16, input.shape))
+    _check("w4_linear", qweight.device, out=(out, torch.bfloat16, (*input.shape[:-1], N)), qweight=(qweight, torch.uint8, (N, K // 2)),
+           scales=(scales, torch.bfloat16, (N, groups)), zeros=(zeros, torch.uint8, (N, groups)), bias=(bias, torch.bfloat16, (N,)))
+    _launch(lib.moe_b200_w4_linear, qweight.device, out.data_ptr(), input.data_ptr(), ld, qweight.data_ptr(), scales.data_ptr(),
+            _ptr(zeros), _ptr(bias), M, N, K, K // groups if K % groups == 0 else -1)
+
+
+def _router_args(op, gating_output, topk_ids, token_mask):
+    if gating_output.dim() != 2 or topk_ids.dim() != 2:
+        raise RuntimeError(f"{op}: gating_output must be [T, E] and topk_ids [T, k]")
+    if gating_output.dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError(f"{op}: gating_output must be float32 or bfloat16")
+    T, E = gating_output.shape
+    k = topk_ids.size(1)
+    _check(op, gating_output.device, gating_output=(gating_output, gating_output.dtype, (T, E)),
+           topk_ids=(topk_ids, torch.int32, (T, k)))
+    if token_mask is not None:
+        _check(op, gating_output.device,
+               token_mask=(token_mask, torch.uint8 if token_mask.dtype == torch.uint8 else torch.bool, (T,)))
+    return T, E, k
+
+
+def router_loss(losses: torch.Tensor, counts: torch.Tensor, num_tokens: torch.Tensor, mean_probs: torch.Tensor,
+                gating_output: torch.Tensor, topk_ids: torch.Tensor, token_mask: torch.Tensor | None = None) -> None:
+    """Balance loss, z loss and per-expert counts of a routed batch. gating_output fp32 or bf16 [T, E], topk_ids int32 [T, k] (ids
+    outside [0, E) are not counted), token_mask bool [T] (False: padding, neither read nor counted). With n counted tokens
+    (divisions by at least 1) and p = softmax(gating_output): counts int32 [E], num_tokens int32 [1] = n, mean_probs fp32 [E] =
+    sum p / n, losses fp32 [2] = (E * sum(counts / n * mean_probs), sum logsumexp^2 / n). E <= 1024. Same bits on every run."""
+    T, E, k = _router_args("router_loss", gating_output, topk_ids, token_mask)
+    dev = gating_output.device
+    _check("router_loss", dev, losses=(losses, torch.float32, (2,)), counts=(counts, torch.int32, (E,)),
+           num_tokens=(num_tokens, torch.int32, (1,)), mean_probs=(mean_probs, torch.float32, (E,)))
+    nbytes = lib.moe_b200_router_loss_workspace_bytes(T, E)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch(lib.moe_b200_router_loss, dev, losses.data_ptr(), counts.data_ptr(), num_tokens.data_ptr(), mean_probs.data_ptr(),
+            gating_output.data_ptr(), gating_output.dtype == torch.bfloat16, topk_ids.data_ptr(), _ptr(token_mask), T, E, k,
+            ws.data_ptr(), nbytes)
+
+
+def router_backward(grad_logits: torch.Tensor, gating_output: torch.Tensor, topk_ids: torch.Tensor, counts: torch.Tensor,
+                    num_tokens: torch.Tensor, grad_losses: torch.Tensor | None, grad_topk_weights: torch.Tensor | None,
+                    renormalize: bool, token_mask: torch.Tensor | None = None) -> None:
+    """grad_logits (like gating_output) = gradient of grad_losses . (balance, z) + sum(grad_topk_weights * topk_weights) with respect
+    to gating_output; counts and num_tokens come from `router_loss` (summed over the ranks of a data-parallel job), the routed weights
+    are those of `topk_softmax` / `topk_softmax_renorm`. grad_losses fp32 [2] and grad_topk_weights fp32 [T, k] may be None. Rows that
+    token_mask leaves out are zero. grad_logits must not share memory with gating_output."""
+    T, E, k = _router_args("router_backward", gating_output, topk_ids, token_mask)
+    _check("router_backward", gating_output.device, grad_logits=(grad_logits, gating_output.dtype, (T, E)),
+           counts=(counts, torch.int32, (E,)), num_tokens=(num_tokens, torch.int32, (1,)),
+           grad_losses=(grad_losses, torch.float32, (2,)), grad_topk_weights=(grad_topk_weights, torch.float32, (T, k)))
+    _launch(lib.moe_b200_router_backward, gating_output.device, grad_logits.data_ptr(), gating_output.data_ptr(),
+            gating_output.dtype == torch.bfloat16, topk_ids.data_ptr(), _ptr(counts), _ptr(num_tokens), _ptr(grad_losses),
+            _ptr(grad_topk_weights), _ptr(token_mask), T, E, k, bool(renormalize))
+
+
 def moe_align_block_size(topk_ids: torch.Tensor, num_experts: int, block_size: int, sorted_token_ids: torch.Tensor,
                          experts_ids: torch.Tensor, num_tokens_post_pad: torch.Tensor) -> None:
     """csrc/ops.cpp:53-60."""
@@ -263,6 +392,6 @@ __all__ = [
     "topk_softmax", "topk_softmax_renorm", "moe_align_block_size", "silu_and_mul", "swigluoai_and_mul", "moe_sum",
     "meta_size", "allocate_shared_buffer_and_handle", "open_mem_handle", "free_shared_buffer", "init_custom_ar",
     "dispose", "register_buffer", "all_reduce", "get_graph_buffer_ipc_meta", "register_graph_buffers",
-    "status_word", "read_status",
+    "status_word", "read_status", "rms_norm_quant_fp8", "add_rms_norm_quant_fp8", "w4_linear", "router_loss", "router_backward",
 ]
 _ = _lib

@@ -1,0 +1,313 @@
+"""Products with 4-bit weights and group scales, dense and over the routed experts, against the same products in 64 bits.
+
+Tolerances. A sum of K products in fp32, in any order and with a truncating adder, is off by at most (K / 16 + 64) * 2^-23 of
+sum |w x|: products of a tensor instruction are exact and added 16 at a time, and at most 64 further additions (groups, warps) follow.
+The output's rounding adds 2^-8 of the value. The experts' intermediate carries at least 16 significant bits (2^-16)."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16 = 2.0 ** -8
+
+
+def _gamma(K):
+    return (K / 16 + 64) * 2.0 ** -23
+
+
+def _weights(N, K, group, zeros, g, lead=()):
+    packed = torch.randint(0, 256, (*lead, N, K // 2), generator=g, dtype=torch.uint8)
+    scale = (0.01 * torch.exp(0.5 * torch.randn(*lead, N, K // group, generator=g))).to(torch.bfloat16)
+    zp = torch.randint(0, 16, (*lead, N, K // group), generator=g, dtype=torch.uint8) if zeros else None
+    return packed.cuda(), scale.cuda(), None if zp is None else zp.cuda()
+
+
+def _dense64(packed, scale, zp, group):
+    code = torch.stack((packed & 15, packed >> 4), -1).flatten(-2).double()
+    z = 8.0 if zp is None else zp.double().repeat_interleave(group, -1)
+    return (code - z) * scale.double().repeat_interleave(group, -1)
+
+
+def _linear(x, packed, scale, zp, bias=None):
+    from layered_prefill_b200 import ops
+    out = torch.full((*x.shape[:-1], packed.size(0)), float("nan"), dtype=torch.bfloat16, device="cuda")
+    ops.w4_linear(out, x, packed, scale, zp, bias)
+    return out
+
+
+def _check_linear(out, x, packed, scale, zp, bias=None):
+    group = 2 * packed.size(-1) // scale.size(-1)
+    w, x = _dense64(packed, scale, zp, group), x.double()
+    y = x @ w.t() + (0 if bias is None else bias.double())
+    bound = BF16 * y.abs() * 1.01 + _gamma(x.size(-1)) * (x.abs() @ w.abs().t() + (0 if bias is None else bias.double().abs()))
+    err = (out.double() - y).abs()
+    assert (err <= bound).all(), (err / bound).max()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 128), (1, 16, 256), (2, 17, 128), (1, 300, 2048), (3, 33, 384), (8, 64, 1024),
+                                   (9, 130, 640), (16, 257, 512), (17, 48, 2048), (31, 100, 896), (33, 65, 256), (70, 40, 384),
+                                   (1, 4099, 128), (5, 2048, 4096), (12, 1111, 8192)])
+def test_dense_shapes(M, N, K, group):
+    g = torch.Generator().manual_seed(M * 1000 + N + K + group)
+    zeros = (M + N) % 2 == 1
+    w = _weights(N, K, group, zeros, g)
+    x = torch.randn(M, K, generator=g).to(torch.bfloat16).cuda()
+    bias = torch.randn(N, generator=g).to(torch.bfloat16).cuda() if N % 3 == 0 else None
+    _check_linear(_linear(x, *w, bias), x, *w, bias)
+
+
+@pytest.mark.parametrize("K,group", [(32, 32), (64, 64), (96, 32), (160, 32), (192, 64), (1088, 64), (1184, 32), (4640, 32)])
+def test_dense_column_counts_that_fill_no_tile(K, group):
+    g = torch.Generator().manual_seed(K)
+    for M in (1, 6, 13):
+        w = _weights(77, K, group, True, g)
+        x = torch.randn(M, K, generator=g).to(torch.bfloat16).cuda()
+        _check_linear(_linear(x, *w), x, *w)
+
+
+def test_every_code_and_zero_point_is_exact():
+    """One column at a time: W itself comes back, and (code - zero) * scale fits bf16's roundings exactly for scale 1."""
+    codes = torch.arange(16, dtype=torch.uint8).repeat(16, 1)           # row z: codes 0..15
+    row = torch.cat([codes, codes.flip(1)], 1)                          # [16, 32]
+    packed = (row[:, 0::2] | (row[:, 1::2] << 4)).cuda()
+    zero = torch.arange(16, dtype=torch.uint8)[:, None].cuda()
+    scale = torch.ones(16, 1, dtype=torch.bfloat16).cuda()
+    x = torch.eye(32, dtype=torch.bfloat16).cuda()
+    out = _linear(x, packed, scale, zero)
+    assert torch.equal(out.t().float().cpu(), row.float() - torch.arange(16.0)[:, None])
+
+
+def test_leading_dimensions_row_strides_and_empty_batches():
+    from layered_prefill_b200 import ops
+    g = torch.Generator().manual_seed(3)
+    w = _weights(50, 256, 64, False, g)
+    x = torch.randn(2, 3, 256, generator=g).to(torch.bfloat16).cuda()
+    assert torch.equal(_linear(x, *w).view(6, 50), _linear(x.view(6, 256), *w))
+    wide = torch.randn(6, 512, generator=g).to(torch.bfloat16).cuda()
+    part = wide[:, 256:]
+    assert torch.equal(_linear(part, *w), _linear(part.contiguous(), *w))
+    ops.w4_linear(torch.empty(0, 50, dtype=torch.bfloat16, device="cuda"), x.view(6, 256)[:0], *w)
+
+
+def test_values_of_x_that_are_not_finite_reach_only_their_row():
+    g = torch.Generator().manual_seed(4)
+    w = _weights(40, 512, 128, True, g)
+    x = torch.randn(11, 512, generator=g).to(torch.bfloat16).cuda()
+    want = _linear(x, *w)
+    bad = x.clone()
+    bad[3, 100], bad[9, 0] = float("nan"), float("inf")
+    out = _linear(bad, *w)
+    rest = [i for i in range(11) if i not in (3, 9)]
+    assert torch.equal(out[rest], want[rest])
+    assert out[3].isnan().all() and (~out[9].isfinite()).all()
+
+
+def test_a_row_does_not_depend_on_the_batch_around_it():
+    g = torch.Generator().manual_seed(8)
+    w = _weights(96, 1024, 64, True, g)
+    x = torch.randn(40, 1024, generator=g).to(torch.bfloat16).cuda()
+    out = _linear(x, *w)
+    for m in (0, 7, 8, 39):
+        _check_linear(_linear(x[m:m + 1], *w), x[m:m + 1], *w)
+    assert torch.equal(out, _linear(x, *w))  # the same bits twice
+
+
+# ---------------------------------------------------------------------------------------------------- experts
+def _act64(gate, up, activation):
+    if activation == "silu":
+        return gate * torch.sigmoid(gate) * up
+    gate, up = gate.clamp(max=7.0), up.clamp(-7.0, 7.0)
+    return gate * torch.sigmoid(1.702 * gate) * (up + 1)
+
+
+def _experts64(x, w13, w2, b13, b2, tw, ti, group, activation):
+    """(out, bound) in 64 bits, slot by slot."""
+    T, H = x.shape
+    out = torch.zeros(T, H, dtype=torch.float64, device=x.device)
+    bound = torch.zeros_like(out)
+    E = w13[0].size(0)
+    for e in range(E):
+        t, j = torch.nonzero(ti == e, as_tuple=True)
+        if t.numel() == 0:
+            continue
+        a = _dense64(w13[0][e], w13[1][e], None if w13[2] is None else w13[2][e], group)
+        b = _dense64(w2[0][e], w2[1][e], None if w2[2] is None else w2[2][e], group)
+        xe = x[t].double()
+        gu = xe @ a.t() + (0 if b13 is None else b13[e].double())
+        dgu = _gamma(H) * (xe.abs() @ a.abs().t() + (0 if b13 is None else b13[e].double().abs()))
+        I = gu.size(1) // 2
+        cut = (lambda v: (v[:, :I], v[:, I:])) if activation == "silu" else (lambda v: (v[:, 0::2], v[:, 1::2]))
+        (gate, up), (dg, du) = cut(gu), cut(dgu)
+        h = _act64(gate, up, activation)
+        # slopes: |d act/d gate| <= 1.2 |up + 1|, |d act/d up| <= |gate|
+        dh = 1.2 * (up.abs() + 1) * dg + gate.abs() * du + 2.0 ** -16 * h.abs() + 2.0 ** -20 * gate.abs() * (up.abs() + 1)
+        y = h @ b.t() + (0 if b2 is None else b2[e].double())
+        dy = dh @ b.abs().t() + _gamma(I) * (h.abs() @ b.abs().t() + (0 if b2 is None else b2[e].double().abs()))
+        w = tw[t, j].double()[:, None]
+        out.index_add_(0, t, w * y)
+        bound.index_add_(0, t, w.abs() * dy + 2.0 ** -22 * (w * y).abs())
+    return out, bound + 1.01 * BF16 * out.abs()
+
+
+def _experts(x, w13, w2, tw, ti, group, b13=None, b2=None, activation="silu", inplace=False):
+    from layered_prefill_b200 import fused_moe
+    return fused_moe.fused_experts(x, w13[0], w2[0], b13, b2, tw, ti, inplace=inplace, activation=activation, w1_scale=w13[1],
+                                   w2_scale=w2[1], w1_zp=w13[2], w2_zp=w2[2], block_shape=[0, group])
+
+
+def _case(T, H, E, k, I, group, zeros, seed, skew=0.0):
+    g = torch.Generator().manual_seed(seed)
+    w13 = _weights(2 * I, H, group, zeros, g, (E,))
+    w2 = _weights(H, I, group, zeros, g, (E,))
+    x = torch.randn(T, H, generator=g).to(torch.bfloat16).cuda()
+    tw, ti = torch.topk(torch.softmax(torch.randn(T, E, generator=g) + skew * torch.randn(E, generator=g), -1), k, -1)
+    return x, w13, w2, tw.cuda(), ti.to(torch.int32).cuda()
+
+
+def _check_experts(out, *args):
+    want, bound = _experts64(*args)
+    err = (out.double() - want).abs()
+    assert (err <= bound).all(), (err / bound).max()
+
+
+@pytest.mark.parametrize("T,H,E,k,I,group", [
+    (1, 128, 8, 1, 64, 32), (1, 2048, 128, 8, 768, 128), (2, 256, 8, 2, 128, 128), (3, 512, 4, 4, 96, 32),
+    (7, 640, 16, 6, 192, 64), (17, 256, 60, 4, 160, 32), (64, 256, 16, 8, 128, 64), (64, 1024, 128, 8, 256, 128),
+    (100, 384, 8, 8, 256, 128), (200, 128, 8, 2, 64, 64), (33, 4096, 8, 2, 1536, 128), (9, 192, 3, 3, 64, 64), (5, 96, 8, 2, 32, 32)])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_expert_shapes(T, H, E, k, I, group, zeros):
+    x, w13, w2, tw, ti = _case(T, H, E, k, I, group, zeros, T + H + I)
+    _check_experts(_experts(x, w13, w2, tw, ti, group), x, w13, w2, None, None, tw, ti, group, "silu")
+
+
+@pytest.mark.parametrize("T", [1, 20, 150])
+def test_interleaved_activation_and_biases(T):
+    x, w13, w2, tw, ti = _case(T, 256, 8, 2, 128, 64, True, 5 + T)
+    g = torch.Generator().manual_seed(1)
+    b13 = torch.randn(8, 256, generator=g).to(torch.bfloat16).cuda()
+    b2 = torch.randn(8, 256, generator=g).to(torch.bfloat16).cuda()
+    for act in ("swigluoai", "silu"):
+        _check_experts(_experts(x, w13, w2, tw, ti, 64, b13, b2, act), x, w13, w2, b13, b2, tw, ti, 64, act)
+
+
+def test_one_expert_takes_every_token():
+    x, w13, w2, tw, ti = _case(90, 256, 8, 1, 128, 32, False, 2)
+    ti[:] = 5
+    _check_experts(_experts(x, w13, w2, tw, ti, 32), x, w13, w2, None, None, tw, ti, 32, "silu")
+
+
+def test_the_same_expert_twice_and_slots_without_one():
+    x, w13, w2, tw, ti = _case(12, 256, 8, 4, 128, 64, True, 3)
+    ti[:, 1] = ti[:, 0]          # the same expert twice for every token
+    ti[2, :] = -1                # a token without an expert
+    ti[4, 3] = 8                 # outside
+    ti[5, 0] = -7
+    out = _experts(x, w13, w2, tw, ti, 64)
+    _check_experts(out, x, w13, w2, None, None, tw, ti, 64, "silu")
+    assert (out[2] == 0).all()
+    ti[:] = -1
+    assert (_experts(x, w13, w2, tw, ti, 64) == 0).all()
+
+
+def test_in_place_empty_batch_and_other_index_types():
+    x, w13, w2, tw, ti = _case(10, 256, 8, 2, 128, 128, False, 4)
+    want = _experts(x, w13, w2, tw, ti, 128)
+    assert torch.equal(_experts(x, w13, w2, tw, ti.long(), 128), want)
+    y = x.clone()
+    assert _experts(y, w13, w2, tw, ti, 128, inplace=True).data_ptr() == y.data_ptr()
+    assert torch.equal(y, want)
+    assert _experts(x[:0], w13, w2, tw[:0], ti[:0], 128).shape == (0, 256)
+
+
+def test_experts_on_two_streams_at_once_and_in_two_graphs():
+    a, b = (_case(24, 512, 16, 4, 256, 64, True, s) for s in (21, 22))
+    want = [_experts(*c[:3], c[3], c[4], 64) for c in (a, b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(20):
+        for i, c in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i] = _experts(*c[:3], c[3], c[4], 64)
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in zip(want, got))
+    graphs, outs = [], []
+    for c in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(_experts(*c[:3], c[3], c[4], 64))
+        graphs.append(g)
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in zip(want, outs))
+
+
+def test_quantised_weights_come_near_the_bf16_block():
+    """A run of the operators as they are used: quant_w4 once, then norm -> router -> 4-bit experts -> 4-bit projection."""
+    from layered_prefill_b200 import fused_moe, linear, ops
+    T, H, E, k, I, g = 24, 512, 16, 4, 256, 64
+    gen = torch.Generator().manual_seed(2)
+    w13 = (torch.randn(E, 2 * I, H, generator=gen) * 0.05).cuda()
+    w2 = (torch.randn(E, H, I, generator=gen) * 0.05).cuda()
+    wg = (torch.randn(E, H, generator=gen) * 0.05).to(torch.bfloat16).cuda()
+    wo = torch.randn(H, 2 * H, generator=gen) * 0.05
+    q13, q2 = fused_moe.quant_w4(w13, g, True), fused_moe.quant_w4(w2, g, True)
+    attn = torch.randn(T, 2 * H, generator=gen).to(torch.bfloat16).cuda()
+    residual = torch.randn(T, H, generator=gen).to(torch.bfloat16).cuda()
+    o_proj = linear.W4RowParallelLinear(2 * H, H, group_size=g, zero_points=True)
+    for name, value in zip(("qweight", "scales", "zeros"), fused_moe.quant_w4(wo, g, True)):
+        p = getattr(o_proj, name)
+        p.weight_loader(p, value)
+    o_proj = o_proj.cuda()
+    y = o_proj(attn)
+    _check_linear(y, attn, o_proj.qweight, o_proj.scales, o_proj.zeros)
+    norm_w = torch.ones(H, dtype=torch.bfloat16, device="cuda")
+    normed, new_res = o_proj.forward_reduce_norm(attn, residual.clone(), norm_w, 1e-6)
+    q = torch.empty(T, H, dtype=torch.float8_e4m3fn, device="cuda")
+    s = torch.empty(T, H // 128, device="cuda")
+    hidden = torch.empty_like(residual)
+    ops.add_rms_norm_quant_fp8(q, s, residual, y, norm_w, 1e-6, normed_out=hidden)
+    assert torch.equal(residual, new_res)
+    logits = hidden @ wg.t()
+    tw, ti, balance, z, counts = fused_moe.fused_topk_with_loss(logits, k, True)
+    assert int(counts.sum()) == T * k and float(balance) >= 0.99 * k
+    got = fused_moe.fused_moe_forward_w4(hidden, logits, q13, q2, k, g)
+    _check_experts(got, hidden, q13, q2, None, None, tw, ti, g, "silu")
+    ref = fused_moe.fused_experts(hidden, w13.to(torch.bfloat16), w2.to(torch.bfloat16), None, None, tw, ti)
+    # each code is off by at most half a step of a range of 15 steps: with random errors 2 * sqrt(1/12) / (15 / 5.6) ~ 0.11 a matrix
+    assert (got.float() - ref.float()).norm() / ref.float().norm() < 0.3
+
+
+def test_refusals():
+    from layered_prefill_b200 import fused_moe, ops
+    from layered_prefill_b200._lib import MoeB200Error
+    g = torch.Generator().manual_seed(1)
+    q, s, z = _weights(32, 256, 64, True, g)
+    x = torch.randn(4, 256, generator=g).to(torch.bfloat16).cuda()
+    out = torch.empty(4, 32, dtype=torch.bfloat16, device="cuda")
+    for bad in (dict(input=x[:, :128]), dict(input=x.float()), dict(out=out[:3]), dict(qweight=q.t().contiguous().t()),
+                dict(scales=s.float()), dict(zeros=z[:, :1]), dict(zeros=z.cpu()), dict(bias=s[0]), dict(input=x.t())):
+        kw = {**dict(out=out, input=x, qweight=q, scales=s, zeros=z), **bad}
+        with pytest.raises(RuntimeError):
+            ops.w4_linear(**kw)
+    with pytest.raises(MoeB200Error):  # groups of 256
+        ops.w4_linear(out, x, q, s[:, :1].contiguous())
+    with pytest.raises(MoeB200Error):  # a row stride that breaks 16-byte rows
+        ops.w4_linear(out, torch.empty(4, 260, dtype=torch.bfloat16, device="cuda")[:, :256], q, s)
+    with pytest.raises(MoeB200Error):  # rows on top of each other
+        ops.w4_linear(out, x[:1].expand(4, 256), q, s)
+    with pytest.raises(MoeB200Error):  # a start between 16-byte boundaries
+        ops.w4_linear(out[:1], torch.empty(264, dtype=torch.bfloat16, device="cuda")[1:257].view(1, 256), q, s)
+    x, w13, w2, tw, ti = _case(4, 256, 8, 2, 128, 64, True, 1)
+    good = dict(w1_scale=w13[1], w2_scale=w2[1], w1_zp=w13[2], w2_zp=w2[2], block_shape=[0, 64])
+    for bad in (dict(w1_scale=None), dict(w1_zp=None), dict(block_shape=[0, 48]), dict(block_shape=[0, 128]),
+                dict(w1_scale=w13[1].float()), dict(a1_scale=tw), dict(expert_map=ti), dict(activation="gelu"),
+                dict(apply_router_weight_on_input=True), dict(w2_scale=w2[1][:, :, :1])):
+        with pytest.raises((ValueError, RuntimeError, NotImplementedError)):
+            fused_moe.fused_experts(x, w13[0], w2[0], None, None, tw, ti, **{**good, **bad})
+    with pytest.raises(RuntimeError):
+        fused_moe.fused_experts(x.float(), w13[0], w2[0], None, None, tw, ti, **good)
