@@ -8,12 +8,19 @@
 // 16-row operand and 8 tokens as columns (mma m16n8k16; tcgen05 wants its operand in shared or tensor memory, i.e. the
 // unpacked weights written out once more, four times the bytes that come in, for tiles that are 128 rows high). A code
 // becomes bf16 in two instructions for two codes: (w >> 4i) & 0x000f000f | 0x43004300 is the pair (128 + code_i, 128 + code_{i+4}) of an
-// eight-code word, minus (128 + zero) is exact. Products with x are exact in fp32; a group's sum is scaled in fp32.
-// The pairing (i, i + 4) is undone on the activations' side (four byte permutes per eight tokens and eight words).
+// eight-code word. The 128 and the zero point leave by the group's sum of x:
+//   sum (code - zero) x = sum (128 + code) x - (128 + zero) sum x
+// Products with x are exact and the sums are fp32, so the difference is off by some 2^-23 * 136 * sum |x|, a hundredth of what the
+// rounding of the output to bf16 costs.
 //
-// Work: a worker is kWk warps that split K; it takes tiles of 16 * kRB weight rows x up to 8 * kTB tokens in turn. Every warp
-// streams its 128-column chunks of codes and activations through a ring of its own with 16-byte cp.async, which runs on
-// into the next tile, so the warps never wait for one another inside a tile; the warps' sums meet in shared memory at its end.
+// Work: a tile is 16 * kRB weight rows x one block of up to 8 * kTB tokens; a CTA takes consecutive tiles, so that it
+// meets few token blocks. The activations of a window of them stay in shared memory, already in the order in which the pairs above
+// come, next to their group sums. A worker is 1 to 16 warps that split a tile's columns. Every warp streams codes through a
+// FIFO of its own (16-byte cp.async, four 128-column steps deep) that runs on into the next tile, so no warp waits for another
+// inside a window.
+#include <algorithm>
+#include <cmath>
+
 #include "launch.cuh"
 #include "moe_b200_internal.cuh"
 #include "ptx.cuh"
@@ -22,10 +29,13 @@ namespace moe_b200 {
 
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 16;
+constexpr int kThreads = 32 * kWarps;
 constexpr int kChunk = 128;         // columns of a step
+constexpr int kStages = 4;          // steps in a warp's FIFO
 constexpr int kListSlots = 1024;    // slots whose lists are built in shared memory
 constexpr int kListExperts = 1024;
+constexpr int kMaxSmem = 227 * 1024;
 
 enum W4Mode { kDense = 0, kGateUp = 1, kDown = 2 };
 
@@ -33,6 +43,9 @@ struct W4Params {
   W4Matrix w;
   int rows;               // weight rows of one matrix (dense N, 2 I, H)
   int K;
+  int span;               // columns whose activations are in shared memory at a time, a multiple of kChunk
+  int cap;                // token rows whose activations fit
+  int packed;             // the scales and zero points of a chunk can be read at once
   int wk_log2;            // log2 of the warps of a worker
   int row_tiles;
   const __nv_bfloat16* x;  // dense / gate_up: [tokens, K]; down: [slots][2][K], the high and the low part
@@ -62,22 +75,12 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-
-// Codes i and i + 4 of a word as bf16 minus the zero point; zz holds 128 + zero twice.
+// Codes i and i + 4 of a word as bf16, plus 128; one shift and one (a & b) | c, which two immediates would make two.
 template <int i>
-__device__ __forceinline__ uint32_t unpack(uint32_t w, uint32_t zz) {
-  return sub_bf16x2(((w >> (4 * i)) & 0x000f000fu) | 0x43004300u, zz);
-}
-
-__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ uint32_t unpack(uint32_t w, uint32_t mask, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w >> (4 * i)), "r"(mask), "r"(magic));
+  return r;
 }
 
 __device__ __forceinline__ float w4_act(float gate, float up, int activation) {
@@ -95,6 +98,7 @@ __device__ void build_lists(SlotLists& l, int* count, uint16_t* table, const int
   for (int e = lane; e < E; e += 32) row[e] = 0;
   __syncwarp();
   constexpr int kPer = kListSlots / (32 * kWarps);
+  static_assert(kPer * 32 * kWarps == kListSlots);
   int mine[kPer], pos[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
@@ -160,38 +164,40 @@ struct W4Shape {
   static constexpr int kParts = kMode == kDown ? 2 : 1;  // high and low part of the activations
   static constexpr int kRows = 16 * kRB;
   static constexpr int kTokens = 8 * kTB;
-  static constexpr int kA = kRows * 64;
-  static constexpr int kX = kTokens * 256;
-  static constexpr int kStage = kA + kParts * kX;
-  static constexpr int kStages = (24 * 1024) / kStage < 6 ? ((24 * 1024) / kStage < 3 ? 3 : (24 * 1024) / kStage) : 6;
+  static constexpr int kStage = kRows * 64;
   static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kRedLd = kRows + 4;  // floats between two tokens' sums: lanes (row g, tokens 2t) hit 32 banks
-  static constexpr int kRed = kWarps * kTokens * kRedLd * 4;
-  static constexpr int kLists = kMode == kDense ? 0 : static_cast<int>(sizeof(SlotLists)) + kListExperts * 4;
-  static constexpr int kSmem = kRing + kRed + (kLists + 15) / 16 * 16;
+  static constexpr int kRed = kWarps * kRB * kTB * 4 * 32 * 4;
+  static constexpr int kLists = kMode == kDense ? 0 : (static_cast<int>(sizeof(SlotLists)) + 15) / 16 * 16;
+  // a token row of `span` columns: 64 bytes more than a multiple of 128, so that the two tokens of an eight-lane phase of a
+  // 16-byte read use different banks
+  __host__ __device__ static constexpr int x_ld(int span) { return span * 2 + 64; }
+  __host__ __device__ static constexpr int x_row_bytes(int span, int gpc) { return kParts * x_ld(span) + span / kChunk * gpc * 4; }
+  static constexpr int kFixed = kRing + kRed + kLists;
 };
 
-// What a tile is: its token block's columns and the first weight row of each of its row blocks.
-struct Tile {
-  int n;        // tokens
-  int base;     // dense: first token; experts: first entry of the slot list
-  int row;      // first row of the tile (gate_up: first of its 8 * kRB intermediate columns)
-  long long mat;  // first row of the expert's matrix
-};
+// kGpc: groups in a chunk. Lane (g, t) = (lane / 4, lane % 4) of a warp holds row g and g + 8 of a row block; its word j of a
+// chunk of 128 columns starts at column col_of(j, t), so that the columns of a word index belong to one group.
+template <int kGpc>
+__device__ __forceinline__ int col_of(int j, int t) {
+  return kGpc == 1 ? 32 * t + 8 * j : (kGpc == 2 ? 64 * (j >> 1) + 16 * t + 8 * (j & 1) : 32 * j + 8 * t);
+}
 
-template <int kMode, int kRB, int kTB>
-__global__ void __launch_bounds__(32 * kWarps, 1) w4_mma_kernel(const W4Params p) {
+template <int kMode, int kRB, int kTB, int kGpc>
+__global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   using S = W4Shape<kMode, kRB, kTB>;
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int wk = 1 << p.wk_log2;
-  const int kw = warp & (wk - 1);                                        // this warp's share of K
-  const int worker = (blockIdx.x * kWarps + warp) >> p.wk_log2;
-  const int workers = (gridDim.x * kWarps) >> p.wk_log2;
-  const uint32_t ring = smem_u32(smem) + warp * (S::kStages * S::kStage);
-  float* red = reinterpret_cast<float*>(smem + S::kRing);
+  const int kw = warp & (wk - 1);             // this warp's share of the columns
+  const int worker = warp >> p.wk_log2;
+  const int workers = kWarps >> p.wk_log2;
+  uint8_t* const fifo = smem + warp * (kStages * S::kStage);
+  float* const red = reinterpret_cast<float*>(smem + S::kRing);
   SlotLists& lists = *reinterpret_cast<SlotLists*>(smem + S::kRing + S::kRed);
+  uint8_t* const x_mem = smem + S::kRing + S::kRed + S::kLists;
+  const int x_ld = S::x_ld(p.span);
+  float* const x_sum = reinterpret_cast<float*>(x_mem + S::kParts * p.cap * x_ld);  // [group][cap]
 
   grid_dependency_wait();
   grid_dependency_launch();
@@ -200,280 +206,393 @@ __global__ void __launch_bounds__(32 * kWarps, 1) w4_mma_kernel(const W4Params p
   if (kMode == kDense) {
     blocks = (p.m + S::kTokens - 1) / S::kTokens;
   } else {
-    static_assert(kMode == kDense || S::kRed >= kWarps * kListExperts * 2, "the table of the sort borrows the sums' place");
-    build_lists(lists, reinterpret_cast<int*>(&lists + 1), reinterpret_cast<uint16_t*>(red), p.ids, p.m, p.E, S::kTokens);
+    static_assert(kMode == kDense || S::kRing >= kWarps * kListExperts * 2 + kListExperts * 4, "the sort borrows the FIFOs' place");
+    build_lists(lists, reinterpret_cast<int*>(smem), reinterpret_cast<uint16_t*>(smem + kListExperts * 4), p.ids, p.m, p.E, S::kTokens);
     blocks = lists.blocks;
   }
-  const int tiles = blocks * p.row_tiles;
-  const int chunks = (p.K + kChunk - 1) / kChunk;
-  const int steps = (chunks - kw + wk - 1) >> p.wk_log2;  // of this warp in a tile
-  const int gpc_log2 = p.w.group == 128 ? 0 : (p.w.group == 64 ? 1 : 2);  // groups in a chunk
+  // this CTA's tiles, token block by token block
+  const long long total = static_cast<long long>(blocks) * p.row_tiles;
+  const int first = static_cast<int>(total * blockIdx.x / gridDim.x), last = static_cast<int>(total * (blockIdx.x + 1) / gridDim.x);
+  if (first == last) return;
+
+  const int spans = (p.K + p.span - 1) / p.span;
   const int groups = p.K / p.w.group;
-
-  auto tile_at = [&](int i) {
-    Tile r;
-    if (kMode == kDense) {
-      const int b = i % blocks;  // a row tile's token blocks follow each other: its weights come from L2 again
-      r.row = i / blocks * S::kRows;
-      r.base = b * S::kTokens;
-      r.n = min(S::kTokens, p.m - r.base);
-      r.mat = 0;
-    } else {
-      const int b = i / p.row_tiles;
-      r.row = i % p.row_tiles * (kMode == kGateUp ? S::kRows / 2 : S::kRows);
-      r.base = lists.start[b];
-      r.n = lists.count[b];
-      r.mat = static_cast<long long>(lists.expert[b]) * p.rows;
-    }
-    return r;
-  };
-  // weight row of row r (0 .. 15) of row block rb
-  auto weight_row = [&](const Tile& tile, int rb, int r) -> int {
-    if (kMode == kGateUp) {  // rows 0-7: gate of 8 columns of the intermediate, rows 8-15: up of the same columns
-      const int j = tile.row + rb * 8 + (r & 7);
-      return p.activation == 0 ? j + (r >> 3) * (p.rows >> 1) : 2 * j + (r >> 3);
-    }
-    return tile.row + rb * 16 + r;
-  };
-  auto x_row = [&](const Tile& tile, int n) -> const __nv_bfloat16* {
-    if (kMode == kDense) return p.x + static_cast<long long>(tile.base + n) * p.x_ld;
-    const int slot = lists.slots[tile.base + n];
-    return p.x + static_cast<long long>(kMode == kGateUp ? slot / p.top_k : slot) * p.x_ld;
-  };
-
-  // ------------------------------------------------------------------ loads of one step into the ring
-  int l_tile = worker, l_step = 0, l_slot = 0;
-  Tile lt = {};
-  const uint8_t* a_src[2 * kRB];
-  bool a_ok[2 * kRB];
-  const __nv_bfloat16* x_src[4 * kTB];
-  auto open_tile = [&]() {
-    if (l_tile >= tiles) return;
-    lt = tile_at(l_tile);
+  const uint32_t row_bytes = static_cast<uint32_t>(p.K) >> 1;
+  // Row r (0 .. 15) of row block rb lies rb * step_rb + (r / 8) * step_half + (r % 8) * step_row rows behind the tile's first.
+  // gate_up: rows 0-7 of a block are the gate of 8 columns of the intermediate, rows 8-15 their up.
+  const int step_row = kMode == kGateUp && p.activation != 0 ? 2 : 1;
+  const int step_half = kMode != kGateUp ? 8 : (p.activation == 0 ? p.rows >> 1 : 1);
+  const int step_rb = kMode == kGateUp ? 8 * step_row : 16;
+  // Rows past the end (of a matrix with fewer than kRows) are read as the last one, and not written.
+  const int row_lo = kMode == kGateUp ? g * step_row : min(g, p.rows - 1);
+  uint32_t q_off[2 * kRB], s_off[2 * kRB];  // of this lane's rows in bytes of codes and in groups, from row_lo on
 #pragma unroll
-    for (int i = 0; i < 2 * kRB; ++i) {
-      const int row = weight_row(lt, i >> 1, (i & 1) * 8 + g);
-      a_ok[i] = kMode == kGateUp || row < p.rows;
-      a_src[i] = p.w.q + (lt.mat + (a_ok[i] ? row : 0)) * (p.K >> 1) + t * 16;
-    }
-#pragma unroll
-    for (int i = 0; i < 4 * kTB; ++i) {
-      const int n = i * 2 + (lane >> 4);
-      x_src[i] = n < lt.n ? x_row(lt, n) + (lane & 15) * 8 : nullptr;
-    }
+  for (int i = 0; i < 2 * kRB; ++i) {
+    const int row = kMode == kGateUp ? (i >> 1) * step_rb + (i & 1) * step_half : min(8 * i + g, p.rows - 1) - row_lo;
+    q_off[i] = static_cast<uint32_t>(row) * row_bytes;
+    s_off[i] = static_cast<uint32_t>(row) * groups;
+  }
+  auto first_row = [&](int tile) -> int {
+    const int r = tile % p.row_tiles;
+    // the last tile takes rows of the one before again rather than rows past the end
+    return kMode == kGateUp ? r * (S::kRows / 2) : max(0, min(r * S::kRows, p.rows - S::kRows));
   };
+  auto first_row_of_matrix = [&](int block) -> long long {
+    return kMode == kDense ? 0 : static_cast<long long>(lists.expert[block]) * p.rows;
+  };
+  auto entries_of = [&](int block, int& base, int& n) {  // first entry (token, place in the slot list) and number of a block's
+    base = kMode == kDense ? block * S::kTokens : lists.start[block];
+    n = kMode == kDense ? min(S::kTokens, p.m - base) : lists.count[block];
+  };
+  const int last_block = (last - 1) / p.row_tiles;
+  auto window_end = [&](int block) {  // the blocks from `block` on whose activations fit together, those of this CTA
+    if (spans > 1) return block + 1;
+    int base, at, n;
+    entries_of(block, base, n);
+    int b = block + 1;
+    for (; b <= last_block; ++b) {
+      entries_of(b, at, n);
+      if (at + n - base > p.cap) break;
+    }
+    return b;
+  };
+  auto steps_of = [&](int span_i) {  // this warp's steps in a span
+    const int chunks = (min(p.span, p.K - span_i * p.span) + kChunk - 1) / kChunk;
+    return (chunks - kw + wk - 1) >> p.wk_log2;
+  };
+
+  // ------------------------------------------------------------------ codes: one step of this warp into its FIFO
+  int l_end_block = window_end(first / p.row_tiles), l_end = min(last, l_end_block * p.row_tiles);  // of the window
+  int l_tile = first + worker, l_span = 0, l_step = 0, l_steps = 0, l_slot = 0, l_col = 0;
+  const uint8_t* l_src = nullptr;
+  auto open = [&]() {  // (l_tile, l_span); a worker's tiles are `workers` apart inside a window
+    while (l_tile >= l_end) {
+      if (l_end == last) {
+        l_tile = last;
+        return;
+      }
+      l_tile = l_end + worker;
+      l_end_block = window_end(l_end_block);
+      l_end = min(last, l_end_block * p.row_tiles);
+    }
+    l_step = 0;
+    l_steps = steps_of(l_span);
+    l_col = l_span * p.span + kw * kChunk + t * 32;
+    l_src = p.w.q + (first_row_of_matrix(l_tile / p.row_tiles) + first_row(l_tile) * step_row + row_lo) * row_bytes + (l_col >> 1);
+  };
+  // 16-byte piece u of a row of 64 bytes is kept at u ^ swap: the reads below are free of bank conflicts at every width
+  const int swap = (g & 2) | ((g >> 2) & 1);
+  const uint32_t l_dst = smem_u32(fifo) + g * 64 + ((t ^ swap) * 16);
   auto load_step = [&]() {
-    if (l_tile < tiles) {
-      const int k0 = (kw + (l_step << p.wk_log2)) * kChunk;
-      const uint32_t dst = ring + l_slot * S::kStage;
-      const bool in_a = k0 + t * 32 < p.K;
+    if (l_tile < last) {
+      const uint32_t size = l_col < p.K ? 16 : 0;  // nothing is read, zeros are written behind the last column
 #pragma unroll
-      for (int i = 0; i < 2 * kRB; ++i) {
-        const int r = i * 8 + g;
-        cp_async_16(dst + r * 64 + ((t + (r >> 1)) & 3) * 16, in_a ? a_src[i] + (k0 >> 1) : p.w.q, in_a && a_ok[i] ? 16 : 0);
-      }
-      const bool in_x = k0 + (lane & 15) * 8 < p.K;
-#pragma unroll
-      for (int i = 0; i < 4 * kTB; ++i) {
-        if (i * 2 < lt.n || i < 4) {
-          const int n = i * 2 + (lane >> 4);
-          const bool ok = in_x && x_src[i] != nullptr;
-          const uint32_t at = dst + S::kA + n * 256 + (((lane & 15) ^ ((n & 1) * 4)) * 16);
-#pragma unroll
-          for (int part = 0; part < S::kParts; ++part)
-            cp_async_16(at + part * S::kX, ok ? x_src[i] + k0 + part * p.K : p.x, ok ? 16 : 0);
+      for (int i = 0; i < 2 * kRB; ++i) cp_async_16(l_dst + l_slot * S::kStage + i * 512, l_src + q_off[i], size);
+      l_src += (kChunk / 2) << p.wk_log2;
+      l_col += kChunk << p.wk_log2;
+      if (++l_step == l_steps) {
+        if (++l_span == spans) {
+          l_span = 0;
+          l_tile += workers;
         }
-      }
-      if (++l_step == steps) {
-        l_step = 0;
-        l_tile += workers;
-        open_tile();
+        open();
       }
     }
     cp_async_commit();
-    if (++l_slot == S::kStages) l_slot = 0;
+    l_slot = (l_slot + 1) & (kStages - 1);
   };
 
-  if (steps > 0) {
-    open_tile();
+  // ------------------------------------------------------------------ activations of entries and a span of columns
+  auto load_x = [&](int base, int n, int span_i) {
+    const int c0 = span_i * p.span;
+    const int chunks = (min(p.span, p.K - c0) + kChunk - 1) / kChunk;
+    // sixteen threads take the sixteen 8-column units of a chunk of a token
+    const int units = (n * chunks * 16 + 31) & ~31;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < units; i += kThreads) {
+      const int u = i & 15, row = min((i >> 4) / chunks, n - 1), c = (i >> 4) % chunks;
+      const int col = c0 + c * kChunk + col_of<kGpc>(u >> 2, u & 3);
+      long long r = base + row;
+      if (kMode == kGateUp) r = lists.slots[r] / p.top_k;
+      if (kMode == kDown) r = lists.slots[r];
+      float s = 0.f;
+#pragma unroll
+      for (int part = 0; part < S::kParts; ++part) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (col < p.K) v = *reinterpret_cast<const uint4*>(p.x + r * p.x_ld + part * p.K + col);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s += __uint_as_float(w[k] << 16) + __uint_as_float(w[k] & 0xffff0000u);
+        // (x0, x4), (x1, x5), (x2, x6), (x3, x7)
+        const uint4 o = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                                   __byte_perm(v.y, v.w, 0x7632));
+        *reinterpret_cast<uint4*>(x_mem + (part * p.cap + row) * x_ld + c * 256 + u * 16) = o;
+      }
+      // the sum over the units of a group: four threads hold a word index, two word indices a group of 64
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      if (kGpc < 4) s += __shfl_xor_sync(0xffffffffu, s, 4);
+      if (kGpc < 2) s += __shfl_xor_sync(0xffffffffu, s, 8);
+      constexpr int kUnits = 16 / kGpc;
+      if (u % kUnits == 0) x_sum[(c * kGpc + u / kUnits) * p.cap + row] = s;
+    }
+  };
+
+  open();
 #pragma unroll 1
-    for (int i = 0; i < S::kStages - 1; ++i) load_step();
-  }
+  for (int i = 0; i < kStages - 1; ++i) load_step();
 
   // ------------------------------------------------------------------ products
+  const uint32_t mask = 0x000f000fu, magic = 0x43004300u;
   int slot = 0;
-  for (int tile_i = worker; tile_i < tiles; tile_i += workers) {
-    const Tile tile = tile_at(tile_i);
-    const int nb = kTB == 1 ? 1 : (tile.n + 7) >> 3;
-    float tot[kRB][kTB][4];
+  for (int block0 = first / p.row_tiles; block0 <= last_block;) {
+    const int block1 = window_end(block0);
+    const int win_first = max(first, block0 * p.row_tiles), win_last = min(last, block1 * p.row_tiles);
+    const int rounds = (win_last - win_first + workers - 1) >> (4 - p.wk_log2);
+    int win_base, win_n, base, n_tokens;
+    entries_of(block0, win_base, win_n);
+    entries_of(block1 - 1, base, n_tokens);
+    win_n = base + n_tokens - win_base;
+    for (int round = 0; round < rounds; ++round) {
+      const int tile = win_first + worker + round * workers;
+      const bool active = tile < win_last;
+      const int block = min(tile / p.row_tiles, block1 - 1);
+      entries_of(block, base, n_tokens);
+      const int row0 = first_row(tile);
+      const long long mat = first_row_of_matrix(block);
+      // columns past the block's tokens are not written: they take the last one's activations
+      const uint8_t* x_lane[kTB];
+      const float* xs_lane[kTB][2];
 #pragma unroll
-    for (int rb = 0; rb < kRB; ++rb)
+      for (int tb = 0; tb < kTB; ++tb) {
+        x_lane[tb] = x_mem + (base - win_base + min(tb * 8 + g, n_tokens - 1)) * x_ld + t * 16 + kw * 256;
 #pragma unroll
-      for (int tb = 0; tb < kTB; ++tb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tot[rb][tb][i] = 0.f;
-    // scales and zero points: lane t of a quad fetches those of group t of the chunk for its rows, one step ahead
-    const __nv_bfloat16* s_src[2 * kRB];
-    const uint8_t* z_src[2 * kRB];
-#pragma unroll
-    for (int i = 0; i < 2 * kRB; ++i) {
-      const int row = weight_row(tile, i >> 1, (i & 1) * 8 + g);
-      const long long at = (tile.mat + (kMode == kGateUp || row < p.rows ? row : 0)) * groups;
-      s_src[i] = p.w.scale + at;
-      z_src[i] = p.w.zero + at;
-    }
-    float s_next[2 * kRB];
-    uint32_t z_next[2 * kRB];
-    auto fetch_scales = [&](int step) {
-      const int gi = ((kw + (step << p.wk_log2)) << gpc_log2) + (t & ((1 << gpc_log2) - 1));
-      const bool ok = step < steps && gi < groups;
-#pragma unroll
-      for (int i = 0; i < 2 * kRB; ++i) {
-        s_next[i] = ok ? __bfloat162float(s_src[i][gi]) : 0.f;
-        z_next[i] = ok && p.w.zero != nullptr ? (z_src[i][gi] & 15u) * 0x00010001u + 0x43004300u : 0x43084308u;
+        for (int o = 0; o < 2; ++o)
+          xs_lane[tb][o] = x_sum + kw * (kGpc * p.cap) + (base - win_base + min(tb * 8 + 2 * t + o, n_tokens - 1));
       }
-    };
-    fetch_scales(0);
-#pragma unroll 1
-    for (int step = 0; step < steps; ++step) {
-      cp_async_wait<S::kStages - 2>();
-      __syncwarp();
-      load_step();  // into the slot that the previous step has left
-      float s_cur[2 * kRB];
-      uint32_t z_cur[2 * kRB];
+      float tot[kRB][kTB][4];
 #pragma unroll
-      for (int i = 0; i < 2 * kRB; ++i) {
-        s_cur[i] = s_next[i];
-        z_cur[i] = z_next[i];
-      }
-      fetch_scales(step + 1);
-      const uint32_t src = ring + slot * S::kStage;
-      if (++slot == S::kStages) slot = 0;
-      float acc[kRB][kTB][4];
-      uint32_t zz[2 * kRB];
+      for (int rb = 0; rb < kRB; ++rb)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {  // 32 columns
-        const int per = 4 >> gpc_log2;  // of these in a group
-        if ((c & (per - 1)) == 0) {
-          const int from = (lane & ~3) | (c >> (2 - gpc_log2));
+        for (int tb = 0; tb < kTB; ++tb)
 #pragma unroll
-          for (int i = 0; i < 2 * kRB; ++i) zz[i] = __shfl_sync(0xffffffffu, z_cur[i], from);
-#pragma unroll
-          for (int rb = 0; rb < kRB; ++rb)
-#pragma unroll
-            for (int tb = 0; tb < kTB; ++tb)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) acc[rb][tb][i] = 0.f;
+          for (int i = 0; i < 4; ++i) tot[rb][tb][i] = 0.f;
+
+      for (int span_i = 0; span_i < spans; ++span_i) {
+        if (spans > 1 || round == 0) {
+          __syncthreads();  // the last readers of the previous activations are done
+          load_x(win_base, win_n, span_i);
+          __syncthreads();
         }
-        uint32_t b[S::kParts][kTB][4];
+        if (!active) continue;
+        const int steps = steps_of(span_i);
+        // scales and zero points of this lane's rows, fetched one step ahead
+        int gi = (span_i * p.span / kChunk + kw) * kGpc;
+        const long long s_at = (mat + row0 * step_row + row_lo) * groups + gi;
+        const __nv_bfloat16* s_src = p.w.scale + s_at;
+        const uint8_t* z_src = p.w.zero + s_at;
+        constexpr int kSWords = kGpc == 4 ? 2 : 1;
+        uint32_t s_next[2 * kRB][kSWords], z_next[2 * kRB];
+        auto fetch_scales = [&]() {
 #pragma unroll
-        for (int tb = 0; tb < kTB; ++tb) {
-          if (tb < nb) {
+          for (int i = 0; i < 2 * kRB; ++i) {
+            const __nv_bfloat16* sp = s_src + s_off[i];
+            const uint8_t* zp = z_src + s_off[i];
+            if (kGpc == 1) {
+              s_next[i][0] = *reinterpret_cast<const uint16_t*>(sp);
+              if (p.w.zero != nullptr) z_next[i] = *zp;
+            } else if (p.packed) {
+              if (kGpc == 2) {
+                s_next[i][0] = *reinterpret_cast<const uint32_t*>(sp);
+                if (p.w.zero != nullptr) z_next[i] = *reinterpret_cast<const uint16_t*>(zp);
+              } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(sp);
+                s_next[i][0] = v.x;
+                s_next[i][kSWords - 1] = v.y;
+                if (p.w.zero != nullptr) z_next[i] = *reinterpret_cast<const uint32_t*>(zp);
+              }
+            } else {
+              z_next[i] = 0;
 #pragma unroll
-            for (int part = 0; part < S::kParts; ++part) {
-              const uint4 v = ld_shared_v4(src + S::kA + part * S::kX + (tb * 8 + g) * 256 + (((c * 4 + t) ^ ((g & 1) * 4)) * 16));
-              b[part][tb][0] = __byte_perm(v.x, v.z, 0x5410);  // (x0, x4)
-              b[part][tb][1] = __byte_perm(v.x, v.z, 0x7632);  // (x1, x5)
-              b[part][tb][2] = __byte_perm(v.y, v.w, 0x5410);  // (x2, x6)
-              b[part][tb][3] = __byte_perm(v.y, v.w, 0x7632);  // (x3, x7)
-            }
-          }
-        }
+              for (int q = 0; q < kSWords; ++q) s_next[i][q] = 0;
 #pragma unroll
-        for (int rb = 0; rb < kRB; ++rb) {
-          const uint32_t at = src + (rb * 16 + g) * 64 + ((c + (g >> 1)) & 3) * 16 + t * 4;
-          const uint32_t lo = ld_shared_u32(at), hi = ld_shared_u32(at + 8 * 64);
-          const uint32_t zl = zz[2 * rb], zh = zz[2 * rb + 1];
-          const uint32_t a0 = unpack<0>(lo, zl), a1 = unpack<0>(hi, zh), a2 = unpack<1>(lo, zl), a3 = unpack<1>(hi, zh);
-          const uint32_t a4 = unpack<2>(lo, zl), a5 = unpack<2>(hi, zh), a6 = unpack<3>(lo, zl), a7 = unpack<3>(hi, zh);
-#pragma unroll
-          for (int tb = 0; tb < kTB; ++tb) {
-            if (tb < nb) {
-#pragma unroll
-              for (int part = 0; part < S::kParts; ++part) {
-                mma_bf16(acc[rb][tb], a0, a1, a2, a3, b[part][tb][0], b[part][tb][1]);
-                mma_bf16(acc[rb][tb], a4, a5, a6, a7, b[part][tb][2], b[part][tb][3]);
+              for (int q = 0; q < kGpc; ++q) {
+                if (gi + q < groups) {
+                  s_next[i][q / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(sp + q)) << (16 * (q & 1));
+                  if (p.w.zero != nullptr) z_next[i] |= static_cast<uint32_t>(zp[q]) << (8 * q);
+                }
               }
             }
           }
+          s_src += kGpc << p.wk_log2;
+          z_src += kGpc << p.wk_log2;
+          gi += kGpc << p.wk_log2;
+        };
+        fetch_scales();
+        const uint8_t* x_at[kTB];
+        const float* xs_at[kTB][2];
+#pragma unroll
+        for (int tb = 0; tb < kTB; ++tb) {
+          x_at[tb] = x_lane[tb];
+          xs_at[tb][0] = xs_lane[tb][0];
+          xs_at[tb][1] = xs_lane[tb][1];
         }
-        if ((c & (per - 1)) == per - 1) {
-          const int from = (lane & ~3) | (c >> (2 - gpc_log2));
+#pragma unroll 1
+        for (int step = 0; step < steps; ++step) {
+          cp_async_wait<kStages - 2>();
+          __syncwarp();
+          const uint8_t* const src = fifo + slot * S::kStage + g * 64;
+          slot = (slot + 1) & (kStages - 1);
+          uint32_t w[2 * kRB][4];
 #pragma unroll
-          for (int rb = 0; rb < kRB; ++rb) {
-            const float sl = __shfl_sync(0xffffffffu, s_cur[2 * rb], from), sh = __shfl_sync(0xffffffffu, s_cur[2 * rb + 1], from);
+          for (int i = 0; i < 2 * kRB; ++i) {
+            if (kGpc == 1) {
+              const uint4 v = *reinterpret_cast<const uint4*>(src + i * 512 + (t ^ swap) * 16);
+              w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
+            } else if (kGpc == 2) {
 #pragma unroll
-            for (int tb = 0; tb < kTB; ++tb) {
-              tot[rb][tb][0] = fmaf(acc[rb][tb][0], sl, tot[rb][tb][0]);
-              tot[rb][tb][1] = fmaf(acc[rb][tb][1], sl, tot[rb][tb][1]);
-              tot[rb][tb][2] = fmaf(acc[rb][tb][2], sh, tot[rb][tb][2]);
-              tot[rb][tb][3] = fmaf(acc[rb][tb][3], sh, tot[rb][tb][3]);
+              for (int h = 0; h < 2; ++h) {
+                const uint2 v = *reinterpret_cast<const uint2*>(src + i * 512 + ((2 * h + (t >> 1)) ^ swap) * 16 + (t & 1) * 8);
+                w[i][2 * h] = v.x; w[i][2 * h + 1] = v.y;
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) w[i][j] = *reinterpret_cast<const uint32_t*>(src + i * 512 + (j ^ swap) * 16 + t * 4);
+            }
+          }
+          load_step();  // into the slot that the previous step has left
+          uint32_t s_cur[2 * kRB][kSWords], z_cur[2 * kRB];
+#pragma unroll
+          for (int i = 0; i < 2 * kRB; ++i) {
+            z_cur[i] = z_next[i];
+#pragma unroll
+            for (int q = 0; q < kSWords; ++q) s_cur[i][q] = s_next[i][q];
+          }
+          if (step + 1 < steps) fetch_scales();
+          float acc[kRB][kTB][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            constexpr int kPer = 4 / kGpc;
+            if (j % kPer == 0) {
+#pragma unroll
+              for (int rb = 0; rb < kRB; ++rb)
+#pragma unroll
+                for (int tb = 0; tb < kTB; ++tb)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) acc[rb][tb][i] = 0.f;
+            }
+            uint4 b[S::kParts][kTB];
+#pragma unroll
+            for (int part = 0; part < S::kParts; ++part)
+#pragma unroll
+              for (int tb = 0; tb < kTB; ++tb)
+                b[part][tb] = *reinterpret_cast<const uint4*>(x_at[tb] + part * p.cap * x_ld + j * 64);
+#pragma unroll
+            for (int rb = 0; rb < kRB; ++rb) {
+              const uint32_t lo = w[2 * rb][j], hi = w[2 * rb + 1][j];
+              const uint32_t a0 = unpack<0>(lo, mask, magic), a1 = unpack<0>(hi, mask, magic);
+              const uint32_t a2 = unpack<1>(lo, mask, magic), a3 = unpack<1>(hi, mask, magic);
+              const uint32_t a4 = unpack<2>(lo, mask, magic), a5 = unpack<2>(hi, mask, magic);
+              const uint32_t a6 = unpack<3>(lo, mask, magic), a7 = unpack<3>(hi, mask, magic);
+#pragma unroll
+              for (int part = 0; part < S::kParts; ++part)
+#pragma unroll
+                for (int tb = 0; tb < kTB; ++tb) {
+                  mma_bf16(acc[rb][tb], a0, a1, a2, a3, b[part][tb].x, b[part][tb].y);
+                  mma_bf16(acc[rb][tb], a4, a5, a6, a7, b[part][tb].z, b[part][tb].w);
+                }
+            }
+            if (j % kPer == kPer - 1) {
+              constexpr int kLast = kPer - 1;
+              const int q = (j - kLast) / kPer;
+              float s[2 * kRB], z[2 * kRB];
+#pragma unroll
+              for (int i = 0; i < 2 * kRB; ++i) {
+                const uint32_t v = s_cur[i][q / 2];
+                s[i] = __uint_as_float(q & 1 ? v & 0xffff0000u : v << 16);
+                z[i] = -136.f;
+                if (p.w.zero != nullptr) z[i] = __uint_as_float(((z_cur[i] >> (8 * q)) & 15u) << 16 | 0xc3000000u);  // -(128 + zero)
+              }
+#pragma unroll
+              for (int tb = 0; tb < kTB; ++tb) {
+                const float xs[2] = {xs_at[tb][0][q * p.cap], xs_at[tb][1][q * p.cap]};
+#pragma unroll
+                for (int rb = 0; rb < kRB; ++rb)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const int r = 2 * rb + (i >> 1);
+                    tot[rb][tb][i] = fmaf(s[r], fmaf(z[r], xs[i & 1], acc[rb][tb][i]), tot[rb][tb][i]);
+                  }
+              }
+            }
+          }
+#pragma unroll
+          for (int tb = 0; tb < kTB; ++tb) {
+            x_at[tb] += 256 << p.wk_log2;
+            xs_at[tb][0] += (kGpc * p.cap) << p.wk_log2;
+            xs_at[tb][1] += (kGpc * p.cap) << p.wk_log2;
+          }
+        }
+      }
+
+      // -------------------------------------------------------------- the worker's warps meet
+      if (wk > 1) {
+        float* mine = red + warp * (kRB * kTB * 128) + lane;
+        if (kw != 0 && active) {
+#pragma unroll
+          for (int i = 0; i < kRB * kTB * 4; ++i) mine[i * 32] = tot[i / (4 * kTB)][i / 4 % kTB][i & 3];
+        }
+        __syncwarp();
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + worker), "r"(32 * wk) : "memory");
+        if (kw == 0 && active) {
+          for (int k = 1; k < wk; ++k)
+#pragma unroll
+            for (int i = 0; i < kRB * kTB * 4; ++i) tot[i / (4 * kTB)][i / 4 % kTB][i & 3] += mine[k * (kRB * kTB * 128) + i * 32];
+        }
+        __syncwarp();
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + worker), "r"(32 * wk) : "memory");
+      }
+      if (kw != 0 || !active) continue;
+      // -------------------------------------------------------------- epilogue: lane holds rows g, g + 8 of tokens 2t, 2t + 1
+#pragma unroll
+      for (int tb = 0; tb < kTB; ++tb)
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          const int n = tb * 8 + 2 * t + o;
+          if (n >= n_tokens) continue;
+          if (kMode == kGateUp) {
+            const int I = p.rows >> 1;
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + static_cast<long long>(lists.slots[base + n]) * 2 * I;
+#pragma unroll
+            for (int rb = 0; rb < kRB; ++rb) {
+              const int j = row0 + rb * 8 + g;
+              float gate = tot[rb][tb][o], up = tot[rb][tb][2 + o];
+              if (p.w.bias != nullptr) {
+                gate += __bfloat162float(p.w.bias[mat + j * step_row]);
+                up += __bfloat162float(p.w.bias[mat + j * step_row + step_half]);
+              }
+              const float v = w4_act(gate, up, p.activation);
+              const __nv_bfloat16 v_hi = __float2bfloat16_rn(v);
+              dst[j] = v_hi;
+              dst[I + j] = __float2bfloat16_rn(v - __bfloat162float(v_hi));
+            }
+          } else {
+            const int s = kMode == kDense ? base + n : lists.slots[base + n];
+            const float scale = kMode == kDense ? 1.f : p.topk_w[s];
+#pragma unroll
+            for (int i = 0; i < 2 * kRB; ++i) {
+              const int row = row0 + i * 8 + g;
+              if (row >= p.rows) continue;
+              float y = tot[i >> 1][tb][2 * (i & 1) + o];
+              if (p.w.bias != nullptr) y += __bfloat162float(p.w.bias[mat + row]);
+              const long long at = static_cast<long long>(s) * p.rows + row;
+              if (kMode == kDense) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
+              else static_cast<float*>(p.out)[at] = y * scale;
             }
           }
         }
-      }
     }
-
-    // ---------------------------------------------------------------- the worker's warps meet; epilogue
-    auto worker_sync = [&]() {
-      __syncwarp();
-      if (wk > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + (warp >> p.wk_log2)), "r"(32 * wk) : "memory");
-    };
-    float* mine = red + warp * (S::kTokens * S::kRedLd);
-#pragma unroll
-    for (int rb = 0; rb < kRB; ++rb)
-#pragma unroll
-      for (int tb = 0; tb < kTB; ++tb) {
-        float* q = mine + (tb * 8 + 2 * t) * S::kRedLd + rb * 16 + g;
-        q[0] = tot[rb][tb][0];
-        q[S::kRedLd] = tot[rb][tb][1];
-        q[8] = tot[rb][tb][2];
-        q[S::kRedLd + 8] = tot[rb][tb][3];
-      }
-    worker_sync();
-    const float* all = red + (warp - kw) * (S::kTokens * S::kRedLd);
-    auto sum_at = [&](int n, int r) {
-      float s = 0.f;
-      for (int i = 0; i < wk; ++i) s += all[(i * S::kTokens + n) * S::kRedLd + r];
-      return s;
-    };
-    const int th = kw * 32 + lane;
-    if (kMode == kGateUp) {
-      constexpr int kCols = S::kRows / 2;
-      const int I = p.rows >> 1;
-      __nv_bfloat16* h = static_cast<__nv_bfloat16*>(p.out);
-      for (int i = th; i < tile.n * kCols; i += 32 * wk) {
-        const int n = i / kCols, jj = i % kCols, j = tile.row + jj;
-        if (j < I) {
-          const int r = (jj >> 3) * 16 + (jj & 7);
-          float gate = sum_at(n, r), up = sum_at(n, r + 8);
-          if (p.w.bias != nullptr) {
-            gate += __bfloat162float(p.w.bias[tile.mat + weight_row(tile, jj >> 3, jj & 7)]);
-            up += __bfloat162float(p.w.bias[tile.mat + weight_row(tile, jj >> 3, 8 + (jj & 7))]);
-          }
-          const float v = w4_act(gate, up, p.activation);
-          const __nv_bfloat16 v_hi = __float2bfloat16_rn(v);
-          __nv_bfloat16* dst = h + static_cast<long long>(lists.slots[tile.base + n]) * 2 * I + j;
-          dst[0] = v_hi;
-          dst[I] = __float2bfloat16_rn(v - __bfloat162float(v_hi));
-        }
-      }
-    } else {
-      for (int i = th; i < tile.n * S::kRows; i += 32 * wk) {
-        const int n = i / S::kRows, r = i % S::kRows, row = tile.row + r;
-        if (row < p.rows) {
-          float y = sum_at(n, r);
-          if (p.w.bias != nullptr) y += __bfloat162float(p.w.bias[tile.mat + row]);
-          if (kMode == kDense) {
-            static_cast<__nv_bfloat16*>(p.out)[static_cast<long long>(tile.base + n) * p.rows + row] = __float2bfloat16_rn(y);
-          } else {
-            const int s = lists.slots[tile.base + n];
-            static_cast<float*>(p.out)[static_cast<long long>(s) * p.rows + row] = y * p.topk_w[s];
-          }
-        }
-      }
-    }
-    worker_sync();
+    block0 = block1;
   }
   cp_async_wait_all();
 }
@@ -501,24 +620,62 @@ w4_sum_kernel(__nv_bfloat16* __restrict__ out, const float* __restrict__ c3, con
   *reinterpret_cast<uint2*>(out + static_cast<long long>(t) * H + n) = o;
 }
 
-// Warps of a worker: all eight while the tiles are too few to keep as many workers busy, fewer when there are many.
-int pick_wk_log2(long long tiles, int chunks, int sms) {
-  int lg = 3;
-  while (lg > 0 && ((1 << lg) > chunks || tiles >= static_cast<long long>(sms) * (kWarps >> lg) * 8)) --lg;
-  return lg;
+// Token blocks that evenly spread slots come to; a guess, for the split of the work only.
+int expected_blocks(int slots, int E) {
+  const double active = E * (1.0 - std::exp(-static_cast<double>(slots) / E));
+  const double full = (slots - 4.0 * active) / 8.0;
+  const int b = static_cast<int>(active + (full > 0 ? full : 0.0));
+  return b < 1 ? 1 : b;
+}
+
+// Warps of a worker: the split with the fewest steps in a row. A window ends with half a round of idle workers on
+// average, and a tile's end is counted as one more step.
+int pick_wk_log2(long long tiles, int ctas, int chunks, double windows) {
+  int best = 0;
+  double best_cost = -1;
+  for (int lg = 0; lg <= 4 && (1 << lg) <= chunks; ++lg) {
+    const int workers = kWarps >> lg;
+    const double tiles_in_row = std::max(1.0, static_cast<double>(tiles) / ctas / workers + 0.5 * windows);
+    const double cost = tiles_in_row * ((chunks + (1 << lg) - 1) / (1 << lg) + 1);
+    if (best_cost < 0 || cost < best_cost) {
+      best = lg;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+
+template <int kMode, int kRB, int kTB, int kGpc>
+cudaError_t launch_groups(W4Params p, long long tiles, cudaStream_t stream) {
+  using S = W4Shape<kMode, kRB, kTB>;
+  constexpr int kRoom = kMaxSmem - S::kFixed;
+  static_assert(kRoom / S::x_row_bytes(8 * kChunk, kGpc) >= S::kTokens);
+  auto kernel = w4_mma_kernel<kMode, kRB, kTB, kGpc>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+  if (e != cudaSuccess) return e;
+  const int sms = device_sm_count();
+  const int chunks = (p.K + kChunk - 1) / kChunk;
+  int spans = 1;  // as few equal spans as leave room for a block's tokens
+  while (kRoom / S::x_row_bytes((chunks + spans - 1) / spans * kChunk, kGpc) < S::kTokens) ++spans;
+  const int span_chunks = (chunks + spans - 1) / spans;
+  p.span = span_chunks * kChunk;
+  const int entries = std::min(p.m, kMode == kDense ? p.m : kListSlots);
+  p.cap = std::min(kRoom / S::x_row_bytes(p.span, kGpc), std::max(entries, 1));
+  p.packed = p.K % kChunk == 0 && reinterpret_cast<uintptr_t>(p.w.scale) % (2 * kGpc) == 0 && reinterpret_cast<uintptr_t>(p.w.zero) % kGpc == 0;
+  const int ctas = static_cast<int>(tiles < sms ? tiles : sms);
+  const int last_chunks = chunks - (chunks - 1) / span_chunks * span_chunks;  // every warp has a step in every span
+  const double windows = spans > 1 ? static_cast<double>(tiles) / p.row_tiles / ctas + 1 : 1 + static_cast<double>(entries) / ctas / p.cap;
+  p.wk_log2 = pick_wk_log2(tiles, ctas, std::min(last_chunks, span_chunks), windows);
+  return launch_pdl(kernel, dim3(ctas), dim3(kThreads), S::kFixed + p.cap * S::x_row_bytes(p.span, kGpc), stream, p);
 }
 
 template <int kMode, int kRB, int kTB>
-cudaError_t launch_shape(W4Params p, long long tiles, cudaStream_t stream) {
-  using S = W4Shape<kMode, kRB, kTB>;
-  static_assert(S::kSmem <= 227 * 1024, "ring, sums and lists have to fit an SM's shared memory");
-  auto kernel = w4_mma_kernel<kMode, kRB, kTB>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-  if (e != cudaSuccess) return e;
-  const int sms = device_sm_count();
-  p.wk_log2 = pick_wk_log2(tiles, (p.K + kChunk - 1) / kChunk, sms);
-  const long long ctas = (tiles * (1 << p.wk_log2) + kWarps - 1) / kWarps;
-  return launch_pdl(kernel, dim3(static_cast<unsigned>(ctas < sms ? ctas : sms)), dim3(32 * kWarps), S::kSmem, stream, p);
+cudaError_t launch_shape(W4Params p, int rows, long long blocks, cudaStream_t stream) {
+  p.row_tiles = (rows + 16 * kRB - 1) / (16 * kRB);
+  const long long tiles = blocks * p.row_tiles;
+  if (p.w.group == 128) return launch_groups<kMode, kRB, kTB, 1>(p, tiles, stream);
+  if (p.w.group == 64) return launch_groups<kMode, kRB, kTB, 2>(p, tiles, stream);
+  return launch_groups<kMode, kRB, kTB, 4>(p, tiles, stream);
 }
 
 }  // namespace
@@ -527,14 +684,14 @@ int launch_w4_linear(__nv_bfloat16* out, const __nv_bfloat16* x, long long x_ld,
   if (M == 0) return kStatusOk;
   W4Params p{};
   p.w = w; p.rows = N; p.K = K; p.x = x; p.x_ld = x_ld; p.m = M; p.out = out;
-  const int rb = N <= 64 * device_sm_count() ? 2 : 4;
-  p.row_tiles = (N + 16 * rb - 1) / (16 * rb);
   const int tb = M <= 8 ? 1 : 2;
-  const long long tiles = static_cast<long long>(p.row_tiles) * ((M + 8 * tb - 1) / (8 * tb));
-  if (tiles > 0x3fffffffll) return set_error(kStatusInvalidArgument, "w4_linear: M x N too large");
+  const long long blocks = (M + 8 * tb - 1) / (8 * tb);
+  if (blocks * ((N + 15) / 16) > 0x3fffffffll) return set_error(kStatusInvalidArgument, "w4_linear: M x N too large");
+  const int sms = device_sm_count();
   cudaError_t e;
-  if (rb == 2) e = tb == 1 ? launch_shape<kDense, 2, 1>(p, tiles, stream) : launch_shape<kDense, 2, 2>(p, tiles, stream);
-  else e = tb == 1 ? launch_shape<kDense, 4, 1>(p, tiles, stream) : launch_shape<kDense, 4, 2>(p, tiles, stream);
+  // 16-row tiles while 32-row ones would leave SMs without work
+  if (blocks * ((N + 31) / 32) < sms) e = tb == 1 ? launch_shape<kDense, 1, 1>(p, N, blocks, stream) : launch_shape<kDense, 1, 2>(p, N, blocks, stream);
+  else e = tb == 1 ? launch_shape<kDense, 2, 1>(p, N, blocks, stream) : launch_shape<kDense, 2, 2>(p, N, blocks, stream);
   if (int st = check_cuda(e, "w4_linear launch")) return st;
   count_launches(1);
   return check_launch("w4_linear");
@@ -551,6 +708,7 @@ int launch_w4_experts(__nv_bfloat16* out, const __nv_bfloat16* x, const W4Matrix
                       cudaStream_t stream) {
   if (E > kListExperts || top_k > kListSlots)
     return set_error(kStatusInvalidArgument, "fused_experts_w4: at most %d experts and %d slots a token", kListExperts, kListSlots);
+  if (static_cast<long long>(I) * H >= 1ll << 32) return set_error(kStatusInvalidArgument, "fused_experts_w4: an expert's matrix is too large (H=%d I=%d)", H, I);
   const int piece = kListSlots / top_k;  // tokens whose slots fit the lists in shared memory
   for (int t0 = 0; t0 < T; t0 += piece) {
     const int tt = T - t0 < piece ? T - t0 : piece;
@@ -558,17 +716,13 @@ int launch_w4_experts(__nv_bfloat16* out, const __nv_bfloat16* x, const W4Matrix
     const int* ids = topk_ids + static_cast<long long>(t0) * top_k;
     __nv_bfloat16* h = static_cast<__nv_bfloat16*>(workspace);
     float* c3 = reinterpret_cast<float*>(h + static_cast<size_t>(slots) * 2 * I);
-    const int active = slots < E ? slots : E;
+    const int blocks = expected_blocks(slots, E);
     W4Params p{};
     p.w = w13; p.rows = 2 * I; p.K = H; p.x = x + static_cast<long long>(t0) * H; p.x_ld = H; p.m = slots; p.ids = ids; p.top_k = top_k;
     p.E = E; p.activation = activation; p.out = h;
-    p.row_tiles = (I + 31) / 32;
-    long long tiles = static_cast<long long>(active) * p.row_tiles;
-    if (int st = check_cuda(launch_shape<kGateUp, 4, 1>(p, tiles, stream), "w4 gate_up launch")) return st;
+    if (int st = check_cuda(launch_shape<kGateUp, 2, 1>(p, 2 * I, blocks, stream), "w4 gate_up launch")) return st;
     p.w = w2; p.rows = H; p.K = I; p.x = h; p.x_ld = 2 * I; p.topk_w = topk_w + static_cast<long long>(t0) * top_k; p.out = c3;
-    p.row_tiles = (H + 63) / 64;
-    tiles = static_cast<long long>(active) * p.row_tiles;
-    if (int st = check_cuda(launch_shape<kDown, 4, 1>(p, tiles, stream), "w4 down launch")) return st;
+    if (int st = check_cuda(launch_shape<kDown, 2, 1>(p, H, blocks, stream), "w4 down launch")) return st;
     if (int st = check_cuda(launch_pdl(w4_sum_kernel, dim3((H / 4 + 255) / 256, tt), dim3(256), 0, stream,
                                        out + static_cast<long long>(t0) * H, c3, ids, E, top_k, H), "w4 sum launch"))
       return st;
