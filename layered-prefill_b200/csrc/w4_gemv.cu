@@ -20,6 +20,7 @@
 // inside a window.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "launch.cuh"
 #include "moe_b200_internal.cuh"
@@ -45,6 +46,7 @@ struct W4Params {
   int K;
   int span;               // columns whose activations are in shared memory at a time, a multiple of kChunk
   int cap;                // token rows whose activations fit
+  int whole;              // K is a multiple of kChunk
   int packed;             // the scales and zero points of a chunk can be read at once
   int wk_log2;            // log2 of the warps of a worker
   int row_tiles;
@@ -69,10 +71,16 @@ struct SlotLists {
 };
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same with nothing in the accumulator yet.
+__device__ __forceinline__ void mma_bf16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // Codes i and i + 4 of a word as bf16, plus 128; one shift and one (a & b) | c, which two immediates would make two.
@@ -81,6 +89,26 @@ __device__ __forceinline__ uint32_t unpack(uint32_t w, uint32_t mask, uint32_t m
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w >> (4 * i)), "r"(mask), "r"(magic));
   return r;
+}
+
+// Reads of the FIFO, at a constant distance behind an address; volatile, for they must stay behind the wait for their copy.
+template <int kOff>
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4+%5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr), "n"(kOff) : "memory");
+  return v;
+}
+template <int kOff>
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2+%3];" : "=r"(v.x), "=r"(v.y) : "r"(addr), "n"(kOff) : "memory");
+  return v;
+}
+template <int kOff>
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1+%2];" : "=r"(v) : "r"(addr), "n"(kOff) : "memory");
+  return v;
 }
 
 __device__ __forceinline__ float w4_act(float gate, float up, int activation) {
@@ -171,7 +199,7 @@ struct W4Shape {
   // a token row of `span` columns: 64 bytes more than a multiple of 128, so that the two tokens of an eight-lane phase of a
   // 16-byte read use different banks
   __host__ __device__ static constexpr int x_ld(int span) { return span * 2 + 64; }
-  __host__ __device__ static constexpr int x_row_bytes(int span, int gpc) { return kParts * x_ld(span) + span / kChunk * gpc * 4; }
+  __host__ __device__ static constexpr int x_row_bytes(int span, int gpc) { return kParts * x_ld(span) + (span / kChunk * gpc | 1) * 4; }
   static constexpr int kFixed = kRing + kRed + kLists;
 };
 
@@ -197,7 +225,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   SlotLists& lists = *reinterpret_cast<SlotLists*>(smem + S::kRing + S::kRed);
   uint8_t* const x_mem = smem + S::kRing + S::kRed + S::kLists;
   const int x_ld = S::x_ld(p.span);
-  float* const x_sum = reinterpret_cast<float*>(x_mem + S::kParts * p.cap * x_ld);  // [group][cap]
+  float* const x_sum = reinterpret_cast<float*>(x_mem + S::kParts * p.cap * x_ld);  // [cap][groups, an odd number of floats]
+  const int xs_ld = p.span / kChunk * kGpc | 1;
 
   grid_dependency_wait();
   grid_dependency_launch();
@@ -256,15 +285,16 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
     }
     return b;
   };
-  auto steps_of = [&](int span_i) {  // this warp's steps in a span
+  auto chunks_of = [&](int span_i, int& begin, int& n) {  // this warp's chunks of a span
     const int chunks = (min(p.span, p.K - span_i * p.span) + kChunk - 1) / kChunk;
-    return (chunks - kw + wk - 1) >> p.wk_log2;
+    begin = (kw * chunks) >> p.wk_log2;
+    n = (((kw + 1) * chunks) >> p.wk_log2) - begin;
   };
 
   // ------------------------------------------------------------------ codes: one step of this warp into its FIFO
   int l_end_block = window_end(first / p.row_tiles), l_end = min(last, l_end_block * p.row_tiles);  // of the window
-  int l_tile = first + worker, l_span = 0, l_step = 0, l_steps = 0, l_slot = 0, l_col = 0;
-  const uint8_t* l_src = nullptr;
+  int l_tile = first + worker, l_span = 0, l_left = 0, l_col = 0;
+  const uint8_t* l_src[2 * kRB];
   auto open = [&]() {  // (l_tile, l_span); a worker's tiles are `workers` apart inside a window
     while (l_tile >= l_end) {
       if (l_end == last) {
@@ -275,31 +305,39 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
       l_end_block = window_end(l_end_block);
       l_end = min(last, l_end_block * p.row_tiles);
     }
-    l_step = 0;
-    l_steps = steps_of(l_span);
-    l_col = l_span * p.span + kw * kChunk + t * 32;
-    l_src = p.w.q + (first_row_of_matrix(l_tile / p.row_tiles) + first_row(l_tile) * step_row + row_lo) * row_bytes + (l_col >> 1);
+    int begin;
+    chunks_of(l_span, begin, l_left);
+    l_col = l_span * p.span + begin * kChunk + t * 32;
+    const uint8_t* src = p.w.q + (first_row_of_matrix(l_tile / p.row_tiles) + first_row(l_tile) * step_row + row_lo) * row_bytes + (l_col >> 1);
+#pragma unroll
+    for (int i = 0; i < 2 * kRB; ++i) l_src[i] = src + q_off[i];
   };
   // 16-byte piece u of a row of 64 bytes is kept at u ^ swap: the reads below are free of bank conflicts at every width
   const int swap = (g & 2) | ((g >> 2) & 1);
   const uint32_t l_dst = smem_u32(fifo) + g * 64 + ((t ^ swap) * 16);
-  auto load_step = [&]() {
-    if (l_tile < last) {
-      const uint32_t size = l_col < p.K ? 16 : 0;  // nothing is read, zeros are written behind the last column
+  // Chunk kSlot of four; a tile's chunks begin at slot 0, and what is missing to a multiple of four stays empty.
+  auto load_chunk = [&](auto slot_c) {
+    constexpr int kSlot = decltype(slot_c)::value;
+    if (kSlot < l_left) {
+      const uint32_t size = p.whole || l_col + kSlot * kChunk < p.K ? 16 : 0;  // zeros are written behind the last column
 #pragma unroll
-      for (int i = 0; i < 2 * kRB; ++i) cp_async_16(l_dst + l_slot * S::kStage + i * 512, l_src + q_off[i], size);
-      l_src += (kChunk / 2) << p.wk_log2;
-      l_col += kChunk << p.wk_log2;
-      if (++l_step == l_steps) {
+      for (int i = 0; i < 2 * kRB; ++i) cp_async_16(l_dst + kSlot * S::kStage + i * 512, l_src[i] + kSlot * (kChunk / 2), size);
+    }
+    cp_async_commit();
+    if (kSlot == kStages - 1) {
+      l_left -= kStages;
+      l_col += kStages * kChunk;
+#pragma unroll
+      for (int i = 0; i < 2 * kRB; ++i) l_src[i] += kStages * kChunk / 2;
+      if (l_left <= 0 && l_tile < last) {
         if (++l_span == spans) {
           l_span = 0;
           l_tile += workers;
         }
+        l_left = 0;
         open();
       }
     }
-    cp_async_commit();
-    l_slot = (l_slot + 1) & (kStages - 1);
   };
 
   // ------------------------------------------------------------------ activations of entries and a span of columns
@@ -334,17 +372,18 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
       if (kGpc < 4) s += __shfl_xor_sync(0xffffffffu, s, 4);
       if (kGpc < 2) s += __shfl_xor_sync(0xffffffffu, s, 8);
       constexpr int kUnits = 16 / kGpc;
-      if (u % kUnits == 0) x_sum[(c * kGpc + u / kUnits) * p.cap + row] = s;
+      if (u % kUnits == 0) x_sum[row * xs_ld + c * kGpc + u / kUnits] = s;
     }
   };
 
   open();
-#pragma unroll 1
-  for (int i = 0; i < kStages - 1; ++i) load_step();
+  load_chunk(std::integral_constant<int, 0>{});
+  load_chunk(std::integral_constant<int, 1>{});
+  load_chunk(std::integral_constant<int, 2>{});
 
   // ------------------------------------------------------------------ products
   const uint32_t mask = 0x000f000fu, magic = 0x43004300u;
-  int slot = 0;
+  const uint32_t fifo_lane = smem_u32(fifo) + g * 64;
   for (int block0 = first / p.row_tiles; block0 <= last_block;) {
     const int block1 = window_end(block0);
     const int win_first = max(first, block0 * p.row_tiles), win_last = min(last, block1 * p.row_tiles);
@@ -365,10 +404,10 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
       const float* xs_lane[kTB][2];
 #pragma unroll
       for (int tb = 0; tb < kTB; ++tb) {
-        x_lane[tb] = x_mem + (base - win_base + min(tb * 8 + g, n_tokens - 1)) * x_ld + t * 16 + kw * 256;
+        x_lane[tb] = x_mem + (base - win_base + min(tb * 8 + g, n_tokens - 1)) * x_ld + t * 16;
 #pragma unroll
         for (int o = 0; o < 2; ++o)
-          xs_lane[tb][o] = x_sum + kw * (kGpc * p.cap) + (base - win_base + min(tb * 8 + 2 * t + o, n_tokens - 1));
+          xs_lane[tb][o] = x_sum + (base - win_base + min(tb * 8 + 2 * t + o, n_tokens - 1)) * xs_ld;
       }
       float tot[kRB][kTB][4];
 #pragma unroll
@@ -385,19 +424,23 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
           __syncthreads();
         }
         if (!active) continue;
-        const int steps = steps_of(span_i);
-        // scales and zero points of this lane's rows, fetched one step ahead
-        int gi = (span_i * p.span / kChunk + kw) * kGpc;
+        int begin, left;
+        chunks_of(span_i, begin, left);
+        // scales and zero points of this lane's rows, fetched one chunk ahead
+        int gi = (span_i * p.span / kChunk + begin) * kGpc;
         const long long s_at = (mat + row0 * step_row + row_lo) * groups + gi;
-        const __nv_bfloat16* s_src = p.w.scale + s_at;
+        const __nv_bfloat16* s_src[2 * kRB];
+#pragma unroll
+        for (int i = 0; i < 2 * kRB; ++i) s_src[i] = p.w.scale + s_at + s_off[i];
         const uint8_t* z_src = p.w.zero + s_at;
         constexpr int kSWords = kGpc == 4 ? 2 : 1;
         uint32_t s_next[2 * kRB][kSWords], z_next[2 * kRB];
-        auto fetch_scales = [&]() {
+        auto fetch_scales = [&](auto ahead_c) {  // of the chunk so many chunks behind s_src
+          constexpr int kAhead = decltype(ahead_c)::value * kGpc;
 #pragma unroll
           for (int i = 0; i < 2 * kRB; ++i) {
-            const __nv_bfloat16* sp = s_src + s_off[i];
-            const uint8_t* zp = z_src + s_off[i];
+            const __nv_bfloat16* sp = s_src[i] + kAhead;
+            const uint8_t* zp = z_src + s_off[i] + kAhead;
             if (kGpc == 1) {
               s_next[i][0] = *reinterpret_cast<const uint16_t*>(sp);
               if (p.w.zero != nullptr) z_next[i] = *zp;
@@ -417,50 +460,55 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
               for (int q = 0; q < kSWords; ++q) s_next[i][q] = 0;
 #pragma unroll
               for (int q = 0; q < kGpc; ++q) {
-                if (gi + q < groups) {
+                if (gi + kAhead + q < groups) {
                   s_next[i][q / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(sp + q)) << (16 * (q & 1));
                   if (p.w.zero != nullptr) z_next[i] |= static_cast<uint32_t>(zp[q]) << (8 * q);
                 }
               }
             }
           }
-          s_src += kGpc << p.wk_log2;
-          z_src += kGpc << p.wk_log2;
-          gi += kGpc << p.wk_log2;
         };
-        fetch_scales();
+        fetch_scales(std::integral_constant<int, 0>{});
         const uint8_t* x_at[kTB];
         const float* xs_at[kTB][2];
 #pragma unroll
         for (int tb = 0; tb < kTB; ++tb) {
-          x_at[tb] = x_lane[tb];
-          xs_at[tb][0] = xs_lane[tb][0];
-          xs_at[tb][1] = xs_lane[tb][1];
+          x_at[tb] = x_lane[tb] + begin * 256;
+          xs_at[tb][0] = xs_lane[tb][0] + begin * kGpc;
+          xs_at[tb][1] = xs_lane[tb][1] + begin * kGpc;
         }
-#pragma unroll 1
-        for (int step = 0; step < steps; ++step) {
+        auto chunk = [&](auto slot_c) {  // the products of chunk kSlot of four
+          constexpr int kSlot = decltype(slot_c)::value;
           cp_async_wait<kStages - 2>();
-          __syncwarp();
-          const uint8_t* const src = fifo + slot * S::kStage + g * 64;
-          slot = (slot + 1) & (kStages - 1);
-          uint32_t w[2 * kRB][4];
-#pragma unroll
-          for (int i = 0; i < 2 * kRB; ++i) {
-            if (kGpc == 1) {
-              const uint4 v = *reinterpret_cast<const uint4*>(src + i * 512 + (t ^ swap) * 16);
-              w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
-            } else if (kGpc == 2) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint2 v = *reinterpret_cast<const uint2*>(src + i * 512 + ((2 * h + (t >> 1)) ^ swap) * 16 + (t & 1) * 8);
-                w[i][2 * h] = v.x; w[i][2 * h + 1] = v.y;
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) w[i][j] = *reinterpret_cast<const uint32_t*>(src + i * 512 + (j ^ swap) * 16 + t * 4);
-            }
+          if (kGpc > 1) __syncwarp();  // with one group in a chunk a lane reads what it has fetched itself
+          if (kSlot >= left) {
+            load_chunk(std::integral_constant<int, (kSlot + 3) % kStages>{});
+            return;
           }
-          load_step();  // into the slot that the previous step has left
+          uint32_t w[2 * kRB][4];
+          auto read_row = [&](auto row_c) {
+            constexpr int i = decltype(row_c)::value, kAt = kSlot * S::kStage + i * 512;
+            if constexpr (kGpc == 1) {
+              const uint4 v = lds128<kAt>(fifo_lane + (t ^ swap) * 16);
+              w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
+            } else if constexpr (kGpc == 2) {
+              const uint2 u = lds64<kAt>(fifo_lane + ((t >> 1) ^ swap) * 16 + (t & 1) * 8);
+              const uint2 v = lds64<kAt>(fifo_lane + ((2 + (t >> 1)) ^ swap) * 16 + (t & 1) * 8);
+              w[i][0] = u.x; w[i][1] = u.y; w[i][2] = v.x; w[i][3] = v.y;
+            } else {
+              w[i][0] = lds32<kAt>(fifo_lane + swap * 16 + t * 4);
+              w[i][1] = lds32<kAt>(fifo_lane + (1 ^ swap) * 16 + t * 4);
+              w[i][2] = lds32<kAt>(fifo_lane + (2 ^ swap) * 16 + t * 4);
+              w[i][3] = lds32<kAt>(fifo_lane + (3 ^ swap) * 16 + t * 4);
+            }
+          };
+          read_row(std::integral_constant<int, 0>{});
+          read_row(std::integral_constant<int, 1>{});
+          if constexpr (kRB > 1) {
+            read_row(std::integral_constant<int, 2 % (2 * kRB)>{});
+            read_row(std::integral_constant<int, 3 % (2 * kRB)>{});
+          }
+          load_chunk(std::integral_constant<int, (kSlot + 3) % kStages>{});  // into the slot that the previous chunk has left
           uint32_t s_cur[2 * kRB][kSWords], z_cur[2 * kRB];
 #pragma unroll
           for (int i = 0; i < 2 * kRB; ++i) {
@@ -468,25 +516,17 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
 #pragma unroll
             for (int q = 0; q < kSWords; ++q) s_cur[i][q] = s_next[i][q];
           }
-          if (step + 1 < steps) fetch_scales();
+          if (kSlot + 1 < left) fetch_scales(std::integral_constant<int, kSlot + 1>{});
           float acc[kRB][kTB][4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             constexpr int kPer = 4 / kGpc;
-            if (j % kPer == 0) {
-#pragma unroll
-              for (int rb = 0; rb < kRB; ++rb)
-#pragma unroll
-                for (int tb = 0; tb < kTB; ++tb)
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) acc[rb][tb][i] = 0.f;
-            }
             uint4 b[S::kParts][kTB];
 #pragma unroll
             for (int part = 0; part < S::kParts; ++part)
 #pragma unroll
               for (int tb = 0; tb < kTB; ++tb)
-                b[part][tb] = *reinterpret_cast<const uint4*>(x_at[tb] + part * p.cap * x_ld + j * 64);
+                b[part][tb] = *reinterpret_cast<const uint4*>(x_at[tb] + part * p.cap * x_ld + kSlot * 256 + j * 64);
 #pragma unroll
             for (int rb = 0; rb < kRB; ++rb) {
               const uint32_t lo = w[2 * rb][j], hi = w[2 * rb + 1][j];
@@ -498,7 +538,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
               for (int part = 0; part < S::kParts; ++part)
 #pragma unroll
                 for (int tb = 0; tb < kTB; ++tb) {
-                  mma_bf16(acc[rb][tb], a0, a1, a2, a3, b[part][tb].x, b[part][tb].y);
+                  if (j % kPer == 0 && part == 0) mma_bf16_first(acc[rb][tb], a0, a1, a2, a3, b[part][tb].x, b[part][tb].y);
+                  else mma_bf16(acc[rb][tb], a0, a1, a2, a3, b[part][tb].x, b[part][tb].y);
                   mma_bf16(acc[rb][tb], a4, a5, a6, a7, b[part][tb].z, b[part][tb].w);
                 }
             }
@@ -515,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
               }
 #pragma unroll
               for (int tb = 0; tb < kTB; ++tb) {
-                const float xs[2] = {xs_at[tb][0][q * p.cap], xs_at[tb][1][q * p.cap]};
+                const float xs[2] = {xs_at[tb][0][kSlot * kGpc + q], xs_at[tb][1][kSlot * kGpc + q]};
 #pragma unroll
                 for (int rb = 0; rb < kRB; ++rb)
 #pragma unroll
@@ -526,12 +567,23 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
               }
             }
           }
+        };
+#pragma unroll 1
+        for (; left > 0; left -= kStages) {
+          chunk(std::integral_constant<int, 0>{});
+          chunk(std::integral_constant<int, 1>{});
+          chunk(std::integral_constant<int, 2>{});
+          chunk(std::integral_constant<int, 3>{});
 #pragma unroll
           for (int tb = 0; tb < kTB; ++tb) {
-            x_at[tb] += 256 << p.wk_log2;
-            xs_at[tb][0] += (kGpc * p.cap) << p.wk_log2;
-            xs_at[tb][1] += (kGpc * p.cap) << p.wk_log2;
+            x_at[tb] += kStages * 256;
+            xs_at[tb][0] += kStages * kGpc;
+            xs_at[tb][1] += kStages * kGpc;
           }
+#pragma unroll
+          for (int i = 0; i < 2 * kRB; ++i) s_src[i] += kStages * kGpc;
+          z_src += kStages * kGpc;
+          gi += kStages * kGpc;
         }
       }
 
@@ -661,7 +713,8 @@ cudaError_t launch_groups(W4Params p, long long tiles, cudaStream_t stream) {
   p.span = span_chunks * kChunk;
   const int entries = std::min(p.m, kMode == kDense ? p.m : kListSlots);
   p.cap = std::min(kRoom / S::x_row_bytes(p.span, kGpc), std::max(entries, 1));
-  p.packed = p.K % kChunk == 0 && reinterpret_cast<uintptr_t>(p.w.scale) % (2 * kGpc) == 0 && reinterpret_cast<uintptr_t>(p.w.zero) % kGpc == 0;
+  p.whole = p.K % kChunk == 0;
+  p.packed = p.whole && reinterpret_cast<uintptr_t>(p.w.scale) % (2 * kGpc) == 0 && reinterpret_cast<uintptr_t>(p.w.zero) % kGpc == 0;
   const int ctas = static_cast<int>(tiles < sms ? tiles : sms);
   const int last_chunks = chunks - (chunks - 1) / span_chunks * span_chunks;  // every warp has a step in every span
   const double windows = spans > 1 ? static_cast<double>(tiles) / p.row_tiles / ctas + 1 : 1 + static_cast<double>(entries) / ctas / p.cap;
