@@ -91,6 +91,12 @@ __device__ __forceinline__ uint32_t unpack(uint32_t w, uint32_t mask, uint32_t m
   return r;
 }
 
+// 16 bytes to shared memory (zeros for size 0), both at a constant distance behind an address.
+template <int kDst, int kSrc>
+__device__ __forceinline__ void cp_async_at(uint32_t dst, const uint8_t* src, uint32_t size) {
+  asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16, %4;" ::"r"(dst), "l"(src), "n"(kDst), "n"(kSrc), "r"(size) : "memory");
+}
+
 // Reads of the FIFO, at a constant distance behind an address; volatile, for they must stay behind the wait for their copy.
 template <int kOff>
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
@@ -203,14 +209,14 @@ struct W4Shape {
   static constexpr int kFixed = kRing + kRed + kLists;
 };
 
-// kGpc: groups in a chunk. Lane (g, t) = (lane / 4, lane % 4) of a warp holds row g and g + 8 of a row block; its word j of a
+// kGpc: groups in a chunk; kZero: zero points are given. Lane (g, t) = (lane / 4, lane % 4) of a warp holds row g and g + 8 of a row block; its word j of a
 // chunk of 128 columns starts at column col_of(j, t), so that the columns of a word index belong to one group.
 template <int kGpc>
 __device__ __forceinline__ int col_of(int j, int t) {
   return kGpc == 1 ? 32 * t + 8 * j : (kGpc == 2 ? 64 * (j >> 1) + 16 * t + 8 * (j & 1) : 32 * j + 8 * t);
 }
 
-template <int kMode, int kRB, int kTB, int kGpc>
+template <int kMode, int kRB, int kTB, int kGpc, bool kZero>
 __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   using S = W4Shape<kMode, kRB, kTB>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -320,8 +326,12 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
     constexpr int kSlot = decltype(slot_c)::value;
     if (kSlot < l_left) {
       const uint32_t size = p.whole || l_col + kSlot * kChunk < p.K ? 16 : 0;  // zeros are written behind the last column
-#pragma unroll
-      for (int i = 0; i < 2 * kRB; ++i) cp_async_16(l_dst + kSlot * S::kStage + i * 512, l_src[i] + kSlot * (kChunk / 2), size);
+      cp_async_at<kSlot * S::kStage, kSlot * (kChunk / 2)>(l_dst, l_src[0], size);
+      cp_async_at<kSlot * S::kStage + 512, kSlot * (kChunk / 2)>(l_dst, l_src[1], size);
+      if constexpr (kRB > 1) {
+        cp_async_at<kSlot * S::kStage + 1024, kSlot * (kChunk / 2)>(l_dst, l_src[2 % (2 * kRB)], size);
+        cp_async_at<kSlot * S::kStage + 1536, kSlot * (kChunk / 2)>(l_dst, l_src[3 % (2 * kRB)], size);
+      }
     }
     cp_async_commit();
     if (kSlot == kStages - 1) {
@@ -376,6 +386,57 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
     }
   };
 
+  // ------------------------------------------------------------------ scales and zero points of this lane's rows
+  // Fetched one chunk ahead, and those of a tile's first chunk before the end of the tile in front of it.
+  constexpr int kSWords = kGpc == 4 ? 2 : 1;
+  const __nv_bfloat16* s_src[2 * kRB];
+  const uint8_t* z_src = nullptr;
+  int gi = 0;
+  uint32_t s_next[2 * kRB][kSWords], z_next[2 * kRB];
+  bool fetched = false;
+  auto open_scales = [&](int tile, int block, int span_i) {
+    int begin, n;
+    chunks_of(span_i, begin, n);
+    gi = (span_i * p.span / kChunk + begin) * kGpc;
+    const long long s_at = (first_row_of_matrix(block) + first_row(tile) * step_row + row_lo) * groups + gi;
+#pragma unroll
+    for (int i = 0; i < 2 * kRB; ++i) s_src[i] = p.w.scale + s_at + s_off[i];
+    z_src = p.w.zero + s_at;
+  };
+          auto fetch_scales = [&](auto ahead_c) {  // of the chunk so many chunks behind s_src
+            constexpr int kAhead = decltype(ahead_c)::value * kGpc;
+  #pragma unroll
+            for (int i = 0; i < 2 * kRB; ++i) {
+              const __nv_bfloat16* sp = s_src[i] + kAhead;
+              const uint8_t* zp = z_src + s_off[i] + kAhead;
+              if (kGpc == 1) {
+                s_next[i][0] = *reinterpret_cast<const uint16_t*>(sp);
+                if (kZero) z_next[i] = *zp;
+              } else if (p.packed) {
+                if (kGpc == 2) {
+                  s_next[i][0] = *reinterpret_cast<const uint32_t*>(sp);
+                  if (kZero) z_next[i] = *reinterpret_cast<const uint16_t*>(zp);
+                } else {
+                  const uint2 v = *reinterpret_cast<const uint2*>(sp);
+                  s_next[i][0] = v.x;
+                  s_next[i][kSWords - 1] = v.y;
+                  if (kZero) z_next[i] = *reinterpret_cast<const uint32_t*>(zp);
+                }
+              } else {
+                if (kZero) z_next[i] = 0;
+  #pragma unroll
+                for (int q = 0; q < kSWords; ++q) s_next[i][q] = 0;
+  #pragma unroll
+                for (int q = 0; q < kGpc; ++q) {
+                  if (gi + kAhead + q < groups) {
+                    s_next[i][q / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(sp + q)) << (16 * (q & 1));
+                    if (kZero) z_next[i] |= static_cast<uint32_t>(zp[q]) << (8 * q);
+                  }
+                }
+              }
+            }
+          };
+
   open();
   load_chunk(std::integral_constant<int, 0>{});
   load_chunk(std::integral_constant<int, 1>{});
@@ -426,49 +487,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
         if (!active) continue;
         int begin, left;
         chunks_of(span_i, begin, left);
-        // scales and zero points of this lane's rows, fetched one chunk ahead
-        int gi = (span_i * p.span / kChunk + begin) * kGpc;
-        const long long s_at = (mat + row0 * step_row + row_lo) * groups + gi;
-        const __nv_bfloat16* s_src[2 * kRB];
-#pragma unroll
-        for (int i = 0; i < 2 * kRB; ++i) s_src[i] = p.w.scale + s_at + s_off[i];
-        const uint8_t* z_src = p.w.zero + s_at;
-        constexpr int kSWords = kGpc == 4 ? 2 : 1;
-        uint32_t s_next[2 * kRB][kSWords], z_next[2 * kRB];
-        auto fetch_scales = [&](auto ahead_c) {  // of the chunk so many chunks behind s_src
-          constexpr int kAhead = decltype(ahead_c)::value * kGpc;
-#pragma unroll
-          for (int i = 0; i < 2 * kRB; ++i) {
-            const __nv_bfloat16* sp = s_src[i] + kAhead;
-            const uint8_t* zp = z_src + s_off[i] + kAhead;
-            if (kGpc == 1) {
-              s_next[i][0] = *reinterpret_cast<const uint16_t*>(sp);
-              if (p.w.zero != nullptr) z_next[i] = *zp;
-            } else if (p.packed) {
-              if (kGpc == 2) {
-                s_next[i][0] = *reinterpret_cast<const uint32_t*>(sp);
-                if (p.w.zero != nullptr) z_next[i] = *reinterpret_cast<const uint16_t*>(zp);
-              } else {
-                const uint2 v = *reinterpret_cast<const uint2*>(sp);
-                s_next[i][0] = v.x;
-                s_next[i][kSWords - 1] = v.y;
-                if (p.w.zero != nullptr) z_next[i] = *reinterpret_cast<const uint32_t*>(zp);
-              }
-            } else {
-              z_next[i] = 0;
-#pragma unroll
-              for (int q = 0; q < kSWords; ++q) s_next[i][q] = 0;
-#pragma unroll
-              for (int q = 0; q < kGpc; ++q) {
-                if (gi + kAhead + q < groups) {
-                  s_next[i][q / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(sp + q)) << (16 * (q & 1));
-                  if (p.w.zero != nullptr) z_next[i] |= static_cast<uint32_t>(zp[q]) << (8 * q);
-                }
-              }
-            }
-          }
-        };
-        fetch_scales(std::integral_constant<int, 0>{});
+        if (!fetched) {
+          open_scales(tile, block, span_i);
+          fetch_scales(std::integral_constant<int, 0>{});
+        }
+        fetched = false;
         const uint8_t* x_at[kTB];
         const float* xs_at[kTB][2];
 #pragma unroll
@@ -512,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
           uint32_t s_cur[2 * kRB][kSWords], z_cur[2 * kRB];
 #pragma unroll
           for (int i = 0; i < 2 * kRB; ++i) {
-            z_cur[i] = z_next[i];
+            if (kZero) z_cur[i] = z_next[i];
 #pragma unroll
             for (int q = 0; q < kSWords; ++q) s_cur[i][q] = s_next[i][q];
           }
@@ -552,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
                 const uint32_t v = s_cur[i][q / 2];
                 s[i] = __uint_as_float(q & 1 ? v & 0xffff0000u : v << 16);
                 z[i] = -136.f;
-                if (p.w.zero != nullptr) z[i] = __uint_as_float(((z_cur[i] >> (8 * q)) & 15u) << 16 | 0xc3000000u);  // -(128 + zero)
+                if (kZero) z[i] = __uint_as_float(((z_cur[i] >> (8 * q)) & 15u) << 16 | 0xc3000000u);  // -(128 + zero)
               }
 #pragma unroll
               for (int tb = 0; tb < kTB; ++tb) {
@@ -585,6 +608,12 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
           z_src += kStages * kGpc;
           gi += kStages * kGpc;
         }
+      }
+
+      if (active && tile + workers < win_last) {
+        open_scales(tile + workers, (tile + workers) / p.row_tiles, 0);
+        fetch_scales(std::integral_constant<int, 0>{});
+        fetched = true;
       }
 
       // -------------------------------------------------------------- the worker's warps meet
@@ -702,7 +731,7 @@ cudaError_t launch_groups(W4Params p, long long tiles, cudaStream_t stream) {
   using S = W4Shape<kMode, kRB, kTB>;
   constexpr int kRoom = kMaxSmem - S::kFixed;
   static_assert(kRoom / S::x_row_bytes(8 * kChunk, kGpc) >= S::kTokens);
-  auto kernel = w4_mma_kernel<kMode, kRB, kTB, kGpc>;
+  auto kernel = p.w.zero != nullptr ? w4_mma_kernel<kMode, kRB, kTB, kGpc, true> : w4_mma_kernel<kMode, kRB, kTB, kGpc, false>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
   if (e != cudaSuccess) return e;
   const int sms = device_sm_count();
