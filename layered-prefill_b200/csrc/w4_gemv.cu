@@ -19,6 +19,7 @@
 // FIFO of its own (16-byte cp.async, four 128-column steps deep) that runs on into the next tile, so no warp waits for another
 // inside a window.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -36,7 +37,7 @@ constexpr int kChunk = 128;         // columns of a step
 constexpr int kStages = 4;          // steps in a warp's FIFO
 constexpr int kListSlots = 1024;    // slots whose lists are built in shared memory
 constexpr int kListExperts = 1024;
-constexpr int kMaxSmem = 227 * 1024;
+constexpr int kMaxSmem = 227 * 1024 - 128;  // dynamic; the sort has a few words of its own
 
 enum W4Mode { kDense = 0, kGateUp = 1, kDown = 2 };
 
@@ -124,72 +125,73 @@ __device__ __forceinline__ float w4_act(float gate, float up, int activation) {
 }
 
 // Sorts the slots by expert, in ascending order inside an expert (every CTA of both passes has to find the same
-// blocks), and cuts each expert's into blocks of `width`. A warp ranks its 128 slots 32 at a time with match.any over its own row
-// of `table` [kWarps][E]; a prefix over the warps and one over the experts give every slot its place. Called by the whole CTA.
-__device__ void build_lists(SlotLists& l, int* count, uint16_t* table, const int* __restrict__ ids, int numel, int E, int width) {
+// blocks), and cuts each expert's into blocks of `width`. 32 slots rank themselves with match.any and leave their counts in a row of
+// `table` [(numel + 31) / 32][E]; prefixes over the rows and over the experts give every slot its place. Called by the whole CTA.
+__device__ void build_lists(SlotLists& l, int* first_of, uint16_t* table, const int* __restrict__ ids, int numel, int E, int width) {
+  __shared__ int warp_total[kWarps];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  uint16_t* row = table + warp * E;
-  for (int e = lane; e < E; e += 32) row[e] = 0;
-  __syncwarp();
-  constexpr int kPer = kListSlots / (32 * kWarps);
-  static_assert(kPer * 32 * kWarps == kListSlots);
-  int mine[kPer], pos[kPer];
+  constexpr int kPer = kListSlots / kThreads;
+  static_assert(kPer * kThreads == kListSlots);
+  const int rows = (numel + 31) >> 5;
+  int mine[kPer], rank[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int s = (warp * kPer + i) * 32 + lane;
+    const int r = warp + i * kWarps;
+    if (r >= rows) break;
+    const int s = r * 32 + lane;
     mine[i] = s < numel ? ids[s] : -1;
     if (mine[i] >= E || mine[i] < 0) mine[i] = -1;
+    for (int e = lane; e < E; e += 32) table[r * E + e] = 0;
+    const unsigned same = __match_any_sync(0xffffffffu, mine[i]);
+    rank[i] = __popc(same & ((1u << lane) - 1u));
+    __syncwarp();
+    if (mine[i] >= 0 && rank[i] == 0) table[r * E + mine[i]] = static_cast<uint16_t>(__popc(same));
+  }
+  __syncthreads();
+  int base = 0;  // slots so far, and blocks in the upper half
+  for (int e0 = 0; e0 < E; e0 += kThreads) {
+    const int e = e0 + t;
+    int c = 0;
+    if (e < E) {
+      for (int r = 0; r < rows; ++r) {
+        const int n = table[r * E + e];
+        table[r * E + e] = static_cast<uint16_t>(c);
+        c += n;
+      }
+    }
+    const int v = c | (((c + width - 1) / width) << 16);
+    int s = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= d) s += o;
+    }
+    if (lane == 31) warp_total[warp] = s;
+    __syncthreads();
+    int before = base;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const int n = warp_total[w];
+      if (w < warp) before += n;
+      base += n;
+    }
+    const int first = before + s - v;
+    if (e < E) first_of[e] = first & 0xffff;
+    for (int b = 0; b * width < c; ++b) {
+      const int at = (first >> 16) + b;
+      l.expert[at] = static_cast<uint16_t>(e);
+      l.start[at] = static_cast<uint16_t>((first & 0xffff) + b * width);
+      l.count[at] = static_cast<uint8_t>(min(width, c - b * width));
+    }
+    if (t == 0) l.blocks = base >> 16;
+    __syncthreads();
   }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const unsigned same = __match_any_sync(0xffffffffu, mine[i]);
-    const int rank = __popc(same & ((1u << lane) - 1u));
-    const int base = mine[i] >= 0 ? row[mine[i]] : 0;
-    pos[i] = base + rank;
-    __syncwarp();
-    if (mine[i] >= 0 && rank == 0) row[mine[i]] = static_cast<uint16_t>(base + __popc(same));
-    __syncwarp();
+    const int r = warp + i * kWarps;
+    if (r >= rows) break;
+    if (mine[i] >= 0) l.slots[first_of[mine[i]] + table[r * E + mine[i]] + rank[i]] = static_cast<uint16_t>(r * 32 + lane);
   }
-  __syncthreads();
-  for (int e = t; e < E; e += blockDim.x) {
-    int sum = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const int c = table[w * E + e];
-      table[w * E + e] = static_cast<uint16_t>(sum);
-      sum += c;
-    }
-    count[e] = sum;
-  }
-  __syncthreads();
-  if (t < 32) {  // first slot and first block of every expert, packed into one word for the scan
-    int base = 0;
-    for (int e0 = 0; e0 < E; e0 += 32) {
-      const int e = e0 + t;
-      const int c = e < E ? count[e] : 0;
-      const int v = c | (((c + width - 1) / width) << 16);
-      int s = v;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, s, d);
-        if (t >= d) s += o;
-      }
-      const int first = base + s - v;
-      if (e < E) count[e] = first & 0xffff;
-      for (int b = 0; b * width < c; ++b) {
-        const int at = (first >> 16) + b;
-        l.expert[at] = static_cast<uint16_t>(e);
-        l.start[at] = static_cast<uint16_t>((first & 0xffff) + b * width);
-        l.count[at] = static_cast<uint8_t>(min(width, c - b * width));
-      }
-      base += __shfl_sync(0xffffffffu, s, 31);
-    }
-    if (t == 0) l.blocks = base >> 16;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (mine[i] >= 0) l.slots[count[mine[i]] + row[mine[i]] + pos[i]] = static_cast<uint16_t>((warp * kPer + i) * 32 + lane);
   __syncthreads();
 }
 
@@ -234,21 +236,28 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   float* const x_sum = reinterpret_cast<float*>(x_mem + S::kParts * p.cap * x_ld);  // [cap][groups, an odd number of floats]
   const int xs_ld = p.span / kChunk * kGpc | 1;
 
-  grid_dependency_wait();
-  grid_dependency_launch();
+  // The down pass follows the gate_up pass, which lets it start only after its own wait: all but the intermediate is
+  // there already, so that the lists are made and the first codes are under way before the wait.
+  if (kMode != kDown) {
+    grid_dependency_wait();
+    grid_dependency_launch();
+  }
 
   int blocks;
   if (kMode == kDense) {
     blocks = (p.m + S::kTokens - 1) / S::kTokens;
   } else {
-    static_assert(kMode == kDense || S::kRing >= kWarps * kListExperts * 2 + kListExperts * 4, "the sort borrows the FIFOs' place");
+    static_assert(kMode == kDense || S::kRing + S::kRed >= kListSlots / 32 * kListExperts * 2 + kListExperts * 4, "the sort borrows the place of FIFOs and sums");
     build_lists(lists, reinterpret_cast<int*>(smem), reinterpret_cast<uint16_t*>(smem + kListExperts * 4), p.ids, p.m, p.E, S::kTokens);
     blocks = lists.blocks;
   }
   // this CTA's tiles, token block by token block
   const long long total = static_cast<long long>(blocks) * p.row_tiles;
   const int first = static_cast<int>(total * blockIdx.x / gridDim.x), last = static_cast<int>(total * (blockIdx.x + 1) / gridDim.x);
-  if (first == last) return;
+  if (first == last) {
+    if (kMode == kDown) grid_dependency_wait();
+    return;
+  }
 
   const int spans = (p.K + p.span - 1) / p.span;
   const int groups = p.K / p.w.group;
@@ -441,6 +450,10 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   load_chunk(std::integral_constant<int, 0>{});
   load_chunk(std::integral_constant<int, 1>{});
   load_chunk(std::integral_constant<int, 2>{});
+  if (kMode == kDown) {
+    grid_dependency_wait();
+    grid_dependency_launch();
+  }
 
   // ------------------------------------------------------------------ products
   const uint32_t mask = 0x000f000fu, magic = 0x43004300u;
@@ -709,55 +722,86 @@ int expected_blocks(int slots, int E) {
   return b < 1 ? 1 : b;
 }
 
-// Warps of a worker: the split with the fewest steps in a row. A window ends with half a round of idle workers on
-// average, and a tile's end is counted as one more step.
-int pick_wk_log2(long long tiles, int ctas, int chunks, double windows) {
-  int best = 0;
-  double best_cost = -1;
-  for (int lg = 0; lg <= 4 && (1 << lg) <= chunks; ++lg) {
-    const int workers = kWarps >> lg;
-    const double tiles_in_row = std::max(1.0, static_cast<double>(tiles) / ctas / workers + 0.5 * windows);
-    const double cost = tiles_in_row * ((chunks + (1 << lg) - 1) / (1 << lg) + 1);
-    if (best_cost < 0 || cost < best_cost) {
-      best = lg;
-      best_cost = cost;
-    }
-  }
-  return best;
-}
+// How a launch is split, and a guess of its time in cycles; the shape with the least is taken. What it weighs: a chunk of a
+// warp takes about 1100 cycles for 16 rows with all warps at work (2200 for 32), a tile's end 3000, a window ends with half a
+// round of idle workers, and activations come at 64 bytes a cycle behind a latency of 1500.
+struct W4Split {
+  int span, cap, wk_log2, ctas;
+  double cost;
+};
 
 template <int kMode, int kRB, int kTB, int kGpc>
-cudaError_t launch_groups(W4Params p, long long tiles, cudaStream_t stream) {
+W4Split split_of(const W4Params& p, long long blocks) {
   using S = W4Shape<kMode, kRB, kTB>;
   constexpr int kRoom = kMaxSmem - S::kFixed;
-  static_assert(kRoom / S::x_row_bytes(8 * kChunk, kGpc) >= S::kTokens);
-  auto kernel = p.w.zero != nullptr ? w4_mma_kernel<kMode, kRB, kTB, kGpc, true> : w4_mma_kernel<kMode, kRB, kTB, kGpc, false>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
-  if (e != cudaSuccess) return e;
-  const int sms = device_sm_count();
+  static_assert(kRoom / S::x_row_bytes(4 * kChunk, kGpc) >= S::kTokens);
+  W4Split r{};
   const int chunks = (p.K + kChunk - 1) / kChunk;
   int spans = 1;  // as few equal spans as leave room for a block's tokens
-  while (kRoom / S::x_row_bytes((chunks + spans - 1) / spans * kChunk, kGpc) < S::kTokens) ++spans;
+  const int entries = std::max(1, std::min(p.m, kMode == kDense ? p.m : kListSlots));
+  while (kRoom / S::x_row_bytes((chunks + spans - 1) / spans * kChunk, kGpc) < std::min(S::kTokens, entries)) ++spans;
   const int span_chunks = (chunks + spans - 1) / spans;
-  p.span = span_chunks * kChunk;
-  const int entries = std::min(p.m, kMode == kDense ? p.m : kListSlots);
-  p.cap = std::min(kRoom / S::x_row_bytes(p.span, kGpc), std::max(entries, 1));
-  p.whole = p.K % kChunk == 0;
-  p.packed = p.whole && reinterpret_cast<uintptr_t>(p.w.scale) % (2 * kGpc) == 0 && reinterpret_cast<uintptr_t>(p.w.zero) % kGpc == 0;
-  const int ctas = static_cast<int>(tiles < sms ? tiles : sms);
+  r.span = span_chunks * kChunk;
+  r.cap = std::min(kRoom / S::x_row_bytes(r.span, kGpc), entries);
+  const int row_tiles = ((kMode == kGateUp ? p.rows / 2 : p.rows) + S::kRows / (kMode == kGateUp ? 2 : 1) - 1) / (S::kRows / (kMode == kGateUp ? 2 : 1));
+  const long long tiles = blocks * row_tiles;
+  const int sms = device_sm_count();
+  r.ctas = static_cast<int>(tiles < sms ? tiles : sms);
+  const double per_cta = static_cast<double>(tiles) / r.ctas;
+  const double tokens = std::max(1.0, std::min<double>(S::kTokens, static_cast<double>(entries) / blocks));  // of a block
+  const double windows = 1 + (spans > 1 ? per_cta / row_tiles : std::min<double>(entries, (per_cta / row_tiles + 1) * tokens) / r.cap);
+  const double rows_a_window = std::min<double>(r.cap, std::max<double>(entries < S::kTokens ? entries : S::kTokens, static_cast<double>(entries) / r.ctas));
   const int last_chunks = chunks - (chunks - 1) / span_chunks * span_chunks;  // every warp has a step in every span
-  const double windows = spans > 1 ? static_cast<double>(tiles) / p.row_tiles / ctas + 1 : 1 + static_cast<double>(entries) / ctas / p.cap;
-  p.wk_log2 = pick_wk_log2(tiles, ctas, std::min(last_chunks, span_chunks), windows);
-  return launch_pdl(kernel, dim3(ctas), dim3(kThreads), S::kFixed + p.cap * S::x_row_bytes(p.span, kGpc), stream, p);
+  r.cost = -1;
+  for (int lg = 0; lg <= 4 && (1 << lg) <= std::min(last_chunks, span_chunks); ++lg) {
+    const double rounds = std::max(std::ceil(per_cta / (kWarps >> lg)), per_cta / (kWarps >> lg) + 0.5 * windows);
+    const double steps = (spans - 1.0) * ((span_chunks + (1 << lg) - 1) >> lg) + ((last_chunks + (1 << lg) - 1) >> lg);
+    const double x_loads = spans > 1 ? rounds * spans : windows;
+    const double cost = rounds * (steps * 1100 * kRB * (1 + 0.4 * (S::kParts * kTB - 1)) + 3000) +
+                        x_loads * (1500 + rows_a_window * S::kParts * r.span * 2 / 64.0);
+    if (r.cost < 0 || cost < r.cost) {
+      r.cost = cost;
+      r.wk_log2 = lg;
+    }
+  }
+  return r;
 }
 
-template <int kMode, int kRB, int kTB>
-cudaError_t launch_shape(W4Params p, int rows, long long blocks, cudaStream_t stream) {
-  p.row_tiles = (rows + 16 * kRB - 1) / (16 * kRB);
-  const long long tiles = blocks * p.row_tiles;
-  if (p.w.group == 128) return launch_groups<kMode, kRB, kTB, 1>(p, tiles, stream);
-  if (p.w.group == 64) return launch_groups<kMode, kRB, kTB, 2>(p, tiles, stream);
-  return launch_groups<kMode, kRB, kTB, 4>(p, tiles, stream);
+template <int kMode, int kRB, int kTB, int kGpc, bool kZero>
+cudaError_t launch_split(W4Params p, const W4Split& s, cudaStream_t stream) {
+  using S = W4Shape<kMode, kRB, kTB>;
+  auto kernel = w4_mma_kernel<kMode, kRB, kTB, kGpc, kZero>;
+  static std::atomic<unsigned long long> done{0};  // devices on which the kernel may take all shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  p.row_tiles = ((kMode == kGateUp ? p.rows / 2 : p.rows) + S::kRows / (kMode == kGateUp ? 2 : 1) - 1) / (S::kRows / (kMode == kGateUp ? 2 : 1));
+  p.span = s.span;
+  p.cap = s.cap;
+  p.wk_log2 = s.wk_log2;
+  p.whole = p.K % kChunk == 0;
+  p.packed = p.whole && reinterpret_cast<uintptr_t>(p.w.scale) % (2 * kGpc) == 0 && reinterpret_cast<uintptr_t>(p.w.zero) % kGpc == 0;
+  return launch_pdl(kernel, dim3(s.ctas), dim3(kThreads), S::kFixed + s.cap * S::x_row_bytes(s.span, kGpc), stream, p);
+}
+
+template <int kMode, int kTB, int kGpc>
+cudaError_t launch_groups(const W4Params& p, long long blocks, cudaStream_t stream) {
+  const W4Split one = split_of<kMode, 1, kTB, kGpc>(p, blocks), two = split_of<kMode, 2, kTB, kGpc>(p, blocks);
+  if (one.cost < two.cost)
+    return p.w.zero != nullptr ? launch_split<kMode, 1, kTB, kGpc, true>(p, one, stream) : launch_split<kMode, 1, kTB, kGpc, false>(p, one, stream);
+  return p.w.zero != nullptr ? launch_split<kMode, 2, kTB, kGpc, true>(p, two, stream) : launch_split<kMode, 2, kTB, kGpc, false>(p, two, stream);
+}
+
+template <int kMode, int kTB>
+cudaError_t launch_mode(const W4Params& p, long long blocks, cudaStream_t stream) {
+  if (p.w.group == 128) return launch_groups<kMode, kTB, 1>(p, blocks, stream);
+  if (p.w.group == 64) return launch_groups<kMode, kTB, 2>(p, blocks, stream);
+  return launch_groups<kMode, kTB, 4>(p, blocks, stream);
 }
 
 }  // namespace
@@ -769,11 +813,7 @@ int launch_w4_linear(__nv_bfloat16* out, const __nv_bfloat16* x, long long x_ld,
   const int tb = M <= 8 ? 1 : 2;
   const long long blocks = (M + 8 * tb - 1) / (8 * tb);
   if (blocks * ((N + 15) / 16) > 0x3fffffffll) return set_error(kStatusInvalidArgument, "w4_linear: M x N too large");
-  const int sms = device_sm_count();
-  cudaError_t e;
-  // 16-row tiles while 32-row ones would leave SMs without work
-  if (blocks * ((N + 31) / 32) < sms) e = tb == 1 ? launch_shape<kDense, 1, 1>(p, N, blocks, stream) : launch_shape<kDense, 1, 2>(p, N, blocks, stream);
-  else e = tb == 1 ? launch_shape<kDense, 2, 1>(p, N, blocks, stream) : launch_shape<kDense, 2, 2>(p, N, blocks, stream);
+  const cudaError_t e = tb == 1 ? launch_mode<kDense, 1>(p, blocks, stream) : launch_mode<kDense, 2>(p, blocks, stream);
   if (int st = check_cuda(e, "w4_linear launch")) return st;
   count_launches(1);
   return check_launch("w4_linear");
@@ -802,9 +842,9 @@ int launch_w4_experts(__nv_bfloat16* out, const __nv_bfloat16* x, const W4Matrix
     W4Params p{};
     p.w = w13; p.rows = 2 * I; p.K = H; p.x = x + static_cast<long long>(t0) * H; p.x_ld = H; p.m = slots; p.ids = ids; p.top_k = top_k;
     p.E = E; p.activation = activation; p.out = h;
-    if (int st = check_cuda(launch_shape<kGateUp, 2, 1>(p, 2 * I, blocks, stream), "w4 gate_up launch")) return st;
+    if (int st = check_cuda(launch_mode<kGateUp, 1>(p, blocks, stream), "w4 gate_up launch")) return st;
     p.w = w2; p.rows = H; p.K = I; p.x = h; p.x_ld = 2 * I; p.topk_w = topk_w + static_cast<long long>(t0) * top_k; p.out = c3;
-    if (int st = check_cuda(launch_shape<kDown, 2, 1>(p, H, blocks, stream), "w4 down launch")) return st;
+    if (int st = check_cuda(launch_mode<kDown, 1>(p, blocks, stream), "w4 down launch")) return st;
     if (int st = check_cuda(launch_pdl(w4_sum_kernel, dim3((H / 4 + 255) / 256, tt), dim3(256), 0, stream,
                                        out + static_cast<long long>(t0) * H, c3, ids, E, top_k, H), "w4 sum launch"))
       return st;
