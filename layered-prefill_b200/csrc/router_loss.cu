@@ -7,9 +7,13 @@
 // (S = sum of the picked p when renormalised, else 1), c being constant:
 //   u_e  = g_b * E * c_e / n^2 + sum_{j: id_j = e} du_j,  du_j = (dw_j - sum_i dw_i w_i) / S  (dw_j without the renormalisation)
 //   dl_e = p_e * (u_e - sum_i p_i u_i + g_z * 2 * lse / n)
-// Both passes read the logits once and recompute the softmax in registers (one warp a token): writing p and reading it
-// back would cost more than the exponentials. Sums over the tokens are fp32 over at most a few hundred terms a
-// warp, then fixed-order sums over warps and CTAs (double in the last step), so that two runs give the same bits; counts are integers.
+// Both passes read the logits once and recompute the softmax in registers (one warp a token, kU tokens at a time so that
+// their loads and reductions overlap): writing p and reading it back would cost more than the exponentials. Sums over the
+// tokens are fp32 over at most a few hundred terms a warp, then fixed-order sums over warps and CTAs (double in the last
+// step), so that two runs give the same bits; counts are integers. Bound: HBM (logits in, gradient out) for large batches,
+// launches for small ones: up to kOneCta tokens one CTA does the whole first pass.
+#include <type_traits>
+
 #include "launch.cuh"
 #include "moe_b200_internal.cuh"
 
@@ -18,13 +22,45 @@ namespace moe_b200 {
 namespace {
 
 constexpr int kMaxExperts = 1024;
-constexpr int kMaxBlocks = 128;  // CTAs of the first pass = rows of the second pass's sum
+constexpr int kMaxBlocks = 296;  // CTAs of the first pass = rows of the second pass's sum
+constexpr int kLossWarps = 16;
+constexpr int kOneCta = 128;     // tokens that one CTA of kOneWarps warps takes alone
+constexpr int kOneWarps = 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <bool kBf16>
-__device__ __forceinline__ float load_logit(const void* p, size_t i) {
-  if constexpr (kBf16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  else return static_cast<const float*>(p)[i];
+// kN experts a lane, in vectors of kW neighbours: vector v of lane l starts at expert (v * 32 + l) * kW.
+template <int kW, int kN>
+struct Lanes {
+  static constexpr int kV = kN / kW;
+  static __device__ __forceinline__ int expert(int i, int lane) { return ((i / kW) * 32 + lane) * kW + i % kW; }
+};
+
+template <bool kBf16, int kW, int kN>
+__device__ __forceinline__ void load_row(const void* logits, size_t off, int E, int lane, float (&x)[kN]) {
+#pragma unroll
+  for (int v = 0; v < kN / kW; ++v) {
+    const int e = (v * 32 + lane) * kW;
+    if constexpr (kW == 4) {
+      if (e < E) {
+        if constexpr (kBf16) {
+          const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(logits) + off + e);
+          x[4 * v] = __uint_as_float(r.x << 16);
+          x[4 * v + 1] = __uint_as_float(r.x & 0xffff0000u);
+          x[4 * v + 2] = __uint_as_float(r.y << 16);
+          x[4 * v + 3] = __uint_as_float(r.y & 0xffff0000u);
+        } else {
+          const float4 r = *reinterpret_cast<const float4*>(static_cast<const float*>(logits) + off + e);
+          x[4 * v] = r.x; x[4 * v + 1] = r.y; x[4 * v + 2] = r.z; x[4 * v + 3] = r.w;
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[4 * v + q] = -INFINITY;
+      }
+    } else {
+      if constexpr (kBf16) x[v] = e < E ? __bfloat162float(static_cast<const __nv_bfloat16*>(logits)[off + e]) : -INFINITY;
+      else x[v] = e < E ? static_cast<const float*>(logits)[off + e] : -INFINITY;
+    }
+  }
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -33,30 +69,21 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// The lane's probabilities (experts lane, lane + 32, ...; 0 past E) and the row's lse.
-template <int kVpl, bool kBf16>
-__device__ __forceinline__ void softmax_row(const void* logits, size_t off, int E, int lane, float (&p)[kVpl], float& lse, float& row_max, float& inv_sum) {
-  float m = -INFINITY;
+// x: logits in, exp(x - max) out (0 past E). A NaN reaches the sum whatever the maximum makes of it.
+template <int kW, int kN>
+__device__ __forceinline__ void exp_row(float (&x)[kN], int E, int lane, float& row_max, float& sum) {
+  float m = x[0];
 #pragma unroll
-  for (int i = 0; i < kVpl; ++i) {
-    const int e = lane + 32 * i;
-    p[i] = e < E ? load_logit<kBf16>(logits, off + e) : -INFINITY;
-    m = (p[i] > m || p[i] != p[i]) ? p[i] : m;  // a NaN logit reaches the sum below in any case
-  }
+  for (int i = 1; i < kN; ++i) m = fmaxf(m, x[i]);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-  float sum = 0.f;
+  sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kVpl; ++i) {
-    p[i] = lane + 32 * i < E ? exp2f((p[i] - m) * kLog2e) : 0.f;
-    sum += p[i];
+  for (int i = 0; i < kN; ++i) {
+    x[i] = Lanes<kW, kN>::expert(i, lane) < E ? exp2f((x[i] - m) * kLog2e) : 0.f;
+    sum += x[i];
   }
-  sum = warp_sum(sum);
-  inv_sum = 1.f / sum;
-#pragma unroll
-  for (int i = 0; i < kVpl; ++i) p[i] *= inv_sum;
   row_max = m;
-  lse = m + logf(sum);
 }
 
 struct LossOut {
@@ -74,12 +101,29 @@ struct LossParts {
   int* n;
 };
 
-// Called by a whole CTA: the sums over `blocks` rows of parts, and the outputs.
+// Called by a whole CTA of up to 1024 threads: the sums over `blocks` rows of parts, and the outputs. Several threads share an
+// expert's rows while there are enough; their sums meet in a fixed order.
 __device__ void finish_losses(const LossParts& w, int blocks, int E, const LossOut& out) {
-  __shared__ double red[32];
+  __shared__ double red[32], s_p[1024];
+  __shared__ int s_c[1024];
   __shared__ int s_n;
   __shared__ double s_z;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int parts = max(1, static_cast<int>(blockDim.x) / E);
+  double p = 0;
+  int c = 0;
+  for (int e = t; e < E * parts; e += blockDim.x) {  // one pass, or parts == 1
+    const int x = e % E, part = e / E;
+    p = 0;
+    c = 0;
+#pragma unroll 8
+    for (int b = part; b < blocks; b += parts) {
+      p += w.p[static_cast<size_t>(b) * E + x];
+      c += w.c[static_cast<size_t>(b) * E + x];
+    }
+    s_p[e] = p;
+    s_c[e] = c;
+  }
   if (warp == 0) {
     int n = 0;
     double z = 0;
@@ -102,11 +146,11 @@ __device__ void finish_losses(const LossParts& w, int blocks, int E, const LossO
   const double inv_n = 1.0 / (n > 0 ? n : 1);
   double bal = 0;
   for (int e = t; e < E; e += blockDim.x) {
-    double p = 0;
-    int c = 0;
-    for (int b = 0; b < blocks; ++b) {
-      p += w.p[static_cast<size_t>(b) * E + e];
-      c += w.c[static_cast<size_t>(b) * E + e];
+    p = 0;
+    c = 0;
+    for (int i = 0; i < parts; ++i) {
+      p += s_p[i * E + e];
+      c += s_c[i * E + e];
     }
     p *= inv_n;
     out.mean_probs[e] = static_cast<float>(p);
@@ -126,40 +170,57 @@ __device__ void finish_losses(const LossParts& w, int blocks, int E, const LossO
   }
 }
 
-template <int kVpl, bool kBf16>
-__global__ void __launch_bounds__(512)
+template <bool kBf16, int kW, int kN, int kU>
+__global__ void __launch_bounds__(kOneWarps * 32)
 router_loss_kernel(const void* __restrict__ logits, const int* __restrict__ ids, const uint8_t* __restrict__ mask, int T, int E,
-                   int k, LossParts w) {
+                   int k, LossParts w, LossOut out) {
   extern __shared__ float smem[];  // [warps][E] sums of p, then [E] counts
-  __shared__ float s_z[16];
-  __shared__ int s_n[16];
-  grid_dependency_launch();
+  __shared__ float s_z[kOneWarps];
+  __shared__ int s_n[kOneWarps];
   grid_dependency_wait();
+  grid_dependency_launch();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x >> 5;
   int* s_counts = reinterpret_cast<int*>(smem + static_cast<size_t>(warps) * E);
   for (int e = t; e < E; e += blockDim.x) s_counts[e] = 0;
   __syncthreads();
-  float acc[kVpl];
+  float acc[kN];
 #pragma unroll
-  for (int i = 0; i < kVpl; ++i) acc[i] = 0.f;
+  for (int i = 0; i < kN; ++i) acc[i] = 0.f;
   float z = 0.f;
   int n = 0;
-  for (int tok = blockIdx.x * warps + warp; tok < T; tok += gridDim.x * warps) {
-    if (mask != nullptr && mask[tok] == 0) continue;  // the same for the whole warp
-    float p[kVpl], lse, m, inv;
-    softmax_row<kVpl, kBf16>(logits, static_cast<size_t>(tok) * E, E, lane, p, lse, m, inv);
+  const int stride = gridDim.x * warps;
+  for (int tok0 = blockIdx.x * warps + warp; tok0 < T; tok0 += kU * stride) {
+    float x[kU][kN];
+    bool live[kU];  // the same for the whole warp
 #pragma unroll
-    for (int i = 0; i < kVpl; ++i) acc[i] += p[i];
-    z = fmaf(lse, lse, z);
-    ++n;
-    for (int j = lane; j < k; j += 32) {
-      const int id = ids[static_cast<size_t>(tok) * k + j];
-      if (id >= 0 && id < E) atomicAdd(&s_counts[id], 1);
+    for (int u = 0; u < kU; ++u) {
+      const int tok = tok0 + u * stride;
+      live[u] = tok < T && (mask == nullptr || mask[tok] != 0);
+      if (live[u]) load_row<kBf16, kW>(logits, static_cast<size_t>(tok) * E, E, lane, x[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (!live[u]) continue;
+      const int tok = tok0 + u * stride;
+      for (int j = lane; j < k; j += 32) {
+        const int id = ids[static_cast<size_t>(tok) * k + j];
+        if (id >= 0 && id < E) atomicAdd(&s_counts[id], 1);
+      }
+      float m, sum;
+      exp_row<kW>(x[u], E, lane, m, sum);
+      sum = warp_sum(sum);
+      const float inv = 1.f / sum, lse = m + logf(sum);
+#pragma unroll
+      for (int i = 0; i < kN; ++i) acc[i] = fmaf(x[u][i], inv, acc[i]);
+      z = fmaf(lse, lse, z);
+      ++n;
     }
   }
 #pragma unroll
-  for (int i = 0; i < kVpl; ++i)
-    if (lane + 32 * i < E) smem[static_cast<size_t>(warp) * E + lane + 32 * i] = acc[i];
+  for (int i = 0; i < kN; ++i) {
+    const int e = Lanes<kW, kN>::expert(i, lane);
+    if (e < E) smem[static_cast<size_t>(warp) * E + e] = acc[i];
+  }
   if (lane == 0) {
     s_z[warp] = z;
     s_n[warp] = n;
@@ -181,102 +242,199 @@ router_loss_kernel(const void* __restrict__ logits, const int* __restrict__ ids,
     w.z[blockIdx.x] = zs;
     w.n[blockIdx.x] = ns;
   }
+  if (gridDim.x == 1) {  // its own parts, through memory
+    __threadfence_block();
+    __syncthreads();
+    finish_losses(w, 1, E, out);
+  }
 }
 
 __global__ void __launch_bounds__(1024) router_loss_finish_kernel(LossParts w, int blocks, int E, LossOut out) {
-  grid_dependency_launch();
   grid_dependency_wait();
+  grid_dependency_launch();
   finish_losses(w, blocks, E, out);
 }
 
-template <int kVpl, bool kBf16>
+// Every warp takes tokens a grid apart, the next one's logits on their way meanwhile. The gradient of the losses is formed in
+// registers; that of the routed weights touches k of the E experts, and is added in a row of shared memory through
+// which the row leaves for the registers that store it.
+template <bool kBf16, int kW, int kN>
 __global__ void __launch_bounds__(256)
 router_backward_kernel(void* __restrict__ grad, const void* __restrict__ logits, const int* __restrict__ ids,
                        const int* __restrict__ counts, const int* __restrict__ num_tokens,
                        const float* __restrict__ grad_losses, const float* __restrict__ grad_w,
                        const uint8_t* __restrict__ mask, int T, int E, int k, int renormalize) {
-  grid_dependency_launch();
+  extern __shared__ float smem[];
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const int tok = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (tok >= T) return;
-  const size_t off = static_cast<size_t>(tok) * E;
-  float g[kVpl];
-  if (mask != nullptr && mask[tok] == 0) {
+  grid_dependency_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float* row = smem + static_cast<size_t>(warp) * E;
+  float base[kN];  // g_b * E * c_e / n^2
+  float g_z = 0.f;
 #pragma unroll
-    for (int i = 0; i < kVpl; ++i) g[i] = 0.f;
-  } else {
-    float p[kVpl], lse, m, inv;
-    softmax_row<kVpl, kBf16>(logits, off, E, lane, p, lse, m, inv);
-    float u[kVpl];
-    float g_z = 0.f;
+  for (int i = 0; i < kN; ++i) base[i] = 0.f;
+  if (grad_losses != nullptr) {
+    const float n = static_cast<float>(max(*num_tokens, 1));
+    const float coef = grad_losses[0] * E / n / n;
+    g_z = grad_losses[1] * 2.f / n;
 #pragma unroll
-    for (int i = 0; i < kVpl; ++i) u[i] = 0.f;
-    if (grad_losses != nullptr) {
-      const float n = static_cast<float>(max(*num_tokens, 1));
-      const float coef = grad_losses[0] * E / n / n;
-      g_z = grad_losses[1] * 2.f * lse / n;
-#pragma unroll
-      for (int i = 0; i < kVpl; ++i)
-        if (lane + 32 * i < E) u[i] = coef * static_cast<float>(counts[lane + 32 * i]);
+    for (int i = 0; i < kN; ++i) {
+      const int e = Lanes<kW, kN>::expert(i, lane);
+      if (e < E) base[i] = coef * static_cast<float>(counts[e]);
     }
-    if (grad_w != nullptr) {
-      // lane j holds slots j, j + 32, ...; S and the weighted sum first, then every slot's term goes to its expert's lane
-      float s = 0.f, gs = 0.f;
-      for (int j = lane; j < k; j += 32) {
-        const int id = ids[static_cast<size_t>(tok) * k + j];
-        if (id >= 0 && id < E) {
-          const float pj = exp2f((load_logit<kBf16>(logits, off + id) - m) * kLog2e) * inv;
-          s += pj;
-          gs += pj * grad_w[static_cast<size_t>(tok) * k + j];
+  }
+  const int stride = gridDim.x * (blockDim.x >> 5);
+  int tok = blockIdx.x * (blockDim.x >> 5) + warp;
+  float next[kN];
+  bool next_live = false;
+  auto fetch = [&](int at) {
+    next_live = at < T && (mask == nullptr || mask[at] != 0);
+    if (next_live) load_row<kBf16, kW>(logits, static_cast<size_t>(at) * E, E, lane, next);
+  };
+  fetch(tok);
+  for (; tok < T; tok += stride) {
+    float x[kN];
+#pragma unroll
+    for (int i = 0; i < kN; ++i) x[i] = next[i];
+    const bool live = next_live;
+    int id = -1;  // of slot `lane`
+    float gw = 0.f;
+    if (live && grad_w != nullptr && lane < k) {
+      id = ids[static_cast<size_t>(tok) * k + lane];
+      gw = grad_w[static_cast<size_t>(tok) * k + lane];
+    }
+    fetch(tok + stride);
+    const size_t off = static_cast<size_t>(tok) * E;
+    if (live) {
+      float m, sum, dot = 0.f;
+      exp_row<kW>(x, E, lane, m, sum);
+#pragma unroll
+      for (int i = 0; i < kN; ++i) dot = fmaf(x[i], base[i], dot);
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        dot += __shfl_xor_sync(0xffffffffu, dot, s);
+      }
+      const float inv = 1.f / sum;
+      float add = g_z * (m + logf(sum)) - dot * inv;
+      if (grad_w == nullptr) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) x[i] = x[i] * inv * (base[i] + add);
+      } else {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          x[i] *= inv;
+          const int e = Lanes<kW, kN>::expert(i, lane);
+          if (e < E) row[e] = x[i];
+        }
+        __syncwarp();
+        // p of the picked experts, their sum and its product with the gradients; slots past 31 in further turns
+        float pj = id >= 0 && id < E ? row[id] : 0.f;
+        float s = pj, gs = id >= 0 && id < E ? pj * gw : 0.f;
+        for (int j = lane + 32; j < k; j += 32) {
+          const int o = ids[static_cast<size_t>(tok) * k + j];
+          if (o >= 0 && o < E) {
+            s += row[o];
+            gs += row[o] * grad_w[static_cast<size_t>(tok) * k + j];
+          }
+        }
+        s = warp_sum(s);
+        gs = warp_sum(gs);
+        const float inv_s = renormalize ? 1.f / s : 1.f;
+        const float mean = renormalize ? gs * inv_s : 0.f;
+        if (!renormalize) add -= gs;  // sum p du, which the renormalisation makes zero
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          const int e = Lanes<kW, kN>::expert(i, lane);
+          if (e < E) row[e] = base[i] + add;  // u - sum p u + g_z 2 lse / n
+        }
+        __syncwarp();
+        for (int j0 = 0; j0 < k; j0 += 32) {
+          if (j0 > 0) {
+            const int j = j0 + lane;
+            id = j < k ? ids[static_cast<size_t>(tok) * k + j] : -1;
+            gw = j < k ? grad_w[static_cast<size_t>(tok) * k + j] : 0.f;
+          }
+          // slots of the same expert add up in slot order, by the first of them
+          const bool ok = id >= 0 && id < E;
+          const unsigned same = __match_any_sync(0xffffffffu, ok ? id : -1 - lane);
+          float du = ok ? (gw - mean) * inv_s : 0.f;
+          const bool lead = ok && __ffs(same) - 1 == lane;
+          if (__any_sync(0xffffffffu, ok && !lead)) {
+            const float own = du;
+            du = 0.f;
+            for (int j = 0; j < 32; ++j) {
+              const float o = __shfl_sync(0xffffffffu, own, j);
+              if (same >> j & 1) du += o;
+            }
+          }
+          if (lead) row[id] += du;
+          __syncwarp();
+        }
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          const int e = Lanes<kW, kN>::expert(i, lane);
+          if (e < E) x[i] *= row[e];
         }
       }
-      s = warp_sum(s);
-      gs = warp_sum(gs);
-      const float inv_s = renormalize ? 1.f / s : 1.f;
-      const float mean = renormalize ? gs * inv_s : 0.f;
-      for (int j = 0; j < k; ++j) {
-        const int id = ids[static_cast<size_t>(tok) * k + j];
-        const float du = (grad_w[static_cast<size_t>(tok) * k + j] - mean) * inv_s;
+    } else {
 #pragma unroll
-        for (int i = 0; i < kVpl; ++i)
-          if (id == lane + 32 * i) u[i] += du;
+      for (int i = 0; i < kN; ++i) x[i] = 0.f;
+    }
+#pragma unroll
+    for (int v = 0; v < kN / kW; ++v) {
+      const int e = (v * 32 + lane) * kW;
+      if (e >= E) continue;
+      if constexpr (kW == 4) {
+        if constexpr (kBf16) {
+          __nv_bfloat162 a = __floats2bfloat162_rn(x[4 * v], x[4 * v + 1]), b = __floats2bfloat162_rn(x[4 * v + 2], x[4 * v + 3]);
+          *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(grad) + off + e) =
+              make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+        } else {
+          *reinterpret_cast<float4*>(static_cast<float*>(grad) + off + e) = make_float4(x[4 * v], x[4 * v + 1], x[4 * v + 2], x[4 * v + 3]);
+        }
+      } else {
+        if constexpr (kBf16) static_cast<__nv_bfloat16*>(grad)[off + e] = __float2bfloat16_rn(x[v]);
+        else static_cast<float*>(grad)[off + e] = x[v];
       }
     }
-    float dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < kVpl; ++i) dot = fmaf(p[i], u[i], dot);
-    dot = warp_sum(dot);
-#pragma unroll
-    for (int i = 0; i < kVpl; ++i) g[i] = p[i] * (u[i] - dot + g_z);
-  }
-#pragma unroll
-  for (int i = 0; i < kVpl; ++i) {
-    const int e = lane + 32 * i;
-    if (e < E) {
-      if constexpr (kBf16) static_cast<__nv_bfloat16*>(grad)[off + e] = __float2bfloat16_rn(g[i]);
-      else static_cast<float*>(grad)[off + e] = g[i];
-    }
   }
 }
 
-int loss_blocks(int T, int warps) {
-  const int want = (T + warps - 1) / warps;
-  return want < 1 ? 1 : (want > kMaxBlocks ? kMaxBlocks : want);
+int loss_warps(int T) { return T <= kOneCta ? kOneWarps : kLossWarps; }
+
+int loss_blocks(int T) {
+  if (T <= kOneCta) return 1;
+  const int want = (T + kLossWarps - 1) / kLossWarps;
+  return want > kMaxBlocks ? kMaxBlocks : want;
 }
 
-constexpr int kLossWarps = 16;
-
-// Calls f(integral_constant<kVpl>) with the smallest supported number of experts a lane.
+// Calls f(kW, kN): vectors of four where they start on their own size and leave few lanes idle, else single experts.
 template <typename F>
-auto with_vpl(int E, F&& f) {
-  const int need = (E + 31) / 32;
-  if (need <= 1) return f(std::integral_constant<int, 1>{});
-  if (need <= 2) return f(std::integral_constant<int, 2>{});
-  if (need <= 4) return f(std::integral_constant<int, 4>{});
-  if (need <= 8) return f(std::integral_constant<int, 8>{});
-  if (need <= 16) return f(std::integral_constant<int, 16>{});
-  return f(std::integral_constant<int, 32>{});
+cudaError_t with_lanes(int E, bool vectors, F&& f) {
+  const int v = (E + 127) / 128, n = (E + 31) / 32;
+  if (vectors && E % 4 == 0 && 4 * v <= n + n / 4) {
+    if (v <= 1) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+    if (v <= 2) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 8>{});
+    if (v <= 4) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 16>{});
+    return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 32>{});
+  }
+  if (n <= 1) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+  if (n <= 2) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
+  if (n <= 4) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
+  if (n <= 6) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 6>{});
+  if (n <= 8) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+  if (n <= 16) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
+  return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{});
+}
+
+bool on_16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+template <typename K>
+cudaError_t allow_smem(K kernel, size_t bytes) {
+  return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) : cudaSuccess;
 }
 
 int check_router(const char* what, int T, int E, int k) {
@@ -289,7 +447,7 @@ int check_router(const char* what, int T, int E, int k) {
 }  // namespace
 
 size_t router_loss_workspace_bytes(int T, int E) {
-  const size_t b = loss_blocks(T, kLossWarps);
+  const size_t b = loss_blocks(T);
   return b * E * 8 + b * 8;
 }
 
@@ -300,26 +458,26 @@ int launch_router_loss(float* losses, int* counts, int* num_tokens, float* mean_
   const size_t need = router_loss_workspace_bytes(T, E);
   if (workspace == nullptr || workspace_bytes < need)
     return set_error(kStatusWorkspaceTooSmall, "router_loss: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
-  const int blocks = loss_blocks(T, kLossWarps);
+  const int blocks = loss_blocks(T), warps = loss_warps(T);
   LossParts w;
   w.p = static_cast<float*>(workspace);
   w.c = reinterpret_cast<int*>(w.p + static_cast<size_t>(blocks) * E);
   w.z = reinterpret_cast<float*>(w.c + static_cast<size_t>(blocks) * E);
   w.n = reinterpret_cast<int*>(w.z + blocks);
-  const size_t smem = (static_cast<size_t>(kLossWarps) + 1) * E * sizeof(float);
-  const cudaError_t e = with_vpl(E, [&](auto vpl) {
-    constexpr int V = decltype(vpl)::value;
-    auto kernel = gating_is_bf16 ? router_loss_kernel<V, true> : router_loss_kernel<V, false>;
-    if (smem > 48 * 1024) {
-      const cudaError_t a = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-      if (a != cudaSuccess) return a;
-    }
-    return launch_pdl(kernel, dim3(blocks), dim3(kLossWarps * 32), smem, stream, gating, topk_ids, token_mask, T, E, k, w);
+  const LossOut out{losses, counts, num_tokens, mean_probs};
+  const size_t smem = (static_cast<size_t>(warps) + 1) * E * sizeof(float);
+  const cudaError_t e = with_lanes(E, on_16(gating), [&](auto wc, auto nc) {
+    constexpr int W = decltype(wc)::value, N = decltype(nc)::value, U = N <= 8 ? 4 : (N <= 16 ? 2 : 1);
+    auto kernel = gating_is_bf16 ? router_loss_kernel<true, W, N, U> : router_loss_kernel<false, W, N, U>;
+    const cudaError_t a = allow_smem(kernel, smem);
+    if (a != cudaSuccess) return a;
+    return launch_pdl(kernel, dim3(blocks), dim3(warps * 32), smem, stream, gating, topk_ids, token_mask, T, E, k, w, out);
   });
   if (int st = check_cuda(e, "router_loss launch")) return st;
-  LossOut out{losses, counts, num_tokens, mean_probs};
-  if (int st = check_cuda(launch_pdl(router_loss_finish_kernel, dim3(1), dim3(1024), 0, stream, w, blocks, E, out), "router_loss finish launch")) return st;
-  count_launches(2);
+  if (blocks > 1) {
+    if (int st = check_cuda(launch_pdl(router_loss_finish_kernel, dim3(1), dim3(1024), 0, stream, w, blocks, E, out), "router_loss finish launch")) return st;
+  }
+  count_launches(blocks > 1 ? 2 : 1);
   return check_launch("router_loss");
 }
 
@@ -328,11 +486,14 @@ int launch_router_backward(void* grad_logits, const void* gating, int gating_is_
                            const uint8_t* token_mask, int T, int E, int k, int renormalize, cudaStream_t stream) {
   if (int st = check_router("router_backward", T, E, k)) return st;
   if (T == 0) return kStatusOk;
-  const cudaError_t e = with_vpl(E, [&](auto vpl) {
-    constexpr int V = decltype(vpl)::value;
-    auto kernel = gating_is_bf16 ? router_backward_kernel<V, true> : router_backward_kernel<V, false>;
-    return launch_pdl(kernel, dim3((T + 7) / 8), dim3(256), 0, stream, grad_logits, gating, topk_ids, counts, num_tokens,
-                      grad_losses, grad_topk_weights, token_mask, T, E, k, renormalize);
+  const size_t smem = grad_topk_weights != nullptr ? 8ull * E * sizeof(float) : 0;
+  const cudaError_t e = with_lanes(E, on_16(gating) && on_16(grad_logits), [&](auto wc, auto nc) {
+    constexpr int W = decltype(wc)::value, N = decltype(nc)::value;
+    auto kernel = gating_is_bf16 ? router_backward_kernel<true, W, N> : router_backward_kernel<false, W, N>;
+    const int most = device_sm_count() * 8;
+    const int want = (T + 7) / 8;
+    return launch_pdl(kernel, dim3(want < most ? want : most), dim3(256), smem, stream, grad_logits, gating, topk_ids, counts,
+                      num_tokens, grad_losses, grad_topk_weights, token_mask, T, E, k, renormalize);
   });
   if (int st = check_cuda(e, "router_backward launch")) return st;
   count_launches(1);
