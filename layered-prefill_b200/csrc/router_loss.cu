@@ -7,8 +7,9 @@
 // (S = sum of the picked p when renormalised, else 1), c being constant:
 //   u_e  = g_b * E * c_e / n^2 + sum_{j: id_j = e} du_j,  du_j = (dw_j - sum_i dw_i w_i) / S  (dw_j without the renormalisation)
 //   dl_e = p_e * (u_e - sum_i p_i u_i + g_z * 2 * lse / n)
-// Both passes read the logits once and recompute the softmax in registers (one warp a token, kU tokens at a time so that
-// their loads and reductions overlap): writing p and reading it back would cost more than the exponentials. Sums over the
+// Both passes read the logits once and recompute the softmax in registers: writing p and reading it back would cost
+// more than the exponentials. Eight lanes take a token of up to 256 experts (32 lanes one of more), so that a warp works on four
+// at once and a reduction costs three shuffles for all of them (with a warp a token the reductions were most of the work). Sums over the
 // tokens are fp32 over at most a few hundred terms a warp, then fixed-order sums over warps and CTAs (double in the last
 // step), so that two runs give the same bits; counts are integers. Bound: HBM (logits in, gradient out) for large batches,
 // launches for small ones: up to kOneCta tokens one CTA does the whole first pass.
@@ -16,6 +17,7 @@
 
 #include "launch.cuh"
 #include "moe_b200_internal.cuh"
+#include "ptx.cuh"
 
 namespace moe_b200 {
 
@@ -28,18 +30,15 @@ constexpr int kOneCta = 128;     // tokens that one CTA of kOneWarps warps takes
 constexpr int kOneWarps = 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// kN experts a lane, in vectors of kW neighbours: vector v of lane l starts at expert (v * 32 + l) * kW.
-template <int kW, int kN>
-struct Lanes {
-  static constexpr int kV = kN / kW;
-  static __device__ __forceinline__ int expert(int i, int lane) { return ((i / kW) * 32 + lane) * kW + i % kW; }
-};
+// kL lanes a token, kN experts a lane in vectors of kW neighbours: vector v of lane l (of the kL) starts at expert (v * kL + l) * kW.
+template <int kL, int kW>
+__device__ __forceinline__ int expert_of(int i, int l) { return ((i / kW) * kL + l) * kW + i % kW; }
 
-template <bool kBf16, int kW, int kN>
-__device__ __forceinline__ void load_row(const void* logits, size_t off, int E, int lane, float (&x)[kN]) {
+template <bool kBf16, int kL, int kW, int kN>
+__device__ __forceinline__ void load_row(const void* logits, size_t off, int E, int l, float (&x)[kN]) {
 #pragma unroll
   for (int v = 0; v < kN / kW; ++v) {
-    const int e = (v * 32 + lane) * kW;
+    const int e = (v * kL + l) * kW;
     if constexpr (kW == 4) {
       if (e < E) {
         if constexpr (kBf16) {
@@ -63,24 +62,31 @@ __device__ __forceinline__ void load_row(const void* logits, size_t off, int E, 
   }
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
+template <int kL>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-  for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  for (int m = kL / 2; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
   return v;
 }
 
-// x: logits in, exp(x - max) out (0 past E). A NaN reaches the sum whatever the maximum makes of it.
-template <int kW, int kN>
-__device__ __forceinline__ void exp_row(float (&x)[kN], int E, int lane, float& row_max, float& sum) {
+__device__ __forceinline__ float exp2_ftz(float x) {  // 2 ulp; what is below 2^-126 of the largest counts as nothing
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// x: logits in, exp(x - max) out (0 past E: those logits are -inf). A NaN reaches the sum whatever the maximum makes of it.
+template <int kL, int kN>
+__device__ __forceinline__ void exp_row(float (&x)[kN], float& row_max, float& sum) {
   float m = x[0];
 #pragma unroll
   for (int i = 1; i < kN; ++i) m = fmaxf(m, x[i]);
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+  for (int s = kL / 2; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
   sum = 0.f;
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
-    x[i] = Lanes<kW, kN>::expert(i, lane) < E ? exp2f((x[i] - m) * kLog2e) : 0.f;
+    x[i] = exp2_ftz((x[i] - m) * kLog2e);
     sum += x[i];
   }
   row_max = m;
@@ -101,30 +107,32 @@ struct LossParts {
   int* n;
 };
 
-// Called by a whole CTA of up to 1024 threads: the sums over `blocks` rows of parts, and the outputs. Several threads share an
-// expert's rows while there are enough; their sums meet in a fixed order.
-__device__ void finish_losses(const LossParts& w, int blocks, int E, const LossOut& out) {
-  __shared__ double red[32], s_p[1024];
+constexpr int kFinishCtas = 8;
+
+// The sums over `blocks` rows of parts, and the outputs. Called by all threads of a CTA (rank 0 of 1) or of a cluster of
+// kFinishCtas, whose CTAs take E / ranks experts each; several threads share an expert's rows. Fixed orders throughout.
+template <int kRanks>
+__device__ void finish_losses(const LossParts& w, int blocks, int E, const LossOut& out, int rank) {
+  __shared__ double red[32], s_p[1024], s_bal[kFinishCtas];
   __shared__ int s_c[1024];
   __shared__ int s_n;
   __shared__ double s_z;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int parts = max(1, static_cast<int>(blockDim.x) / E);
-  double p = 0;
-  int c = 0;
-  for (int e = t; e < E * parts; e += blockDim.x) {  // one pass, or parts == 1
-    const int x = e % E, part = e / E;
-    p = 0;
-    c = 0;
+  const int per = (E + kRanks - 1) / kRanks, e0 = rank * per, mine = max(0, min(per, E - e0));
+  const int parts = static_cast<int>(blockDim.x) / per;  // blockDim.x >= per
+  if (t < parts * mine) {
+    const int x = t % mine, part = t / mine;
+    double p = 0;
+    int c = 0;
 #pragma unroll 8
     for (int b = part; b < blocks; b += parts) {
-      p += w.p[static_cast<size_t>(b) * E + x];
-      c += w.c[static_cast<size_t>(b) * E + x];
+      p += w.p[static_cast<size_t>(b) * E + e0 + x];
+      c += w.c[static_cast<size_t>(b) * E + e0 + x];
     }
-    s_p[e] = p;
-    s_c[e] = c;
+    s_p[t] = p;
+    s_c[t] = c;
   }
-  if (warp == 0) {
+  if (warp == static_cast<int>(blockDim.x >> 5) - 1) {
     int n = 0;
     double z = 0;
     for (int b = lane; b < blocks; b += 32) {
@@ -145,32 +153,40 @@ __device__ void finish_losses(const LossParts& w, int blocks, int E, const LossO
   const int n = s_n;
   const double inv_n = 1.0 / (n > 0 ? n : 1);
   double bal = 0;
-  for (int e = t; e < E; e += blockDim.x) {
-    p = 0;
-    c = 0;
+  if (t < mine) {
+    double p = 0;
+    int c = 0;
     for (int i = 0; i < parts; ++i) {
-      p += s_p[i * E + e];
-      c += s_c[i * E + e];
+      p += s_p[i * mine + t];
+      c += s_c[i * mine + t];
     }
     p *= inv_n;
-    out.mean_probs[e] = static_cast<float>(p);
-    out.counts[e] = c;
-    bal += p * c * inv_n;
+    out.mean_probs[e0 + t] = static_cast<float>(p);
+    out.counts[e0 + t] = c;
+    bal = p * c * inv_n;
   }
 #pragma unroll
   for (int m = 16; m > 0; m >>= 1) bal += __shfl_xor_sync(0xffffffffu, bal, m);
   if (lane == 0) red[warp] = bal;
   __syncthreads();
   if (t == 0) {
-    double s = 0;
-    for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) s += red[i];
-    out.losses[0] = static_cast<float>(s * E);
+    bal = 0;
+    for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) bal += red[i];
+    if (kRanks > 1) st_cluster_f64(&s_bal[rank], 0, bal);
+  }
+  if (kRanks > 1) cluster_sync_all();
+  if (rank == 0 && t == 0) {
+    if (kRanks > 1) {
+      bal = 0;
+      for (int i = 0; i < kRanks; ++i) bal += s_bal[i];
+    }
+    out.losses[0] = static_cast<float>(bal * E);
     out.losses[1] = static_cast<float>(s_z * inv_n);
     *out.num_tokens = n;
   }
 }
 
-template <bool kBf16, int kW, int kN, int kU>
+template <bool kBf16, int kL, int kW, int kN>
 __global__ void __launch_bounds__(kOneWarps * 32)
 router_loss_kernel(const void* __restrict__ logits, const int* __restrict__ ids, const uint8_t* __restrict__ mask, int T, int E,
                    int k, LossParts w, LossOut out) {
@@ -179,7 +195,9 @@ router_loss_kernel(const void* __restrict__ logits, const int* __restrict__ ids,
   __shared__ int s_n[kOneWarps];
   grid_dependency_wait();
   grid_dependency_launch();
+  constexpr int kTokens = 32 / kL;  // of a warp at a time
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x >> 5;
+  const int l = lane % kL;
   int* s_counts = reinterpret_cast<int*>(smem + static_cast<size_t>(warps) * E);
   for (int e = t; e < E; e += blockDim.x) s_counts[e] = 0;
   __syncthreads();
@@ -188,38 +206,44 @@ router_loss_kernel(const void* __restrict__ logits, const int* __restrict__ ids,
   for (int i = 0; i < kN; ++i) acc[i] = 0.f;
   float z = 0.f;
   int n = 0;
-  const int stride = gridDim.x * warps;
-  for (int tok0 = blockIdx.x * warps + warp; tok0 < T; tok0 += kU * stride) {
-    float x[kU][kN];
-    bool live[kU];  // the same for the whole warp
+  const int stride = gridDim.x * warps * kTokens;
+  for (int tok0 = (blockIdx.x * warps + warp) * kTokens; tok0 < T; tok0 += stride) {
+    const int tok = tok0 + lane / kL;
+    const bool live = tok < T && (mask == nullptr || mask[tok] != 0);
+    float x[kN];
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int tok = tok0 + u * stride;
-      live[u] = tok < T && (mask == nullptr || mask[tok] != 0);
-      if (live[u]) load_row<kBf16, kW>(logits, static_cast<size_t>(tok) * E, E, lane, x[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      if (!live[u]) continue;
-      const int tok = tok0 + u * stride;
-      for (int j = lane; j < k; j += 32) {
+    for (int i = 0; i < kN; ++i) x[i] = 0.f;
+    if (live) {
+      load_row<kBf16, kL, kW>(logits, static_cast<size_t>(tok) * E, E, l, x);
+      for (int j = l; j < k; j += kL) {
         const int id = ids[static_cast<size_t>(tok) * k + j];
         if (id >= 0 && id < E) atomicAdd(&s_counts[id], 1);
       }
-      float m, sum;
-      exp_row<kW>(x[u], E, lane, m, sum);
-      sum = warp_sum(sum);
+    }
+    float m, sum;
+    exp_row<kL>(x, m, sum);
+    sum = lanes_sum<kL>(sum);
+    if (live) {
       const float inv = 1.f / sum, lse = m + logf(sum);
 #pragma unroll
-      for (int i = 0; i < kN; ++i) acc[i] = fmaf(x[u][i], inv, acc[i]);
+      for (int i = 0; i < kN; ++i) acc[i] = fmaf(x[i], inv, acc[i]);
       z = fmaf(lse, lse, z);
       ++n;
     }
   }
 #pragma unroll
-  for (int i = 0; i < kN; ++i) {
-    const int e = Lanes<kW, kN>::expert(i, lane);
-    if (e < E) smem[static_cast<size_t>(warp) * E + e] = acc[i];
+  for (int s = 16; s >= kL; s >>= 1) {  // the tokens of the warp
+#pragma unroll
+    for (int i = 0; i < kN; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], s);
+    z += __shfl_xor_sync(0xffffffffu, z, s);
+    n += __shfl_xor_sync(0xffffffffu, n, s);
+  }
+  if (lane < kL) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int e = expert_of<kL, kW>(i, l);
+      if (e < E) smem[static_cast<size_t>(warp) * E + e] = acc[i];
+    }
   }
   if (lane == 0) {
     s_z[warp] = z;
@@ -245,20 +269,20 @@ router_loss_kernel(const void* __restrict__ logits, const int* __restrict__ ids,
   if (gridDim.x == 1) {  // its own parts, through memory
     __threadfence_block();
     __syncthreads();
-    finish_losses(w, 1, E, out);
+    finish_losses<1>(w, 1, E, out, 0);
   }
 }
 
 __global__ void __launch_bounds__(1024) router_loss_finish_kernel(LossParts w, int blocks, int E, LossOut out) {
   grid_dependency_wait();
   grid_dependency_launch();
-  finish_losses(w, blocks, E, out);
+  finish_losses<kFinishCtas>(w, blocks, E, out, static_cast<int>(cluster_ctarank()));
 }
 
-// Every warp takes tokens a grid apart, the next one's logits on their way meanwhile. The gradient of the losses is formed in
+// Every warp takes tokens a grid apart, the next ones' logits on their way meanwhile. The gradient of the losses is formed in
 // registers; that of the routed weights touches k of the E experts, and is added in a row of shared memory through
 // which the row leaves for the registers that store it.
-template <bool kBf16, int kW, int kN>
+template <bool kBf16, int kL, int kW, int kN>
 __global__ void __launch_bounds__(256)
 router_backward_kernel(void* __restrict__ grad, const void* __restrict__ logits, const int* __restrict__ ids,
                        const int* __restrict__ counts, const int* __restrict__ num_tokens,
@@ -267,126 +291,141 @@ router_backward_kernel(void* __restrict__ grad, const void* __restrict__ logits,
   extern __shared__ float smem[];
   grid_dependency_wait();
   grid_dependency_launch();
+  constexpr int kTokens = 32 / kL;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float* row = smem + static_cast<size_t>(warp) * E;
-  float base[kN];  // g_b * E * c_e / n^2
-  float g_z = 0.f;
+  const int l = lane % kL, group = lane / kL;
+  float* row = smem + static_cast<size_t>(warp * kTokens + group) * E;
+  float g_b = 0.f, g_z = 0.f;  // g_b * E / n^2 (times c_e), g_z * 2 / n (times lse)
+  float base[kN];
 #pragma unroll
   for (int i = 0; i < kN; ++i) base[i] = 0.f;
   if (grad_losses != nullptr) {
     const float n = static_cast<float>(max(*num_tokens, 1));
-    const float coef = grad_losses[0] * E / n / n;
+    g_b = grad_losses[0] * E / n / n;
     g_z = grad_losses[1] * 2.f / n;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int e = Lanes<kW, kN>::expert(i, lane);
-      if (e < E) base[i] = coef * static_cast<float>(counts[e]);
+      const int e = expert_of<kL, kW>(i, l);
+      if (e < E) base[i] = g_b * static_cast<float>(counts[e]);
     }
   }
-  const int stride = gridDim.x * (blockDim.x >> 5);
-  int tok = blockIdx.x * (blockDim.x >> 5) + warp;
+  const int stride = gridDim.x * (blockDim.x >> 5) * kTokens;
   float next[kN];
   bool next_live = false;
+  int next_id = -1;  // of slot l
+  float next_gw = 0.f;
   auto fetch = [&](int at) {
     next_live = at < T && (mask == nullptr || mask[at] != 0);
-    if (next_live) load_row<kBf16, kW>(logits, static_cast<size_t>(at) * E, E, lane, next);
+    next_id = -1;
+    next_gw = 0.f;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) next[i] = 0.f;
+    if (next_live) {
+      load_row<kBf16, kL, kW>(logits, static_cast<size_t>(at) * E, E, l, next);
+      if (grad_w != nullptr && l < k) {
+        next_id = ids[static_cast<size_t>(at) * k + l];
+        next_gw = grad_w[static_cast<size_t>(at) * k + l];
+      }
+    }
   };
-  fetch(tok);
-  for (; tok < T; tok += stride) {
+  int tok0 = (blockIdx.x * (blockDim.x >> 5) + warp) * kTokens;
+  if (tok0 >= T) return;
+  fetch(tok0 + group);
+  for (; tok0 < T; tok0 += stride) {
+    const int tok = tok0 + group;
     float x[kN];
 #pragma unroll
     for (int i = 0; i < kN; ++i) x[i] = next[i];
     const bool live = next_live;
-    int id = -1;  // of slot `lane`
-    float gw = 0.f;
-    if (live && grad_w != nullptr && lane < k) {
-      id = ids[static_cast<size_t>(tok) * k + lane];
-      gw = grad_w[static_cast<size_t>(tok) * k + lane];
-    }
+    int id = next_id;
+    float gw = next_gw;
     fetch(tok + stride);
-    const size_t off = static_cast<size_t>(tok) * E;
-    if (live) {
-      float m, sum, dot = 0.f;
-      exp_row<kW>(x, E, lane, m, sum);
+    float m, sum, dot = 0.f;
+    exp_row<kL>(x, m, sum);
 #pragma unroll
-      for (int i = 0; i < kN; ++i) dot = fmaf(x[i], base[i], dot);
+    for (int i = 0; i < kN; ++i) dot = fmaf(x[i], base[i], dot);
+    sum = lanes_sum<kL>(sum);
+    dot = lanes_sum<kL>(dot);
+    const float inv = 1.f / sum;
+    float add = g_z * (m + logf(sum)) - dot * inv;
+    if (grad_w == nullptr) {
 #pragma unroll
-      for (int s = 16; s > 0; s >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, s);
-        dot += __shfl_xor_sync(0xffffffffu, dot, s);
+      for (int i = 0; i < kN; ++i) x[i] = x[i] * inv * (base[i] + add);
+    } else {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        x[i] *= inv;
+        const int e = expert_of<kL, kW>(i, l);
+        if (e < E) row[e] = x[i];
       }
-      const float inv = 1.f / sum;
-      float add = g_z * (m + logf(sum)) - dot * inv;
-      if (grad_w == nullptr) {
-#pragma unroll
-        for (int i = 0; i < kN; ++i) x[i] = x[i] * inv * (base[i] + add);
-      } else {
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-          x[i] *= inv;
-          const int e = Lanes<kW, kN>::expert(i, lane);
-          if (e < E) row[e] = x[i];
-        }
-        __syncwarp();
-        // p of the picked experts, their sum and its product with the gradients; slots past 31 in further turns
-        float pj = id >= 0 && id < E ? row[id] : 0.f;
-        float s = pj, gs = id >= 0 && id < E ? pj * gw : 0.f;
-        for (int j = lane + 32; j < k; j += 32) {
+      __syncwarp();
+      // p of the picked experts, their sum and its product with the gradients; slots past the lanes in further turns
+      float s = 0.f, gs = 0.f;
+      if (id >= 0 && id < E) {
+        s = row[id];
+        gs = s * gw;
+      }
+      if (live) {
+        for (int j = l + kL; j < k; j += kL) {
           const int o = ids[static_cast<size_t>(tok) * k + j];
           if (o >= 0 && o < E) {
             s += row[o];
-            gs += row[o] * grad_w[static_cast<size_t>(tok) * k + j];
+            gs = fmaf(row[o], grad_w[static_cast<size_t>(tok) * k + j], gs);
           }
-        }
-        s = warp_sum(s);
-        gs = warp_sum(gs);
-        const float inv_s = renormalize ? 1.f / s : 1.f;
-        const float mean = renormalize ? gs * inv_s : 0.f;
-        if (!renormalize) add -= gs;  // sum p du, which the renormalisation makes zero
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-          const int e = Lanes<kW, kN>::expert(i, lane);
-          if (e < E) row[e] = base[i] + add;  // u - sum p u + g_z 2 lse / n
-        }
-        __syncwarp();
-        for (int j0 = 0; j0 < k; j0 += 32) {
-          if (j0 > 0) {
-            const int j = j0 + lane;
-            id = j < k ? ids[static_cast<size_t>(tok) * k + j] : -1;
-            gw = j < k ? grad_w[static_cast<size_t>(tok) * k + j] : 0.f;
-          }
-          // slots of the same expert add up in slot order, by the first of them
-          const bool ok = id >= 0 && id < E;
-          const unsigned same = __match_any_sync(0xffffffffu, ok ? id : -1 - lane);
-          float du = ok ? (gw - mean) * inv_s : 0.f;
-          const bool lead = ok && __ffs(same) - 1 == lane;
-          if (__any_sync(0xffffffffu, ok && !lead)) {
-            const float own = du;
-            du = 0.f;
-            for (int j = 0; j < 32; ++j) {
-              const float o = __shfl_sync(0xffffffffu, own, j);
-              if (same >> j & 1) du += o;
-            }
-          }
-          if (lead) row[id] += du;
-          __syncwarp();
-        }
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-          const int e = Lanes<kW, kN>::expert(i, lane);
-          if (e < E) x[i] *= row[e];
         }
       }
-    } else {
+      s = lanes_sum<kL>(s);
+      gs = lanes_sum<kL>(gs);
+      const float inv_s = renormalize ? 1.f / s : 1.f;
+      const float mean = renormalize ? gs * inv_s : 0.f;
+      if (!renormalize) add -= gs;  // sum p du, which the renormalisation makes zero
+      __syncwarp();
 #pragma unroll
-      for (int i = 0; i < kN; ++i) x[i] = 0.f;
+      for (int i = 0; i < kN; ++i) {
+        const int e = expert_of<kL, kW>(i, l);
+        if (e < E) row[e] = base[i] + add;  // u - sum p u + g_z 2 lse / n
+      }
+      __syncwarp();
+      for (int j0 = 0; j0 < k; j0 += kL) {
+        if (j0 > 0) {
+          const int j = j0 + l;
+          const bool in = live && j < k;
+          id = in ? ids[static_cast<size_t>(tok) * k + j] : -1;
+          gw = in ? grad_w[static_cast<size_t>(tok) * k + j] : 0.f;
+        }
+        // slots of the same expert add up in slot order, by the first of them
+        const bool ok = id >= 0 && id < E;
+        const unsigned same = __match_any_sync(0xffffffffu, ok ? group * kMaxExperts + id : -1 - lane);
+        float du = ok ? (gw - mean) * inv_s : 0.f;
+        const bool lead = ok && __ffs(same) - 1 == lane;
+        if (__any_sync(0xffffffffu, ok && !lead)) {
+          const float own = du;
+          du = 0.f;
+          for (int j = 0; j < 32; ++j) {
+            const float o = __shfl_sync(0xffffffffu, own, j);
+            if (same >> j & 1) du += o;
+          }
+        }
+        if (lead) row[id] += du;
+        __syncwarp();
+      }
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int e = expert_of<kL, kW>(i, l);
+        if (e < E) x[i] *= row[e];
+      }
     }
+    if (tok >= T) continue;
+    const size_t off = static_cast<size_t>(tok) * E;
 #pragma unroll
     for (int v = 0; v < kN / kW; ++v) {
-      const int e = (v * 32 + lane) * kW;
+      const int e = (v * kL + l) * kW;
       if (e >= E) continue;
+      if (!live) {
+#pragma unroll
+        for (int q = 0; q < kW; ++q) x[kW * v + q] = 0.f;
+      }
       if constexpr (kW == 4) {
         if constexpr (kBf16) {
           __nv_bfloat162 a = __floats2bfloat162_rn(x[4 * v], x[4 * v + 1]), b = __floats2bfloat162_rn(x[4 * v + 2], x[4 * v + 3]);
@@ -403,31 +442,38 @@ router_backward_kernel(void* __restrict__ grad, const void* __restrict__ logits,
   }
 }
 
+int lanes_of(int E) { return E <= 256 ? 8 : 32; }
 int loss_warps(int T) { return T <= kOneCta ? kOneWarps : kLossWarps; }
 
-int loss_blocks(int T) {
+int loss_blocks(int T, int E) {
   if (T <= kOneCta) return 1;
-  const int want = (T + kLossWarps - 1) / kLossWarps;
+  const int per = kLossWarps * 32 / lanes_of(E), want = (T + per - 1) / per;
   return want > kMaxBlocks ? kMaxBlocks : want;
 }
 
-// Calls f(kW, kN): vectors of four where they start on their own size and leave few lanes idle, else single experts.
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+// Calls f(kL, kW, kN): vectors of four where they start on their own size, else single experts.
 template <typename F>
 cudaError_t with_lanes(int E, bool vectors, F&& f) {
-  const int v = (E + 127) / 128, n = (E + 31) / 32;
-  if (vectors && E % 4 == 0 && 4 * v <= n + n / 4) {
-    if (v <= 1) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
-    if (v <= 2) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 8>{});
-    if (v <= 4) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 16>{});
-    return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 32>{});
+  if (lanes_of(E) == 32) {
+    if (vectors && E % 4 == 0) return E <= 512 ? f(Int<32>{}, Int<4>{}, Int<16>{}) : f(Int<32>{}, Int<4>{}, Int<32>{});
+    return E <= 512 ? f(Int<32>{}, Int<1>{}, Int<16>{}) : f(Int<32>{}, Int<1>{}, Int<32>{});
   }
-  if (n <= 1) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-  if (n <= 2) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
-  if (n <= 4) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
-  if (n <= 6) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 6>{});
-  if (n <= 8) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
-  if (n <= 16) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
-  return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{});
+  if (vectors && E % 4 == 0) {
+    const int v = (E + 31) / 32;
+    if (v <= 1) return f(Int<8>{}, Int<4>{}, Int<4>{});
+    if (v <= 2) return f(Int<8>{}, Int<4>{}, Int<8>{});
+    if (v <= 4) return f(Int<8>{}, Int<4>{}, Int<16>{});
+    if (v <= 5) return f(Int<8>{}, Int<4>{}, Int<20>{});
+    return f(Int<8>{}, Int<4>{}, Int<32>{});
+  }
+  const int n = (E + 7) / 8;
+  if (n <= 2) return f(Int<8>{}, Int<1>{}, Int<2>{});
+  if (n <= 8) return f(Int<8>{}, Int<1>{}, Int<8>{});
+  if (n <= 16) return f(Int<8>{}, Int<1>{}, Int<16>{});
+  return f(Int<8>{}, Int<1>{}, Int<32>{});
 }
 
 bool on_16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -447,7 +493,7 @@ int check_router(const char* what, int T, int E, int k) {
 }  // namespace
 
 size_t router_loss_workspace_bytes(int T, int E) {
-  const size_t b = loss_blocks(T);
+  const size_t b = loss_blocks(T, E);
   return b * E * 8 + b * 8;
 }
 
@@ -458,7 +504,7 @@ int launch_router_loss(float* losses, int* counts, int* num_tokens, float* mean_
   const size_t need = router_loss_workspace_bytes(T, E);
   if (workspace == nullptr || workspace_bytes < need)
     return set_error(kStatusWorkspaceTooSmall, "router_loss: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
-  const int blocks = loss_blocks(T), warps = loss_warps(T);
+  const int blocks = loss_blocks(T, E), warps = loss_warps(T);
   LossParts w;
   w.p = static_cast<float*>(workspace);
   w.c = reinterpret_cast<int*>(w.p + static_cast<size_t>(blocks) * E);
@@ -466,16 +512,16 @@ int launch_router_loss(float* losses, int* counts, int* num_tokens, float* mean_
   w.n = reinterpret_cast<int*>(w.z + blocks);
   const LossOut out{losses, counts, num_tokens, mean_probs};
   const size_t smem = (static_cast<size_t>(warps) + 1) * E * sizeof(float);
-  const cudaError_t e = with_lanes(E, on_16(gating), [&](auto wc, auto nc) {
-    constexpr int W = decltype(wc)::value, N = decltype(nc)::value, U = N <= 8 ? 4 : (N <= 16 ? 2 : 1);
-    auto kernel = gating_is_bf16 ? router_loss_kernel<true, W, N, U> : router_loss_kernel<false, W, N, U>;
+  const cudaError_t e = with_lanes(E, on_16(gating), [&](auto lc, auto wc, auto nc) {
+    constexpr int L = decltype(lc)::value, W = decltype(wc)::value, N = decltype(nc)::value;
+    auto kernel = gating_is_bf16 ? router_loss_kernel<true, L, W, N> : router_loss_kernel<false, L, W, N>;
     const cudaError_t a = allow_smem(kernel, smem);
     if (a != cudaSuccess) return a;
     return launch_pdl(kernel, dim3(blocks), dim3(warps * 32), smem, stream, gating, topk_ids, token_mask, T, E, k, w, out);
   });
   if (int st = check_cuda(e, "router_loss launch")) return st;
   if (blocks > 1) {
-    if (int st = check_cuda(launch_pdl(router_loss_finish_kernel, dim3(1), dim3(1024), 0, stream, w, blocks, E, out), "router_loss finish launch")) return st;
+    if (int st = check_cuda(launch_pdl_cluster(router_loss_finish_kernel, dim3(kFinishCtas), dim3(1024), 0, stream, kFinishCtas, w, blocks, E, out), "router_loss finish launch")) return st;
   }
   count_launches(blocks > 1 ? 2 : 1);
   return check_launch("router_loss");
@@ -486,12 +532,13 @@ int launch_router_backward(void* grad_logits, const void* gating, int gating_is_
                            const uint8_t* token_mask, int T, int E, int k, int renormalize, cudaStream_t stream) {
   if (int st = check_router("router_backward", T, E, k)) return st;
   if (T == 0) return kStatusOk;
-  const size_t smem = grad_topk_weights != nullptr ? 8ull * E * sizeof(float) : 0;
-  const cudaError_t e = with_lanes(E, on_16(gating) && on_16(grad_logits), [&](auto wc, auto nc) {
-    constexpr int W = decltype(wc)::value, N = decltype(nc)::value;
-    auto kernel = gating_is_bf16 ? router_backward_kernel<true, W, N> : router_backward_kernel<false, W, N>;
+  const int tokens = 8 * 32 / lanes_of(E);  // of a CTA at a time
+  const size_t smem = grad_topk_weights != nullptr ? static_cast<size_t>(tokens) * E * sizeof(float) : 0;
+  const cudaError_t e = with_lanes(E, on_16(gating) && on_16(grad_logits), [&](auto lc, auto wc, auto nc) {
+    constexpr int L = decltype(lc)::value, W = decltype(wc)::value, N = decltype(nc)::value;
+    auto kernel = gating_is_bf16 ? router_backward_kernel<true, L, W, N> : router_backward_kernel<false, L, W, N>;
     const int most = device_sm_count() * 8;
-    const int want = (T + 7) / 8;
+    const int want = (T + tokens - 1) / tokens;
     return launch_pdl(kernel, dim3(want < most ? want : most), dim3(256), smem, stream, grad_logits, gating, topk_ids, counts,
                       num_tokens, grad_losses, grad_topk_weights, token_mask, T, E, k, renormalize);
   });
