@@ -280,9 +280,8 @@ def _fused_experts_w4(hidden_states, w1, w2, topk_weights, topk_ids, inplace, ac
         raise ValueError(f"4-bit weights come in groups of 32, 64 or 128, got {group_size}")
     if activation not in ACT_CODES:
         raise ValueError(f"Unsupported FusedMoe activation: {activation}")
-    for name, v in dict(a1_scale=a1_scale, a2_scale=a2_scale, expert_map=expert_map).items():
-        if v is not None:
-            raise ValueError(f"{name} is not supported with 4-bit weights")
+    if a1_scale is not None or a2_scale is not None or expert_map is not None:
+        raise ValueError("a1_scale, a2_scale and expert_map are not supported with 4-bit weights")
     if apply_router_weight_on_input or global_num_experts not in (-1, w1.size(0)):
         raise NotImplementedError("apply_router_weight_on_input and expert parallelism are not used by the reference's models")
     if hidden_states.dim() != 2 or topk_ids.dim() != 2 or topk_weights.shape != topk_ids.shape:
@@ -291,15 +290,14 @@ def _fused_experts_w4(hidden_states, w1, w2, topk_weights, topk_ids, inplace, ac
     E, inter, k, g = w1.size(0), w1.size(1) // 2, topk_ids.size(1), group_size
     if H % g or inter % g:
         raise ValueError(f"H and I must be whole numbers of groups of {g} (H={H}, I={inter})")
-    tw = topk_weights if topk_weights.dtype == torch.float32 else topk_weights.float()
-    ti = topk_ids if topk_ids.dtype == torch.int32 else topk_ids.to(torch.int32)
-    tw, ti = tw.contiguous(), ti.contiguous()
+    tw = topk_weights if topk_weights.dtype is torch.float32 and topk_weights.is_contiguous() else topk_weights.float().contiguous()
+    ti = topk_ids if topk_ids.dtype is torch.int32 and topk_ids.is_contiguous() else topk_ids.to(torch.int32).contiguous()
     bf16, u8, dev = torch.bfloat16, torch.uint8, hidden_states.device
-    ops._check("fused_experts (4-bit)", dev, hidden_states=(hidden_states, bf16, (T, H)), w1=(w1, u8, (E, 2 * inter, H // 2)),
-               w2=(w2, u8, (E, H, inter // 2)), w1_scale=(w1_scale, bf16, (E, 2 * inter, H // g)),
-               w2_scale=(w2_scale, bf16, (E, H, inter // g)), w1_zp=(w1_zp, u8, (E, 2 * inter, H // g)),
-               w2_zp=(w2_zp, u8, (E, H, inter // g)), w1_bias=(w1_bias, bf16, (E, 2 * inter)), w2_bias=(w2_bias, bf16, (E, H)),
-               topk_weights=(tw, torch.float32, (T, k)), topk_ids=(ti, torch.int32, (T, k)))
+    ops._check("fused_experts (4-bit)", dev, "hidden_states w1 w2 w1_scale w2_scale w1_zp w2_zp w1_bias w2_bias topk_weights topk_ids",
+               (hidden_states, bf16, (T, H)), (w1, u8, (E, 2 * inter, H // 2)), (w2, u8, (E, H, inter // 2)),
+               (w1_scale, bf16, (E, 2 * inter, H // g)), (w2_scale, bf16, (E, H, inter // g)), (w1_zp, u8, (E, 2 * inter, H // g)),
+               (w2_zp, u8, (E, H, inter // g)), (w1_bias, bf16, (E, 2 * inter)), (w2_bias, bf16, (E, H)),
+               (tw, torch.float32, (T, k)), (ti, torch.int32, (T, k)))
     out = hidden_states if inplace else torch.empty_like(hidden_states)
     nbytes = lib.moe_b200_fused_experts_w4_workspace_bytes(T, E, k, H, inter)
     # not the shared scratch buffer: a tensor of the current stream (or of the capture's own pool), a few KB a slot

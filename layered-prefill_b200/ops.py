@@ -126,16 +126,19 @@ def _launch(fn, device: torch.device, *args) -> None:
         check(status)
 
 
-def _is(t: torch.Tensor, dtype: torch.dtype, shape, device: torch.device) -> bool:
-    return t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous()
-
-
-def _check(op: str, device: torch.device, **tensors) -> None:
-    """name=(tensor, dtype, shape): CUDA tensor of that device, dtype and shape, contiguous. None tensors pass."""
+def _check(op: str, device: torch.device, names: str, *specs) -> None:
+    """specs, named by names: (tensor or None, dtype, shape); contiguous tensors of that CUDA device, dtype and shape."""
+    idx = device.index
+    for t, dtype, shape in specs:
+        if t is not None and (t.get_device() != idx or t.dtype is not dtype or t.shape != shape or not t.is_contiguous()):
+            break
+    else:
+        if device.type == "cuda":
+            return
     if device.type != "cuda":
         raise RuntimeError(f"{op}: takes CUDA tensors only (got one on {device}); there is no CPU path")
-    for name, (t, dtype, shape) in tensors.items():
-        if t is None or _is(t, dtype, shape, device):
+    for name, (t, dtype, shape) in zip(names.split(), specs):
+        if t is None:
             continue
         if t.device != device:
             raise RuntimeError(f"{op}: {name} must be on {device} like the other tensors, got {t.device}")
@@ -143,7 +146,8 @@ def _check(op: str, device: torch.device, **tensors) -> None:
             raise RuntimeError(f"{op}: {name} must be {dtype}, got {t.dtype}")
         if t.shape != shape:
             raise RuntimeError(f"{op}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-        raise RuntimeError(f"{op}: {name} must be contiguous")
+        if not t.is_contiguous():
+            raise RuntimeError(f"{op}: {name} must be contiguous")
 
 
 def _ptr(t) -> int:
@@ -154,11 +158,11 @@ def _norm_quant(op, out, scales, residual, input, weight, epsilon, group_size, n
     H = input.size(-1) if input.dim() else 0
     T = input.numel() // H if H else 0
     groups = 1 if group_size == -1 or (group_size == H and H != 128) else H // 128
-    bf16, shape = torch.bfloat16, input.shape
-    _check(op, input.device, input=(input, bf16, shape), out=(out, torch.float8_e4m3fn, shape), weight=(weight, bf16, (H,)),
-           residual=(residual, bf16, shape), residual_out=(residual_out, bf16, shape), normed_out=(normed_out, bf16, shape),
-           scales=(scales, torch.float32, (*shape[:-1], groups)))
-    _launch(lib.moe_b200_rms_norm_quant_fp8, input.device, out.data_ptr(), scales.data_ptr(), _ptr(normed_out),
+    bf16, shape, device = torch.bfloat16, input.shape, input.device
+    _check(op, device, "input out weight scales residual residual_out normed_out", (input, bf16, shape),
+           (out, torch.float8_e4m3fn, shape), (weight, bf16, (H,)), (scales, torch.float32, (*shape[:-1], groups)),
+           (residual, bf16, shape), (residual_out, bf16, shape), (normed_out, bf16, shape))
+    _launch(lib.moe_b200_rms_norm_quant_fp8, device, out.data_ptr(), scales.data_ptr(), _ptr(normed_out),
             _ptr(residual_out), _ptr(residual), input.data_ptr(), weight.data_ptr(), epsilon, T, H, group_size)
 
 
@@ -193,12 +197,11 @@ def w4_linear(out: torch.Tensor, input: torch.Tensor, qweight: torch.Tensor, sca
     ld = K
     if input.dim() == 2 and input.stride(1) == 1 and not input.is_contiguous():
         ld = input.stride(0)
-        _check("w4_linear", qweight.device, input=(input[:1], torch.bfloat16, (min(M, 1), K)))
-    else:
-        _check("w4_linear", qweight.device, input=(input, torch.bfloat16, input.shape))
-    _check("w4_linear", qweight.device, out=(out, torch.bfloat16, (*input.shape[:-1], N)), qweight=(qweight, torch.uint8, (N, K // 2)),
-           scales=(scales, torch.bfloat16, (N, groups)), zeros=(zeros, torch.uint8, (N, groups)), bias=(bias, torch.bfloat16, (N,)))
-    _launch(lib.moe_b200_w4_linear, qweight.device, out.data_ptr(), input.data_ptr(), ld, qweight.data_ptr(), scales.data_ptr(),
+    bf16, u8, device, shape = torch.bfloat16, torch.uint8, qweight.device, input.shape
+    checked = (input, bf16, shape) if ld == K else (input[:1], bf16, (min(M, 1), K))
+    _check("w4_linear", device, "input out qweight scales zeros bias", checked, (out, bf16, (*shape[:-1], N)),
+           (qweight, u8, (N, K // 2)), (scales, bf16, (N, groups)), (zeros, u8, (N, groups)), (bias, bf16, (N,)))
+    _launch(lib.moe_b200_w4_linear, device, out.data_ptr(), input.data_ptr(), ld, qweight.data_ptr(), scales.data_ptr(),
             _ptr(zeros), _ptr(bias), M, N, K, K // groups if K % groups == 0 else -1)
 
 
@@ -209,12 +212,9 @@ def _router_args(op, gating_output, topk_ids, token_mask):
         raise RuntimeError(f"{op}: gating_output must be float32 or bfloat16")
     T, E = gating_output.shape
     k = topk_ids.size(1)
-    _check(op, gating_output.device, gating_output=(gating_output, gating_output.dtype, (T, E)),
-           topk_ids=(topk_ids, torch.int32, (T, k)))
-    if token_mask is not None:
-        _check(op, gating_output.device,
-               token_mask=(token_mask, torch.uint8 if token_mask.dtype == torch.uint8 else torch.bool, (T,)))
-    return T, E, k
+    specs = ((gating_output, gating_output.dtype, (T, E)), (topk_ids, torch.int32, (T, k)),
+             (token_mask, torch.uint8 if token_mask is not None and token_mask.dtype == torch.uint8 else torch.bool, (T,)))
+    return T, E, k, specs
 
 
 def router_loss(losses: torch.Tensor, counts: torch.Tensor, num_tokens: torch.Tensor, mean_probs: torch.Tensor,
@@ -223,10 +223,11 @@ def router_loss(losses: torch.Tensor, counts: torch.Tensor, num_tokens: torch.Te
     outside [0, E) are not counted), token_mask bool [T] (False: padding, neither read nor counted). With n counted tokens
     (divisions by at least 1) and p = softmax(gating_output): counts int32 [E], num_tokens int32 [1] = n, mean_probs fp32 [E] =
     sum p / n, losses fp32 [2] = (E * sum(counts / n * mean_probs), sum logsumexp^2 / n). E <= 1024. Same bits on every run."""
-    T, E, k = _router_args("router_loss", gating_output, topk_ids, token_mask)
+    T, E, k, specs = _router_args("router_loss", gating_output, topk_ids, token_mask)
     dev = gating_output.device
-    _check("router_loss", dev, losses=(losses, torch.float32, (2,)), counts=(counts, torch.int32, (E,)),
-           num_tokens=(num_tokens, torch.int32, (1,)), mean_probs=(mean_probs, torch.float32, (E,)))
+    _check("router_loss", dev, "gating_output topk_ids token_mask losses counts num_tokens mean_probs", *specs,
+           (losses, torch.float32, (2,)), (counts, torch.int32, (E,)), (num_tokens, torch.int32, (1,)),
+           (mean_probs, torch.float32, (E,)))
     nbytes = lib.moe_b200_router_loss_workspace_bytes(T, E)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _launch(lib.moe_b200_router_loss, dev, losses.data_ptr(), counts.data_ptr(), num_tokens.data_ptr(), mean_probs.data_ptr(),
@@ -241,11 +242,12 @@ def router_backward(grad_logits: torch.Tensor, gating_output: torch.Tensor, topk
     to gating_output; counts and num_tokens come from `router_loss` (summed over the ranks of a data-parallel job), the routed weights
     are those of `topk_softmax` / `topk_softmax_renorm`. grad_losses fp32 [2] and grad_topk_weights fp32 [T, k] may be None. Rows that
     token_mask leaves out are zero. grad_logits must not share memory with gating_output."""
-    T, E, k = _router_args("router_backward", gating_output, topk_ids, token_mask)
-    _check("router_backward", gating_output.device, grad_logits=(grad_logits, gating_output.dtype, (T, E)),
-           counts=(counts, torch.int32, (E,)), num_tokens=(num_tokens, torch.int32, (1,)),
-           grad_losses=(grad_losses, torch.float32, (2,)), grad_topk_weights=(grad_topk_weights, torch.float32, (T, k)))
-    _launch(lib.moe_b200_router_backward, gating_output.device, grad_logits.data_ptr(), gating_output.data_ptr(),
+    T, E, k, specs = _router_args("router_backward", gating_output, topk_ids, token_mask)
+    dev = gating_output.device
+    _check("router_backward", dev, "gating_output topk_ids token_mask grad_logits counts num_tokens grad_losses grad_topk_weights",
+           *specs, (grad_logits, gating_output.dtype, (T, E)), (counts, torch.int32, (E,)), (num_tokens, torch.int32, (1,)),
+           (grad_losses, torch.float32, (2,)), (grad_topk_weights, torch.float32, (T, k)))
+    _launch(lib.moe_b200_router_backward, dev, grad_logits.data_ptr(), gating_output.data_ptr(),
             gating_output.dtype == torch.bfloat16, topk_ids.data_ptr(), _ptr(counts), _ptr(num_tokens), _ptr(grad_losses),
             _ptr(grad_topk_weights), _ptr(token_mask), T, E, k, bool(renormalize))
 
