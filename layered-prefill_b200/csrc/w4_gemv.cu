@@ -5,17 +5,22 @@
 //
 // Bound: the weight bytes. An SM has to turn 23 bytes = 46 codes a cycle into products to keep up with HBM, which plain
 // fused multiply-adds cannot (one instruction a code and token), so the products run on the tensor cores with the WEIGHTS as the
-// 16-row operand and 8 tokens as columns (mma m16n8k16; tcgen05 wants its operand in shared or tensor memory, i.e. the
-// unpacked weights written out once more, four times the bytes that come in, for tiles that are 128 rows high). A code
-// becomes bf16 in two instructions for two codes: (w >> 4i) & 0x000f000f | 0x43004300 is the pair (128 + code_i, 128 + code_{i+4}) of an
-// eight-code word. The 128 and the zero point leave by the group's sum of x:
-//   sum (code - zero) x = sum (128 + code) x - (128 + zero) sum x
-// Products with x are exact and the sums are fp32, so the difference is off by some 2^-23 * 136 * sum |x|, a hundredth of what the
-// rounding of the output to bf16 costs.
+// 16-row operand and 8 tokens as columns. tcgen05 wants its operand in shared or tensor memory, i.e. the unpacked
+// weights written out once more for tiles that are 128 rows high; mma.sync takes them from the registers in which they are unpacked.
+// The integer form (m16n8k32, u8 codes) takes codes as they are: three instructions unpack eight of them (w & 0x0f0f0f0f and
+// (w >> 4) & 0x0f0f0f0f), against seven to bf16 (shift, mask and a 128 that has to leave the sum again), and one instruction multiplies
+// 32 columns instead of 16 at the same rate. Unpacking is what bounds the loop next to the loads.
+//   The activations become 16-bit integers with a power of two f for every token and group of columns:
+//   x = f * (256 hi + lo), hi signed and lo unsigned bytes, two products a word; f puts the group's largest |x| between 2^14 and 2^15.
+//   A bf16 value has 8 significant bits, so that all within 2^7 of the group's largest are exact and smaller ones are off by at most
+//   2^-16 of the largest; the intermediate h of the experts (fp32) is off by that everywhere. Integer sums are exact; then
+//   sum (code - zero) x = f * (256 sum code hi + sum code lo - zero * sum x) in fp32, times the group's scale, summed in fp32.
+//   A group with a value that is not finite gets f = NaN, so that its token's results are NaN.
+// The sums start at 0x4b400000, which makes their bits the float 12582912 + sum: no conversion instruction.
 //
 // Work: a tile is 16 * kRB weight rows x one block of up to 8 * kTB tokens; a CTA takes consecutive tiles, so that it
-// meets few token blocks. The activations of a window of them stay in shared memory, already in the order in which the pairs above
-// come, next to their group sums. A worker is 1 to 16 warps that split a tile's columns. Every warp streams codes through a
+// meets few token blocks. The activations of a window of them stay in shared memory as the integers above, in the
+// order in which the codes come, next to their group sums. A worker is 1 to 16 warps that split a tile's columns. Every warp streams codes through a
 // FIFO of its own (16-byte cp.async, four 128-column steps deep) that runs on into the next tile, so no warp waits for another
 // inside a window.
 #include <algorithm>
@@ -51,7 +56,7 @@ struct W4Params {
   int packed;             // the scales and zero points of a chunk can be read at once
   int wk_log2;            // log2 of the warps of a worker
   int row_tiles;
-  const __nv_bfloat16* x;  // dense / gate_up: [tokens, K]; down: [slots][2][K], the high and the low part
+  const void* x;          // dense / gate_up: bf16 [tokens, K]; down: fp32 [slots, K]
   long long x_ld;
   int m;                  // dense: tokens; experts: slots
   const int* ids;
@@ -59,7 +64,7 @@ struct W4Params {
   int E;
   int activation;
   const float* topk_w;
-  void* out;              // dense bf16 [m][rows]; gate_up bf16 [slots][2][I]; down fp32 [slots][rows]
+  void* out;              // dense bf16 [m][rows]; gate_up fp32 [slots][I]; down fp32 [slots][rows]
 };
 
 // Token blocks of the routed experts: slots in expert order and, per block, its expert and where its slots are.
@@ -71,26 +76,21 @@ struct SlotLists {
   int blocks;
 };
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// d = c + codes (16 rows x 32 columns, u8) * x bytes (32 columns x 8 tokens), signed (the high bytes) or unsigned.
+template <bool kSigned>
+__device__ __forceinline__ void mma_codes(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const int (&c)[4]) {
+  if constexpr (kSigned)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+  else
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
 
-// The same with nothing in the accumulator yet.
-__device__ __forceinline__ void mma_bf16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-
-// Codes i and i + 4 of a word as bf16, plus 128; one shift and one (a & b) | c, which two immediates would make two.
-template <int i>
-__device__ __forceinline__ uint32_t unpack(uint32_t w, uint32_t mask, uint32_t magic) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w >> (4 * i)), "r"(mask), "r"(magic));
-  return r;
-}
+constexpr int kFloatBits = 0x4b400000;    // bits of 12582912.f, one more for every unit up to 2^22
+constexpr float kFloatBias = 12582912.f;
 
 // 16 bytes to shared memory (zeros for size 0), both at a constant distance behind an address.
 template <int kDst, int kSrc>
@@ -119,9 +119,9 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
 }
 
 __device__ __forceinline__ float w4_act(float gate, float up, int activation) {
-  if (activation == 0) return gate / (1.f + __expf(-gate)) * up;
+  if (activation == 0) return __fdividef(gate, 1.f + __expf(-gate)) * up;
   const float g = fminf(gate, 7.f), u = fminf(fmaxf(up, -7.f), 7.f);
-  return g / (1.f + __expf(-1.702f * g)) * (u + 1.f);
+  return __fdividef(g, 1.f + __expf(-1.702f * g)) * (u + 1.f);
 }
 
 // Sorts the slots by expert, in ascending order inside an expert (every CTA of both passes has to find the same
@@ -197,7 +197,6 @@ __device__ void build_lists(SlotLists& l, int* first_of, uint16_t* table, const 
 
 template <int kMode, int kRB, int kTB>
 struct W4Shape {
-  static constexpr int kParts = kMode == kDown ? 2 : 1;  // high and low part of the activations
   static constexpr int kRows = 16 * kRB;
   static constexpr int kTokens = 8 * kTB;
   static constexpr int kStage = kRows * 64;
@@ -207,7 +206,7 @@ struct W4Shape {
   // a token row of `span` columns: 64 bytes more than a multiple of 128, so that the two tokens of an eight-lane phase of a
   // 16-byte read use different banks
   __host__ __device__ static constexpr int x_ld(int span) { return span * 2 + 64; }
-  __host__ __device__ static constexpr int x_row_bytes(int span, int gpc) { return kParts * x_ld(span) + (span / kChunk * gpc | 1) * 4; }
+  __host__ __device__ static constexpr int x_row_bytes(int span, int gpc) { return x_ld(span) + (span / kChunk * gpc | 1) * 8; }
   static constexpr int kFixed = kRing + kRed + kLists;
 };
 
@@ -233,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   SlotLists& lists = *reinterpret_cast<SlotLists*>(smem + S::kRing + S::kRed);
   uint8_t* const x_mem = smem + S::kRing + S::kRed + S::kLists;
   const int x_ld = S::x_ld(p.span);
-  float* const x_sum = reinterpret_cast<float*>(x_mem + S::kParts * p.cap * x_ld);  // [cap][groups, an odd number of floats]
+  float2* const x_sum = reinterpret_cast<float2*>(x_mem + p.cap * x_ld);  // (sum of the integers, f) [cap][groups, made odd]
   const int xs_ld = p.span / kChunk * kGpc | 1;
 
   // The down pass follows the gate_up pass, which lets it start only after its own wait: all but the intermediate is
@@ -365,33 +364,68 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
     const int chunks = (min(p.span, p.K - c0) + kChunk - 1) / kChunk;
     // sixteen threads take the sixteen 8-column units of a chunk of a token
     const int units = (n * chunks * 16 + 31) & ~31;
-#pragma unroll 4
+#pragma unroll 2
     for (int i = threadIdx.x; i < units; i += kThreads) {
       const int u = i & 15, row = min((i >> 4) / chunks, n - 1), c = (i >> 4) % chunks;
       const int col = c0 + c * kChunk + col_of<kGpc>(u >> 2, u & 3);
       long long r = base + row;
       if (kMode == kGateUp) r = lists.slots[r] / p.top_k;
       if (kMode == kDown) r = lists.slots[r];
-      float s = 0.f;
+      float x[8];
 #pragma unroll
-      for (int part = 0; part < S::kParts; ++part) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (col < p.K) v = *reinterpret_cast<const uint4*>(p.x + r * p.x_ld + part * p.K + col);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      for (int k = 0; k < 8; ++k) x[k] = 0.f;
+      if (col < p.K) {
+        if constexpr (kMode == kDown) {
+          const float* src = static_cast<const float*>(p.x) + r * p.x_ld + col;
+          const float4 lo = *reinterpret_cast<const float4*>(src), hi = *reinterpret_cast<const float4*>(src + 4);
+          x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w;
+          x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
+        } else {
+          const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.x) + r * p.x_ld + col);
+          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s += __uint_as_float(w[k] << 16) + __uint_as_float(w[k] & 0xffff0000u);
-        // (x0, x4), (x1, x5), (x2, x6), (x3, x7)
-        const uint4 o = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                                   __byte_perm(v.y, v.w, 0x7632));
-        *reinterpret_cast<uint4*>(x_mem + (part * p.cap + row) * x_ld + c * 256 + u * 16) = o;
+          for (int k = 0; k < 4; ++k) {
+            x[2 * k] = __uint_as_float(w[k] << 16);
+            x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+          }
+        }
       }
-      // the sum over the units of a group: four threads hold a word index, two word indices a group of 64
+      // largest magnitude of the group, as bits (which order like the values, NaN last): four threads hold a word index, two
+      // word indices a group of 64
+      uint32_t big = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) big = max(big, __float_as_uint(x[k]) & 0x7fffffffu);
+      big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      if (kGpc < 4) big = max(big, __shfl_xor_sync(0xffffffffu, big, 4));
+      if (kGpc < 2) big = max(big, __shfl_xor_sync(0xffffffffu, big, 8));
+      const int e = max(static_cast<int>(big >> 23), 20);  // biased exponent; what is below 2^-107 of nothing stays nothing
+      const float f = big >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __uint_as_float(static_cast<uint32_t>(e - 14) << 23);
+      const float to_int = __uint_as_float(static_cast<uint32_t>(254 + 14 - min(e, 254)) << 23);  // 2^(14 - exponent)
+      uint32_t v[8];
+      int s = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        // the integer in the low bits, rounded to nearest; an fp32 value may lie past 32767.5, a bf16 one does not
+        v[k] = __float_as_uint(kMode == kDown ? fminf(x[k] * to_int, 32767.f) + kFloatBias : fmaf(x[k], to_int, kFloatBias));
+        s += static_cast<int>(v[k]) - kFloatBits;
+      }
+      if (big >= 0x7f800000u) s = 0;
+      // bytes 1 (high) and 0 (low) of columns 0, 2, 4, 6 and of 1, 3, 5, 7
+      uint32_t o[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t a02 = __byte_perm(v[h], v[2 + h], 0x5410), a46 = __byte_perm(v[4 + h], v[6 + h], 0x5410);
+        o[h] = __byte_perm(a02, a46, 0x7531);
+        o[2 + h] = __byte_perm(a02, a46, 0x6420);
+      }
+      *reinterpret_cast<uint4*>(x_mem + row * x_ld + c * 256 + u * 16) = make_uint4(o[0], o[1], o[2], o[3]);
       s += __shfl_xor_sync(0xffffffffu, s, 1);
       s += __shfl_xor_sync(0xffffffffu, s, 2);
       if (kGpc < 4) s += __shfl_xor_sync(0xffffffffu, s, 4);
       if (kGpc < 2) s += __shfl_xor_sync(0xffffffffu, s, 8);
       constexpr int kUnits = 16 / kGpc;
-      if (u % kUnits == 0) x_sum[row * xs_ld + c * kGpc + u / kUnits] = s;
+      if (u % kUnits == 0) x_sum[row * xs_ld + c * kGpc + u / kUnits] = make_float2(static_cast<float>(s), f);
     }
   };
 
@@ -456,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   }
 
   // ------------------------------------------------------------------ products
-  const uint32_t mask = 0x000f000fu, magic = 0x43004300u;
+  const int start[4] = {kFloatBits, kFloatBits, kFloatBits, kFloatBits};
   const uint32_t fifo_lane = smem_u32(fifo) + g * 64;
   for (int block0 = first / p.row_tiles; block0 <= last_block;) {
     const int block1 = window_end(block0);
@@ -475,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
       const long long mat = first_row_of_matrix(block);
       // columns past the block's tokens are not written: they take the last one's activations
       const uint8_t* x_lane[kTB];
-      const float* xs_lane[kTB][2];
+      const float2* xs_lane[kTB][2];
 #pragma unroll
       for (int tb = 0; tb < kTB; ++tb) {
         x_lane[tb] = x_mem + (base - win_base + min(tb * 8 + g, n_tokens - 1)) * x_ld + t * 16;
@@ -506,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
         }
         fetched = false;
         const uint8_t* x_at[kTB];
-        const float* xs_at[kTB][2];
+        const float2* xs_at[kTB][2];
 #pragma unroll
         for (int tb = 0; tb < kTB; ++tb) {
           x_at[tb] = x_lane[tb] + begin * 256;
@@ -553,31 +587,27 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
             for (int q = 0; q < kSWords; ++q) s_cur[i][q] = s_next[i][q];
           }
           if (kSlot + 1 < left) fetch_scales(std::integral_constant<int, kSlot + 1>{});
-          float acc[kRB][kTB][4];
+          int high[kRB][kTB][4], low[kRB][kTB][4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             constexpr int kPer = 4 / kGpc;
-            uint4 b[S::kParts][kTB];
+            uint4 b[kTB];
 #pragma unroll
-            for (int part = 0; part < S::kParts; ++part)
-#pragma unroll
-              for (int tb = 0; tb < kTB; ++tb)
-                b[part][tb] = *reinterpret_cast<const uint4*>(x_at[tb] + part * p.cap * x_ld + kSlot * 256 + j * 64);
+            for (int tb = 0; tb < kTB; ++tb) b[tb] = *reinterpret_cast<const uint4*>(x_at[tb] + kSlot * 256 + j * 64);
 #pragma unroll
             for (int rb = 0; rb < kRB; ++rb) {
-              const uint32_t lo = w[2 * rb][j], hi = w[2 * rb + 1][j];
-              const uint32_t a0 = unpack<0>(lo, mask, magic), a1 = unpack<0>(hi, mask, magic);
-              const uint32_t a2 = unpack<1>(lo, mask, magic), a3 = unpack<1>(hi, mask, magic);
-              const uint32_t a4 = unpack<2>(lo, mask, magic), a5 = unpack<2>(hi, mask, magic);
-              const uint32_t a6 = unpack<3>(lo, mask, magic), a7 = unpack<3>(hi, mask, magic);
+              const uint32_t lo = w[2 * rb][j], hi = w[2 * rb + 1][j];  // rows g and g + 8
+              const uint32_t a[4] = {lo & 0x0f0f0f0fu, hi & 0x0f0f0f0fu, (lo >> 4) & 0x0f0f0f0fu, (hi >> 4) & 0x0f0f0f0fu};
 #pragma unroll
-              for (int part = 0; part < S::kParts; ++part)
-#pragma unroll
-                for (int tb = 0; tb < kTB; ++tb) {
-                  if (j % kPer == 0 && part == 0) mma_bf16_first(acc[rb][tb], a0, a1, a2, a3, b[part][tb].x, b[part][tb].y);
-                  else mma_bf16(acc[rb][tb], a0, a1, a2, a3, b[part][tb].x, b[part][tb].y);
-                  mma_bf16(acc[rb][tb], a4, a5, a6, a7, b[part][tb].z, b[part][tb].w);
+              for (int tb = 0; tb < kTB; ++tb) {
+                if (j % kPer == 0) {
+                  mma_codes<true>(high[rb][tb], a, b[tb].x, b[tb].y, start);
+                  mma_codes<false>(low[rb][tb], a, b[tb].z, b[tb].w, start);
+                } else {
+                  mma_codes<true>(high[rb][tb], a, b[tb].x, b[tb].y, high[rb][tb]);
+                  mma_codes<false>(low[rb][tb], a, b[tb].z, b[tb].w, low[rb][tb]);
                 }
+              }
             }
             if (j % kPer == kPer - 1) {
               constexpr int kLast = kPer - 1;
@@ -587,18 +617,20 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
               for (int i = 0; i < 2 * kRB; ++i) {
                 const uint32_t v = s_cur[i][q / 2];
                 s[i] = __uint_as_float(q & 1 ? v & 0xffff0000u : v << 16);
-                z[i] = -136.f;
-                if (kZero) z[i] = __uint_as_float(((z_cur[i] >> (8 * q)) & 15u) << 16 | 0xc3000000u);  // -(128 + zero)
+                z[i] = -8.f;
+                // -zero: 0xcb000000 are the bits of -8388608, one less for every unit
+                if (kZero) z[i] = __uint_as_float(((z_cur[i] >> (8 * q)) & 15u) | 0xcb000000u) + 8388608.f;
               }
 #pragma unroll
               for (int tb = 0; tb < kTB; ++tb) {
-                const float xs[2] = {xs_at[tb][0][kSlot * kGpc + q], xs_at[tb][1][kSlot * kGpc + q]};
+                const float2 xs[2] = {xs_at[tb][0][kSlot * kGpc + q], xs_at[tb][1][kSlot * kGpc + q]};
 #pragma unroll
                 for (int rb = 0; rb < kRB; ++rb)
 #pragma unroll
                   for (int i = 0; i < 4; ++i) {
                     const int r = 2 * rb + (i >> 1);
-                    tot[rb][tb][i] = fmaf(s[r], fmaf(z[r], xs[i & 1], acc[rb][tb][i]), tot[rb][tb][i]);
+                    const float sum = fmaf(__int_as_float(high[rb][tb][i]) - kFloatBias, 256.f, __int_as_float(low[rb][tb][i]) - kFloatBias);
+                    tot[rb][tb][i] = fmaf(s[r] * xs[i & 1].y, fmaf(z[r], xs[i & 1].x, sum), tot[rb][tb][i]);
                   }
               }
             }
@@ -656,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
           if (n >= n_tokens) continue;
           if (kMode == kGateUp) {
             const int I = p.rows >> 1;
-            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + static_cast<long long>(lists.slots[base + n]) * 2 * I;
+            float* dst = static_cast<float*>(p.out) + static_cast<long long>(lists.slots[base + n]) * I;
 #pragma unroll
             for (int rb = 0; rb < kRB; ++rb) {
               const int j = row0 + rb * 8 + g;
@@ -665,10 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
                 gate += __bfloat162float(p.w.bias[mat + j * step_row]);
                 up += __bfloat162float(p.w.bias[mat + j * step_row + step_half]);
               }
-              const float v = w4_act(gate, up, p.activation);
-              const __nv_bfloat16 v_hi = __float2bfloat16_rn(v);
-              dst[j] = v_hi;
-              dst[I + j] = __float2bfloat16_rn(v - __bfloat162float(v_hi));
+              dst[j] = w4_act(gate, up, p.activation);
             }
           } else {
             const int s = kMode == kDense ? base + n : lists.slots[base + n];
@@ -757,8 +786,8 @@ W4Split split_of(const W4Params& p, long long blocks) {
     const double rounds = std::max(std::ceil(per_cta / (kWarps >> lg)), per_cta / (kWarps >> lg) + 0.5 * windows);
     const double steps = (spans - 1.0) * ((span_chunks + (1 << lg) - 1) >> lg) + ((last_chunks + (1 << lg) - 1) >> lg);
     const double x_loads = spans > 1 ? rounds * spans : windows;
-    const double cost = rounds * (steps * 1100 * kRB * (1 + 0.4 * (S::kParts * kTB - 1)) + 3000) +
-                        x_loads * (1500 + rows_a_window * S::kParts * r.span * 2 / 64.0);
+    const double cost = rounds * (steps * 1100 * kRB * (1 + 0.4 * (kTB - 1)) + 3000) +
+                        x_loads * (1500 + rows_a_window * (kMode == kDown ? 4 : 2) * r.span / 64.0);
     if (r.cost < 0 || cost < r.cost) {
       r.cost = cost;
       r.wk_log2 = lg;
@@ -836,14 +865,14 @@ int launch_w4_experts(__nv_bfloat16* out, const __nv_bfloat16* x, const W4Matrix
     const int tt = T - t0 < piece ? T - t0 : piece;
     const int slots = tt * top_k;
     const int* ids = topk_ids + static_cast<long long>(t0) * top_k;
-    __nv_bfloat16* h = static_cast<__nv_bfloat16*>(workspace);
-    float* c3 = reinterpret_cast<float*>(h + static_cast<size_t>(slots) * 2 * I);
+    float* h = static_cast<float*>(workspace);
+    float* c3 = h + static_cast<size_t>(slots) * I;
     const int blocks = expected_blocks(slots, E);
     W4Params p{};
     p.w = w13; p.rows = 2 * I; p.K = H; p.x = x + static_cast<long long>(t0) * H; p.x_ld = H; p.m = slots; p.ids = ids; p.top_k = top_k;
     p.E = E; p.activation = activation; p.out = h;
     if (int st = check_cuda(launch_mode<kGateUp, 1>(p, blocks, stream), "w4 gate_up launch")) return st;
-    p.w = w2; p.rows = H; p.K = I; p.x = h; p.x_ld = 2 * I; p.topk_w = topk_w + static_cast<long long>(t0) * top_k; p.out = c3;
+    p.w = w2; p.rows = H; p.K = I; p.x = h; p.x_ld = I; p.topk_w = topk_w + static_cast<long long>(t0) * top_k; p.out = c3;
     if (int st = check_cuda(launch_mode<kDown, 1>(p, blocks, stream), "w4 down launch")) return st;
     if (int st = check_cuda(launch_pdl(w4_sum_kernel, dim3((H / 4 + 255) / 256, tt), dim3(256), 0, stream,
                                        out + static_cast<long long>(t0) * H, c3, ids, E, top_k, H), "w4 sum launch"))
