@@ -249,8 +249,10 @@ int moe_b200_router_backward(void* grad_logits, const void* gating, int gating_i
  *   out bf16 [M, N] = x @ W^T + bias;  x bf16, rows x_row_stride elements apart (a multiple of 8)
  * group_size 32, 64 or 128 and K % group_size == 0; any N. fp32 sums, one rounding. qweight and x on 16 bytes.
  */
+size_t moe_b200_w4_linear_workspace_bytes(int M, int K, int group_size); /* 0: none needed */
 int moe_b200_w4_linear(void* out, const void* x, int64_t x_row_stride, const void* qweight, const void* scale,
-                       const void* zero, const void* bias, int M, int N, int K, int group_size, void* stream);
+                       const void* zero, const void* bias, int M, int N, int K, int group_size, void* workspace,
+                       size_t workspace_bytes, void* stream);
 /*
  * fused_experts with such weights: w13 codes [E, 2*I, H/2] (gate rows then up rows, interleaved for
  * MOE_B200_ACT_SWIGLUOAI), w2 codes [E, H, I/2], scales [E, 2*I, H/g] and [E, H, I/g], zeros alike or NULL, biases bf16

@@ -74,7 +74,8 @@ SIGNATURES = {
     "moe_b200_router_loss_workspace_bytes": (c_size_t, [c_int, c_int]),
     "moe_b200_router_loss": (c_int, [c_void_p] * 5 + [c_int, c_void_p, c_void_p] + [c_int] * 3 + [c_void_p, c_size_t, c_void_p]),
     "moe_b200_router_backward": (c_int, [c_void_p, c_void_p, c_int] + [c_void_p] * 6 + [c_int] * 4 + [c_void_p]),
-    "moe_b200_w4_linear": (c_int, [c_void_p, c_void_p, c_int64] + [c_void_p] * 4 + [c_int] * 4 + [c_void_p]),
+    "moe_b200_w4_linear_workspace_bytes": (c_size_t, [c_int] * 3),
+    "moe_b200_w4_linear": (c_int, [c_void_p, c_void_p, c_int64] + [c_void_p] * 4 + [c_int] * 4 + [c_void_p, c_size_t, c_void_p]),
     "moe_b200_fused_experts_w4_workspace_bytes": (c_size_t, [c_int] * 5),
     "moe_b200_fused_experts_w4": (c_int, [c_void_p] * 12 + [c_int] * 7 + [c_void_p, c_size_t, c_void_p]),
     "moe_b200_quant_fp8_per_token_group": (c_int, [c_void_p, c_int, c_int, c_void_p, POINTER(c_float), c_void_p]),

@@ -513,8 +513,14 @@ int moe_b200_router_backward(void* grad_logits, const void* gating, int gating_i
                                 grad_topk_weights, token_mask, T, E, k, renormalize, static_cast<cudaStream_t>(stream));
 }
 
+size_t moe_b200_w4_linear_workspace_bytes(int M, int K, int group_size) {
+  if (M <= 0 || K <= 0 || (group_size != 32 && group_size != 64 && group_size != 128)) return 0;
+  return w4_linear_workspace_bytes(M, K, group_size);
+}
+
 int moe_b200_w4_linear(void* out, const void* x, int64_t x_row_stride, const void* qweight, const void* scale,
-                       const void* zero, const void* bias, int M, int N, int K, int group_size, void* stream) {
+                       const void* zero, const void* bias, int M, int N, int K, int group_size, void* workspace,
+                       size_t workspace_bytes, void* stream) {
   if (M < 0 || N <= 0) return set_error(kStatusInvalidArgument, "w4_linear: bad sizes M=%d N=%d", M, N);
   if (int st = check_w4_group("w4_linear", group_size, K)) return st;
   if (M == 0) return kStatusOk;
@@ -522,8 +528,11 @@ int moe_b200_w4_linear(void* out, const void* x, int64_t x_row_stride, const voi
     return set_error(kStatusInvalidArgument, "w4_linear: null pointer");
   if (!aligned(x, 16) || !aligned(qweight, 16) || (M > 1 && (x_row_stride % 8 != 0 || x_row_stride < K)))
     return set_error(kStatusInvalidArgument, "w4_linear: x and qweight must start on 16 bytes and the rows of x lie a multiple of 8 elements, at least K, apart");
+  const size_t need = w4_linear_workspace_bytes(M, K, group_size);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
+    return set_error(kStatusWorkspaceTooSmall, "w4_linear: workspace of %zu bytes on 16 needed, %zu given", need, workspace_bytes);
   return launch_w4_linear(static_cast<__nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(x), x_row_stride,
-                          w4_matrix(qweight, scale, zero, bias, group_size), M, N, K, static_cast<cudaStream_t>(stream));
+                          w4_matrix(qweight, scale, zero, bias, group_size), M, N, K, workspace, static_cast<cudaStream_t>(stream));
 }
 
 size_t moe_b200_fused_experts_w4_workspace_bytes(int T, int E, int top_k, int H, int I) {

@@ -125,8 +125,9 @@ struct W4Matrix {
   const __nv_bfloat16* bias;
   int group;
 };
+size_t w4_linear_workspace_bytes(int M, int K, int group);
 int launch_w4_linear(__nv_bfloat16* out, const __nv_bfloat16* x, long long x_ld, const W4Matrix& w, int M, int N, int K,
-                     cudaStream_t stream);
+                     void* workspace, cudaStream_t stream);
 size_t w4_experts_workspace_bytes(int T, int top_k, int H, int I);
 int launch_w4_experts(__nv_bfloat16* out, const __nv_bfloat16* x, const W4Matrix& w13, const W4Matrix& w2, const float* topk_w,
                       const int* topk_ids, int T, int E, int top_k, int H, int I, int activation, void* workspace,

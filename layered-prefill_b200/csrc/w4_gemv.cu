@@ -10,12 +10,14 @@
 // The integer form (m16n8k32, u8 codes) takes codes as they are: three instructions unpack eight of them (w & 0x0f0f0f0f and
 // (w >> 4) & 0x0f0f0f0f), against seven to bf16 (shift, mask and a 128 that has to leave the sum again), and one instruction multiplies
 // 32 columns instead of 16 at the same rate. Unpacking is what bounds the loop next to the loads.
-//   The activations become 16-bit integers with a power of two f for every token and group of columns:
-//   x = f * (256 hi + lo), hi signed and lo unsigned bytes, two products a word; f puts the group's largest |x| between 2^14 and 2^15.
-//   A bf16 value has 8 significant bits, so that all within 2^7 of the group's largest are exact and smaller ones are off by at most
+//   The activations become 16-bit integers with a power of two f for every token and 128 columns:
+//   x = f * (256 hi + lo), hi signed and lo unsigned bytes, two products a word; f puts the largest |x| of them between 2^14 and 2^15.
+//   A bf16 value has 8 significant bits, so that all within 2^7 of the largest are exact and smaller ones are off by at most
 //   2^-16 of the largest; the intermediate h of the experts (fp32) is off by that everywhere. Integer sums are exact; then
 //   sum (code - zero) x = f * (256 sum code hi + sum code lo - zero * sum x) in fp32, times the group's scale, summed in fp32.
-//   A group with a value that is not finite gets f = NaN, so that its token's results are NaN.
+//   Where a value is not finite f is NaN, so that its token's results are NaN.
+//   A CTA makes these integers itself where they are few; where many CTAs would make many of them (a batch, a long K) a kernel in
+//   front does it once, while this one prepares its lists and its first codes.
 // The sums start at 0x4b400000, which makes their bits the float 12582912 + sum: no conversion instruction.
 //
 // Work: a tile is 16 * kRB weight rows x one block of up to 8 * kTB tokens; a CTA takes consecutive tiles, so that it
@@ -42,6 +44,7 @@ constexpr int kChunk = 128;         // columns of a step
 constexpr int kStages = 4;          // steps in a warp's FIFO
 constexpr int kListSlots = 1024;    // slots whose lists are built in shared memory
 constexpr int kListExperts = 1024;
+constexpr size_t kPreparedChunks = 64;
 constexpr int kMaxSmem = 227 * 1024 - 128;  // dynamic; the sort has a few words of its own
 
 enum W4Mode { kDense = 0, kGateUp = 1, kDown = 2 };
@@ -64,6 +67,8 @@ struct W4Params {
   int E;
   int activation;
   const float* topk_w;
+  const uint8_t* xq;      // integers made in front (quant_x_kernel), or null
+  const float* xm;
   void* out;              // dense bf16 [m][rows]; gate_up fp32 [slots][I]; down fp32 [slots][rows]
 };
 
@@ -206,7 +211,7 @@ struct W4Shape {
   // a token row of `span` columns: 64 bytes more than a multiple of 128, so that the two tokens of an eight-lane phase of a
   // 16-byte read use different banks
   __host__ __device__ static constexpr int x_ld(int span) { return span * 2 + 64; }
-  __host__ __device__ static constexpr int x_row_bytes(int span, int gpc) { return x_ld(span) + (span / kChunk * gpc | 1) * 8; }
+  __host__ __device__ static constexpr int x_row_bytes(int span, int gpc) { return x_ld(span) + (span / kChunk * (gpc + 1) | 1) * 4; }
   static constexpr int kFixed = kRing + kRed + kLists;
 };
 
@@ -215,6 +220,81 @@ struct W4Shape {
 template <int kGpc>
 __device__ __forceinline__ int col_of(int j, int t) {
   return kGpc == 1 ? 32 * t + 8 * j : (kGpc == 2 ? 64 * (j >> 1) + 16 * t + 8 * (j & 1) : 32 * j + 8 * t);
+}
+
+// The integers of 128 columns of a token by sixteen neighbouring lanes, lane u holding the eight columns from col_of(u / 4, u % 4) on.
+// ints: bytes 1 (high) of columns 0, 2, 4, 6 and of 1, 3, 5, 7, then bytes 0; sum: of its group; returns f.
+template <int kGpc, bool kFp32>
+__device__ __forceinline__ float quant_x(const float (&x)[8], uint4& ints, int& sum) {
+  uint32_t big = 0;  // the largest magnitude as bits, which order like the values, NaN last
+#pragma unroll
+  for (int k = 0; k < 8; ++k) big = max(big, __float_as_uint(x[k]) & 0x7fffffffu);
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, m));
+  const bool finite = big < 0x7f800000u;
+  const int e = min(max(static_cast<int>(big >> 23), 20), 254);  // biased exponent; 2^-107 and less count as that
+  const float to_int = __uint_as_float(static_cast<uint32_t>(254 + 14 - e) << 23);  // 2^(14 - exponent)
+  uint32_t v[8];
+  sum = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    // the integer in the low bits, rounded to nearest; an fp32 value may lie past 32767.5, a bf16 one does not
+    v[k] = __float_as_uint(kFp32 ? fminf(x[k] * to_int, 32767.f) + kFloatBias : fmaf(x[k], to_int, kFloatBias));
+    sum += static_cast<int>(v[k]) - kFloatBits;
+  }
+  uint32_t o[4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t a02 = __byte_perm(v[h], v[2 + h], 0x5410), a46 = __byte_perm(v[4 + h], v[6 + h], 0x5410);
+    o[h] = __byte_perm(a02, a46, 0x7531);
+    o[2 + h] = __byte_perm(a02, a46, 0x6420);
+  }
+  ints = make_uint4(o[0], o[1], o[2], o[3]);
+  if (!finite) sum = 0;
+  sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+  if (kGpc < 4) sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+  if (kGpc < 2) sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+  return finite ? __uint_as_float(static_cast<uint32_t>(e - 14) << 23) : __uint_as_float(0x7fffffffu);
+}
+
+__device__ __forceinline__ void load_x8(const __nv_bfloat16* src, float (&x)[8]) {
+  const uint4 q = *reinterpret_cast<const uint4*>(src);
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    x[2 * k] = __uint_as_float(w[k] << 16);
+    x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void load_x8(const float* src, float (&x)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+
+// xq [rows][chunks][256] and xm [rows][chunks][kGpc + 1] (the groups' sums, f) of bf16 rows.
+template <int kGpc>
+__global__ void __launch_bounds__(256)
+quant_x_kernel(uint8_t* __restrict__ xq, float* __restrict__ xm, const __nv_bfloat16* __restrict__ x, long long x_ld, int rows, int K) {
+  grid_dependency_wait();
+  grid_dependency_launch();
+  const int chunks = (K + kChunk - 1) / kChunk;
+  const long long at = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 4;  // chunk of a row
+  const int u = threadIdx.x & 15;
+  const bool ok = at < static_cast<long long>(rows) * chunks;
+  const int row = ok ? static_cast<int>(at / chunks) : 0, c = ok ? static_cast<int>(at % chunks) : 0;
+  const int col = c * kChunk + col_of<kGpc>(u >> 2, u & 3);
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (col < K) load_x8(x + row * x_ld + col, v);
+  uint4 ints;
+  int sum;
+  const float f = quant_x<kGpc, false>(v, ints, sum);
+  if (!ok) return;
+  *reinterpret_cast<uint4*>(xq + at * 256 + u * 16) = ints;
+  constexpr int kUnits = 16 / kGpc;
+  if (u % kUnits == 0) xm[at * (kGpc + 1) + u / kUnits] = static_cast<float>(sum);
+  if (u == 0) xm[at * (kGpc + 1) + kGpc] = f;
 }
 
 template <int kMode, int kRB, int kTB, int kGpc, bool kZero>
@@ -232,12 +312,14 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   SlotLists& lists = *reinterpret_cast<SlotLists*>(smem + S::kRing + S::kRed);
   uint8_t* const x_mem = smem + S::kRing + S::kRed + S::kLists;
   const int x_ld = S::x_ld(p.span);
-  float2* const x_sum = reinterpret_cast<float2*>(x_mem + p.cap * x_ld);  // (sum of the integers, f) [cap][groups, made odd]
-  const int xs_ld = p.span / kChunk * kGpc | 1;
+  float* const x_sum = reinterpret_cast<float*>(x_mem + p.cap * x_ld);  // [cap][chunks][kGpc sums of the integers, f], rows of an odd length
+  const int xs_ld = p.span / kChunk * (kGpc + 1) | 1;
 
-  // The down pass follows the gate_up pass, which lets it start only after its own wait: all but the intermediate is
-  // there already, so that the lists are made and the first codes are under way before the wait.
-  if (kMode != kDown) {
+  // The down pass follows the gate_up pass, and a pass with prepared integers the kernel that makes them, and both let this one
+  // start only after their own wait: all but what they write is there already, so that the lists are made and the first codes
+  // are under way before the wait.
+  const bool early = kMode == kDown || p.xq != nullptr;
+  if (!early) {
     grid_dependency_wait();
     grid_dependency_launch();
   }
@@ -254,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   const long long total = static_cast<long long>(blocks) * p.row_tiles;
   const int first = static_cast<int>(total * blockIdx.x / gridDim.x), last = static_cast<int>(total * (blockIdx.x + 1) / gridDim.x);
   if (first == last) {
-    if (kMode == kDown) grid_dependency_wait();
+    if (early) grid_dependency_wait();
     return;
   }
 
@@ -362,70 +444,42 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   auto load_x = [&](int base, int n, int span_i) {
     const int c0 = span_i * p.span;
     const int chunks = (min(p.span, p.K - c0) + kChunk - 1) / kChunk;
-    // sixteen threads take the sixteen 8-column units of a chunk of a token
-    const int units = (n * chunks * 16 + 31) & ~31;
-#pragma unroll 2
-    for (int i = threadIdx.x; i < units; i += kThreads) {
-      const int u = i & 15, row = min((i >> 4) / chunks, n - 1), c = (i >> 4) % chunks;
-      const int col = c0 + c * kChunk + col_of<kGpc>(u >> 2, u & 3);
-      long long r = base + row;
-      if (kMode == kGateUp) r = lists.slots[r] / p.top_k;
-      if (kMode == kDown) r = lists.slots[r];
-      float x[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = 0.f;
-      if (col < p.K) {
-        if constexpr (kMode == kDown) {
-          const float* src = static_cast<const float*>(p.x) + r * p.x_ld + col;
-          const float4 lo = *reinterpret_cast<const float4*>(src), hi = *reinterpret_cast<const float4*>(src + 4);
-          x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w;
-          x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
-        } else {
-          const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.x) + r * p.x_ld + col);
-          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            x[2 * k] = __uint_as_float(w[k] << 16);
-            x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-          }
-        }
+    auto source_row = [&](int row) -> long long {
+      if (kMode == kDense) return base + row;
+      return kMode == kGateUp ? lists.slots[base + row] / p.top_k : lists.slots[base + row];
+    };
+    // half a warp takes a chunk of a token
+    int row = 0, c = warp * 2 + (lane >> 4);
+    const int u = lane & 15;
+    for (int at = warp * 2; at < n * chunks; at += 2 * kWarps) {
+      while (c >= chunks) {
+        c -= chunks;
+        ++row;
       }
-      // largest magnitude of the group, as bits (which order like the values, NaN last): four threads hold a word index, two
-      // word indices a group of 64
-      uint32_t big = 0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) big = max(big, __float_as_uint(x[k]) & 0x7fffffffu);
-      big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
-      big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      if (kGpc < 4) big = max(big, __shfl_xor_sync(0xffffffffu, big, 4));
-      if (kGpc < 2) big = max(big, __shfl_xor_sync(0xffffffffu, big, 8));
-      const int e = max(static_cast<int>(big >> 23), 20);  // biased exponent; what is below 2^-107 of nothing stays nothing
-      const float f = big >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __uint_as_float(static_cast<uint32_t>(e - 14) << 23);
-      const float to_int = __uint_as_float(static_cast<uint32_t>(254 + 14 - min(e, 254)) << 23);  // 2^(14 - exponent)
-      uint32_t v[8];
-      int s = 0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        // the integer in the low bits, rounded to nearest; an fp32 value may lie past 32767.5, a bf16 one does not
-        v[k] = __float_as_uint(kMode == kDown ? fminf(x[k] * to_int, 32767.f) + kFloatBias : fmaf(x[k], to_int, kFloatBias));
-        s += static_cast<int>(v[k]) - kFloatBits;
+      const int r = min(row, n - 1);  // behind the last chunk: one of the last token again
+      if (kMode != kDown && p.xq != nullptr) {
+        const int all = (p.K + kChunk - 1) / kChunk;
+        const long long src = source_row(r) * all + c0 / kChunk + c;
+        cp_async_16(smem_u32(x_mem + r * x_ld + c * 256 + u * 16), p.xq + src * 256 + u * 16, 16);
+        if (u <= kGpc) x_sum[r * xs_ld + c * (kGpc + 1) + u] = p.xm[src * (kGpc + 1) + u];
+      } else {
+        const int col = c0 + c * kChunk + col_of<kGpc>(u >> 2, u & 3);
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        using X = std::conditional_t<kMode == kDown, float, __nv_bfloat16>;
+        if (col < p.K) load_x8(static_cast<const X*>(p.x) + source_row(r) * p.x_ld + col, v);
+        uint4 ints;
+        int sum;
+        const float f = quant_x<kGpc, kMode == kDown>(v, ints, sum);
+        *reinterpret_cast<uint4*>(x_mem + r * x_ld + c * 256 + u * 16) = ints;
+        constexpr int kUnits = 16 / kGpc;
+        if (u % kUnits == 0) x_sum[r * xs_ld + c * (kGpc + 1) + u / kUnits] = static_cast<float>(sum);
+        if (u == 0) x_sum[r * xs_ld + c * (kGpc + 1) + kGpc] = f;
       }
-      if (big >= 0x7f800000u) s = 0;
-      // bytes 1 (high) and 0 (low) of columns 0, 2, 4, 6 and of 1, 3, 5, 7
-      uint32_t o[4];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t a02 = __byte_perm(v[h], v[2 + h], 0x5410), a46 = __byte_perm(v[4 + h], v[6 + h], 0x5410);
-        o[h] = __byte_perm(a02, a46, 0x7531);
-        o[2 + h] = __byte_perm(a02, a46, 0x6420);
-      }
-      *reinterpret_cast<uint4*>(x_mem + row * x_ld + c * 256 + u * 16) = make_uint4(o[0], o[1], o[2], o[3]);
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      if (kGpc < 4) s += __shfl_xor_sync(0xffffffffu, s, 4);
-      if (kGpc < 2) s += __shfl_xor_sync(0xffffffffu, s, 8);
-      constexpr int kUnits = 16 / kGpc;
-      if (u % kUnits == 0) x_sum[row * xs_ld + c * kGpc + u / kUnits] = make_float2(static_cast<float>(s), f);
+      c += 2 * kWarps;
+    }
+    if (kMode != kDown && p.xq != nullptr) {
+      cp_async_commit();
+      cp_async_wait_all();
     }
   };
 
@@ -484,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   load_chunk(std::integral_constant<int, 0>{});
   load_chunk(std::integral_constant<int, 1>{});
   load_chunk(std::integral_constant<int, 2>{});
-  if (kMode == kDown) {
+  if (early) {
     grid_dependency_wait();
     grid_dependency_launch();
   }
@@ -509,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
       const long long mat = first_row_of_matrix(block);
       // columns past the block's tokens are not written: they take the last one's activations
       const uint8_t* x_lane[kTB];
-      const float2* xs_lane[kTB][2];
+      const float* xs_lane[kTB][2];
 #pragma unroll
       for (int tb = 0; tb < kTB; ++tb) {
         x_lane[tb] = x_mem + (base - win_base + min(tb * 8 + g, n_tokens - 1)) * x_ld + t * 16;
@@ -540,12 +594,12 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
         }
         fetched = false;
         const uint8_t* x_at[kTB];
-        const float2* xs_at[kTB][2];
+        const float* xs_at[kTB][2];
 #pragma unroll
         for (int tb = 0; tb < kTB; ++tb) {
           x_at[tb] = x_lane[tb] + begin * 256;
-          xs_at[tb][0] = xs_lane[tb][0] + begin * kGpc;
-          xs_at[tb][1] = xs_lane[tb][1] + begin * kGpc;
+          xs_at[tb][0] = xs_lane[tb][0] + begin * (kGpc + 1);
+          xs_at[tb][1] = xs_lane[tb][1] + begin * (kGpc + 1);
         }
         auto chunk = [&](auto slot_c) {  // the products of chunk kSlot of four
           constexpr int kSlot = decltype(slot_c)::value;
@@ -588,6 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
           }
           if (kSlot + 1 < left) fetch_scales(std::integral_constant<int, kSlot + 1>{});
           int high[kRB][kTB][4], low[kRB][kTB][4];
+          float part[kRB][kTB][4];  // of the chunk, in units of f
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             constexpr int kPer = 4 / kGpc;
@@ -617,24 +672,38 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
               for (int i = 0; i < 2 * kRB; ++i) {
                 const uint32_t v = s_cur[i][q / 2];
                 s[i] = __uint_as_float(q & 1 ? v & 0xffff0000u : v << 16);
-                z[i] = -8.f;
                 // -zero: 0xcb000000 are the bits of -8388608, one less for every unit
                 if (kZero) z[i] = __uint_as_float(((z_cur[i] >> (8 * q)) & 15u) | 0xcb000000u) + 8388608.f;
               }
 #pragma unroll
-              for (int tb = 0; tb < kTB; ++tb) {
-                const float2 xs[2] = {xs_at[tb][0][kSlot * kGpc + q], xs_at[tb][1][kSlot * kGpc + q]};
+              for (int tb = 0; tb < kTB; ++tb)
 #pragma unroll
-                for (int rb = 0; rb < kRB; ++rb)
+                for (int o = 0; o < 2; ++o) {
+                  const float xs = xs_at[tb][o][kSlot * (kGpc + 1) + q];
+                  const float off = fmaf(8.f, xs, kFloatBias);
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    const int r = 2 * rb + (i >> 1);
-                    const float sum = fmaf(__int_as_float(high[rb][tb][i]) - kFloatBias, 256.f, __int_as_float(low[rb][tb][i]) - kFloatBias);
-                    tot[rb][tb][i] = fmaf(s[r] * xs[i & 1].y, fmaf(z[r], xs[i & 1].x, sum), tot[rb][tb][i]);
+                  for (int i = 0; i < 2 * kRB; ++i) {
+                    // 256 times the high sum, exactly; the low sum still has its bias, which leaves with the zero point's share
+                    const float sum = fmaf(__int_as_float(high[i >> 1][tb][2 * (i & 1) + o]), 256.f, -256.f * kFloatBias) +
+                                      __int_as_float(low[i >> 1][tb][2 * (i & 1) + o]);
+                    const float v = kZero ? fmaf(z[i], xs, sum - kFloatBias) : sum - off;
+                    float& acc = part[i >> 1][tb][2 * (i & 1) + o];
+                    acc = q == 0 ? s[i] * v : fmaf(s[i], v, acc);
                   }
-              }
+                }
             }
           }
+#pragma unroll
+          for (int tb = 0; tb < kTB; ++tb)
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+              const float f = xs_at[tb][o][kSlot * (kGpc + 1) + kGpc];
+#pragma unroll
+              for (int i = 0; i < 2 * kRB; ++i) {
+                float& sum = tot[i >> 1][tb][2 * (i & 1) + o];
+                sum = fmaf(f, part[i >> 1][tb][2 * (i & 1) + o], sum);
+              }
+            }
         };
 #pragma unroll 1
         for (; left > 0; left -= kStages) {
@@ -645,8 +714,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
 #pragma unroll
           for (int tb = 0; tb < kTB; ++tb) {
             x_at[tb] += kStages * 256;
-            xs_at[tb][0] += kStages * kGpc;
-            xs_at[tb][1] += kStages * kGpc;
+            xs_at[tb][0] += kStages * (kGpc + 1);
+            xs_at[tb][1] += kStages * (kGpc + 1);
           }
 #pragma unroll
           for (int i = 0; i < 2 * kRB; ++i) s_src[i] += kStages * kGpc;
@@ -819,39 +888,66 @@ cudaError_t launch_split(W4Params p, const W4Split& s, cudaStream_t stream) {
 }
 
 template <int kMode, int kTB, int kGpc>
-cudaError_t launch_groups(const W4Params& p, long long blocks, cudaStream_t stream) {
+cudaError_t launch_groups(W4Params p, long long blocks, int x_rows, void* xq, cudaStream_t stream) {
+  if (xq != nullptr) {
+    const long long chunks = static_cast<long long>(x_rows) * ((p.K + kChunk - 1) / kChunk);
+    p.xq = static_cast<uint8_t*>(xq);
+    p.xm = reinterpret_cast<float*>(static_cast<uint8_t*>(xq) + chunks * 256);
+    const cudaError_t e = launch_pdl(quant_x_kernel<kGpc>, dim3(static_cast<unsigned>((chunks + 15) / 16)), dim3(256), 0, stream,
+                                     static_cast<uint8_t*>(xq), const_cast<float*>(p.xm), static_cast<const __nv_bfloat16*>(p.x),
+                                     p.x_ld, x_rows, p.K);
+    if (e != cudaSuccess) return e;
+    count_launches(1);
+  }
   const W4Split one = split_of<kMode, 1, kTB, kGpc>(p, blocks), two = split_of<kMode, 2, kTB, kGpc>(p, blocks);
   if (one.cost < two.cost)
     return p.w.zero != nullptr ? launch_split<kMode, 1, kTB, kGpc, true>(p, one, stream) : launch_split<kMode, 1, kTB, kGpc, false>(p, one, stream);
   return p.w.zero != nullptr ? launch_split<kMode, 2, kTB, kGpc, true>(p, two, stream) : launch_split<kMode, 2, kTB, kGpc, false>(p, two, stream);
 }
 
+// x_rows, xq: rows of bf16 activations and room for their integers, or null
 template <int kMode, int kTB>
-cudaError_t launch_mode(const W4Params& p, long long blocks, cudaStream_t stream) {
-  if (p.w.group == 128) return launch_groups<kMode, kTB, 1>(p, blocks, stream);
-  if (p.w.group == 64) return launch_groups<kMode, kTB, 2>(p, blocks, stream);
-  return launch_groups<kMode, kTB, 4>(p, blocks, stream);
+cudaError_t launch_mode(const W4Params& p, long long blocks, int x_rows, void* xq, cudaStream_t stream) {
+  if (p.w.group == 128) return launch_groups<kMode, kTB, 1>(p, blocks, x_rows, xq, stream);
+  if (p.w.group == 64) return launch_groups<kMode, kTB, 2>(p, blocks, x_rows, xq, stream);
+  return launch_groups<kMode, kTB, 4>(p, blocks, x_rows, xq, stream);
+}
+
+// Room for the integers of `rows` activations of K columns, 0 where the CTAs make them themselves: with up to 16 chunks of
+// 128 columns (one turn of half the warps of a CTA) the kernel in front takes longer than it saves.
+size_t prepared_bytes(int rows, int K, int group) {
+  const size_t chunks = static_cast<size_t>(rows) * ((K + kChunk - 1) / kChunk);
+  return chunks <= kPreparedChunks ? 0 : chunks * (256 + 4 * (kChunk / group + 1));
 }
 
 }  // namespace
 
-int launch_w4_linear(__nv_bfloat16* out, const __nv_bfloat16* x, long long x_ld, const W4Matrix& w, int M, int N, int K, cudaStream_t stream) {
+size_t w4_linear_workspace_bytes(int M, int K, int group) { return prepared_bytes(M, K, group); }
+
+int launch_w4_linear(__nv_bfloat16* out, const __nv_bfloat16* x, long long x_ld, const W4Matrix& w, int M, int N, int K,
+                     void* workspace, cudaStream_t stream) {
   if (M == 0) return kStatusOk;
   W4Params p{};
   p.w = w; p.rows = N; p.K = K; p.x = x; p.x_ld = x_ld; p.m = M; p.out = out;
   const int tb = M <= 8 ? 1 : 2;
   const long long blocks = (M + 8 * tb - 1) / (8 * tb);
   if (blocks * ((N + 15) / 16) > 0x3fffffffll) return set_error(kStatusInvalidArgument, "w4_linear: M x N too large");
-  const cudaError_t e = tb == 1 ? launch_mode<kDense, 1>(p, blocks, stream) : launch_mode<kDense, 2>(p, blocks, stream);
+  void* xq = prepared_bytes(M, K, w.group) > 0 ? workspace : nullptr;
+  const cudaError_t e = tb == 1 ? launch_mode<kDense, 1>(p, blocks, M, xq, stream) : launch_mode<kDense, 2>(p, blocks, M, xq, stream);
   if (int st = check_cuda(e, "w4_linear launch")) return st;
   count_launches(1);
   return check_launch("w4_linear");
 }
 
+namespace {
+size_t w4_aligned(size_t v) { return (v + 255) / 256 * 256; }
+}  // namespace
+
 size_t w4_experts_workspace_bytes(int T, int top_k, int H, int I) {
   const int piece = top_k < kListSlots ? kListSlots / top_k : 1;
-  const size_t slots = static_cast<size_t>(T < 1 ? 1 : (T < piece ? T : piece)) * top_k;
-  return slots * (4 * static_cast<size_t>(I) + 4 * static_cast<size_t>(H));
+  const int tt = T < 1 ? 1 : (T < piece ? T : piece);
+  const size_t slots = static_cast<size_t>(tt) * top_k;
+  return w4_aligned(slots * 4 * I) + w4_aligned(slots * 4 * H) + prepared_bytes(tt, H, 32);
 }
 
 int launch_w4_experts(__nv_bfloat16* out, const __nv_bfloat16* x, const W4Matrix& w13, const W4Matrix& w2, const float* topk_w,
@@ -865,15 +961,17 @@ int launch_w4_experts(__nv_bfloat16* out, const __nv_bfloat16* x, const W4Matrix
     const int tt = T - t0 < piece ? T - t0 : piece;
     const int slots = tt * top_k;
     const int* ids = topk_ids + static_cast<long long>(t0) * top_k;
-    float* h = static_cast<float*>(workspace);
-    float* c3 = h + static_cast<size_t>(slots) * I;
+    uint8_t* at = static_cast<uint8_t*>(workspace);
+    float* h = reinterpret_cast<float*>(at);
+    float* c3 = reinterpret_cast<float*>(at += w4_aligned(static_cast<size_t>(slots) * 4 * I));
+    void* xq = prepared_bytes(tt, H, w13.group) > 0 ? at + w4_aligned(static_cast<size_t>(slots) * 4 * H) : nullptr;
     const int blocks = expected_blocks(slots, E);
     W4Params p{};
     p.w = w13; p.rows = 2 * I; p.K = H; p.x = x + static_cast<long long>(t0) * H; p.x_ld = H; p.m = slots; p.ids = ids; p.top_k = top_k;
     p.E = E; p.activation = activation; p.out = h;
-    if (int st = check_cuda(launch_mode<kGateUp, 1>(p, blocks, stream), "w4 gate_up launch")) return st;
+    if (int st = check_cuda(launch_mode<kGateUp, 1>(p, blocks, tt, xq, stream), "w4 gate_up launch")) return st;
     p.w = w2; p.rows = H; p.K = I; p.x = h; p.x_ld = I; p.topk_w = topk_w + static_cast<long long>(t0) * top_k; p.out = c3;
-    if (int st = check_cuda(launch_mode<kDown, 1>(p, blocks, stream), "w4 down launch")) return st;
+    if (int st = check_cuda(launch_mode<kDown, 1>(p, blocks, 0, nullptr, stream), "w4 down launch")) return st;
     if (int st = check_cuda(launch_pdl(w4_sum_kernel, dim3((H / 4 + 255) / 256, tt), dim3(256), 0, stream,
                                        out + static_cast<long long>(t0) * H, c3, ids, E, top_k, H), "w4 sum launch"))
       return st;

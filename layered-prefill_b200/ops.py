@@ -201,8 +201,11 @@ def w4_linear(out: torch.Tensor, input: torch.Tensor, qweight: torch.Tensor, sca
     checked = (input, bf16, shape) if ld == K else (input[:1], bf16, (min(M, 1), K))
     _check("w4_linear", device, "input out qweight scales zeros bias", checked, (out, bf16, (*shape[:-1], N)),
            (qweight, u8, (N, K // 2)), (scales, bf16, (N, groups)), (zeros, u8, (N, groups)), (bias, bf16, (N,)))
+    group = K // groups if K % groups == 0 else -1
+    nbytes = lib.moe_b200_w4_linear_workspace_bytes(M, K, group)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _launch(lib.moe_b200_w4_linear, device, out.data_ptr(), input.data_ptr(), ld, qweight.data_ptr(), scales.data_ptr(),
-            _ptr(zeros), _ptr(bias), M, N, K, K // groups if K % groups == 0 else -1)
+            _ptr(zeros), _ptr(bias), M, N, K, group, _ptr(ws), nbytes)
 
 
 def _router_args(op, gating_output, topk_ids, token_mask):

@@ -30,7 +30,11 @@ def test_norm_quant_refusals():
 
 def test_w4_linear_refusals():
     lib, err = _lib()
-    f = lib.moe_b200_w4_linear
+    room = lib.moe_b200_w4_linear_workspace_bytes
+
+    def f(out, x, ld, q, s, z, b, M, N, K, g, stream, ws=P, ws_bytes=1 << 30):
+        return lib.moe_b200_w4_linear(out, x, ld, q, s, z, b, M, N, K, g, ws, ws_bytes, stream)
+
     assert f(P, P, 256, P, P, None, None, 0, 8, 256, 64, None) == 0
     for ld, (M, N, K, g) in ((256, (1, 8, 256, 48)), (256, (1, 8, 224, 64)), (256, (-1, 8, 256, 64)), (256, (1, 0, 256, 64)),
                              (260, (2, 8, 256, 64)), (0, (2, 8, 256, 64)), (128, (2, 8, 256, 64)), (256, (1, 8, 0, 64))):
@@ -38,6 +42,10 @@ def test_w4_linear_refusals():
     assert f(P, P + 2, 256, P, P, None, None, 1, 8, 256, 64, None) == 1 and "16 bytes" in err()
     assert f(P, P, 256, P + 8, P, None, None, 1, 8, 256, 64, None) == 1
     assert f(P, P, 256, P, None, None, None, 1, 8, 256, 64, None) == 1 and "null" in err()
+    need = room(16, 8192, 64)
+    assert need > 16 * 8192 * 2 and room(1, 2048, 128) == 0 and room(0, 2048, 128) == 0 and room(64, 8192, 48) == 0
+    assert f(P, P, 8192, P, P, None, None, 16, 8, 8192, 64, None, P, need - 1) == 3 and "workspace" in err()
+    assert f(P, P, 8192, P, P, None, None, 16, 8, 8192, 64, None, None, need) == 3
 
 
 def test_w4_experts_refusals():
