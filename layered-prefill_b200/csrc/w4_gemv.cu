@@ -357,8 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
     q_off[i] = static_cast<uint32_t>(row) * row_bytes;
     s_off[i] = static_cast<uint32_t>(row) * groups;
   }
-  auto first_row = [&](int tile) -> int {
-    const int r = tile % p.row_tiles;
+  auto first_row = [&](int r) -> int {  // of row tile r
     // the last tile takes rows of the one before again rather than rows past the end
     return kMode == kGateUp ? r * (S::kRows / 2) : max(0, min(r * S::kRows, p.rows - S::kRows));
   };
@@ -369,7 +368,19 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
     base = kMode == kDense ? block * S::kTokens : lists.start[block];
     n = kMode == kDense ? min(S::kTokens, p.m - base) : lists.count[block];
   };
-  const int last_block = (last - 1) / p.row_tiles;
+  // A place in this CTA's work: tile number, its token block and its row tile. Going on from one to the next takes no division.
+  struct Place {
+    int tile, block, r;
+  };
+  auto advance = [&](Place& at, int by) {
+    at.tile += by;
+    at.r += by;
+    while (at.r >= p.row_tiles) {
+      at.r -= p.row_tiles;
+      ++at.block;
+    }
+  };
+  const int first_block = first / p.row_tiles, last_block = (last - 1) / p.row_tiles;
   auto window_end = [&](int block) {  // the blocks from `block` on whose activations fit together, those of this CTA
     if (spans > 1) return block + 1;
     int base, at, n;
@@ -388,23 +399,26 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   };
 
   // ------------------------------------------------------------------ codes: one step of this warp into its FIFO
-  int l_end_block = window_end(first / p.row_tiles), l_end = min(last, l_end_block * p.row_tiles);  // of the window
-  int l_tile = first + worker, l_span = 0, l_left = 0, l_col = 0;
+  int l_end_block = window_end(first_block), l_end = min(last, l_end_block * p.row_tiles);  // of the window
+  Place l_at{first, first_block, first - first_block * p.row_tiles};
+  advance(l_at, worker);
+  int l_span = 0, l_left = 0, l_col = 0;
   const uint8_t* l_src[2 * kRB];
-  auto open = [&]() {  // (l_tile, l_span); a worker's tiles are `workers` apart inside a window
-    while (l_tile >= l_end) {
+  auto open = [&]() {  // (l_at, l_span); a worker's tiles are `workers` apart inside a window
+    while (l_at.tile >= l_end) {
       if (l_end == last) {
-        l_tile = last;
+        l_at.tile = last;
         return;
       }
-      l_tile = l_end + worker;
+      l_at = Place{l_end, l_end_block, 0};
+      advance(l_at, worker);
       l_end_block = window_end(l_end_block);
       l_end = min(last, l_end_block * p.row_tiles);
     }
     int begin;
     chunks_of(l_span, begin, l_left);
     l_col = l_span * p.span + begin * kChunk + t * 32;
-    const uint8_t* src = p.w.q + (first_row_of_matrix(l_tile / p.row_tiles) + first_row(l_tile) * step_row + row_lo) * row_bytes + (l_col >> 1);
+    const uint8_t* src = p.w.q + (first_row_of_matrix(l_at.block) + first_row(l_at.r) * step_row + row_lo) * row_bytes + (l_col >> 1);
 #pragma unroll
     for (int i = 0; i < 2 * kRB; ++i) l_src[i] = src + q_off[i];
   };
@@ -429,10 +443,10 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
       l_col += kStages * kChunk;
 #pragma unroll
       for (int i = 0; i < 2 * kRB; ++i) l_src[i] += kStages * kChunk / 2;
-      if (l_left <= 0 && l_tile < last) {
+      if (l_left <= 0 && l_at.tile < last) {
         if (++l_span == spans) {
           l_span = 0;
-          l_tile += workers;
+          advance(l_at, workers);
         }
         l_left = 0;
         open();
@@ -491,11 +505,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   int gi = 0;
   uint32_t s_next[2 * kRB][kSWords], z_next[2 * kRB];
   bool fetched = false;
-  auto open_scales = [&](int tile, int block, int span_i) {
+  auto open_scales = [&](const Place& at, int span_i) {
     int begin, n;
     chunks_of(span_i, begin, n);
     gi = (span_i * p.span / kChunk + begin) * kGpc;
-    const long long s_at = (first_row_of_matrix(block) + first_row(tile) * step_row + row_lo) * groups + gi;
+    const long long s_at = (first_row_of_matrix(at.block) + first_row(at.r) * step_row + row_lo) * groups + gi;
 #pragma unroll
     for (int i = 0; i < 2 * kRB; ++i) s_src[i] = p.w.scale + s_at + s_off[i];
     z_src = p.w.zero + s_at;
@@ -546,21 +560,25 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   // ------------------------------------------------------------------ products
   const int start[4] = {kFloatBits, kFloatBits, kFloatBits, kFloatBits};
   const uint32_t fifo_lane = smem_u32(fifo) + g * 64;
-  for (int block0 = first / p.row_tiles; block0 <= last_block;) {
+  for (int block0 = first_block; block0 <= last_block;) {
     const int block1 = window_end(block0);
-    const int win_first = max(first, block0 * p.row_tiles), win_last = min(last, block1 * p.row_tiles);
-    const int rounds = (win_last - win_first + workers - 1) >> (4 - p.wk_log2);
+    Place at{first, first_block, first - first_block * p.row_tiles};
+    if (block0 > first_block) at = Place{block0 * p.row_tiles, block0, 0};
+    const int win_last = min(last, block1 * p.row_tiles);
+    const int rounds = (win_last - at.tile + workers - 1) >> (4 - p.wk_log2);
+    advance(at, worker);
     int win_base, win_n, base, n_tokens;
     entries_of(block0, win_base, win_n);
     entries_of(block1 - 1, base, n_tokens);
     win_n = base + n_tokens - win_base;
     for (int round = 0; round < rounds; ++round) {
-      const int tile = win_first + worker + round * workers;
-      const bool active = tile < win_last;
-      const int block = min(tile / p.row_tiles, block1 - 1);
+      const bool active = at.tile < win_last;
+      const int block = active ? at.block : block0;
       entries_of(block, base, n_tokens);
-      const int row0 = first_row(tile);
+      const int row0 = first_row(at.r);
       const long long mat = first_row_of_matrix(block);
+      const Place here = at;
+      advance(at, workers);
       // columns past the block's tokens are not written: they take the last one's activations
       const uint8_t* x_lane[kTB];
       const float* xs_lane[kTB][2];
@@ -589,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
         int begin, left;
         chunks_of(span_i, begin, left);
         if (!fetched) {
-          open_scales(tile, block, span_i);
+          open_scales(here, span_i);
           fetch_scales(std::integral_constant<int, 0>{});
         }
         fetched = false;
@@ -724,8 +742,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
         }
       }
 
-      if (active && tile + workers < win_last) {
-        open_scales(tile + workers, (tile + workers) / p.row_tiles, 0);
+      if (active && at.tile < win_last) {
+        open_scales(at, 0);
         fetch_scales(std::integral_constant<int, 0>{});
         fetched = true;
       }
@@ -821,8 +839,9 @@ int expected_blocks(int slots, int E) {
 }
 
 // How a launch is split, and a guess of its time in cycles; the shape with the least is taken. What it weighs: a chunk of a
-// warp takes about 1100 cycles for 16 rows with all warps at work (2200 for 32), a tile's end 3000, a window ends with half a
-// round of idle workers, and activations come at 64 bytes a cycle behind a latency of 1500.
+// warp takes about 850 cycles for 16 rows with all warps at work (1450 for 32), more with small groups and two token blocks, a
+// tile's end 2200, a window is a whole number of rounds and, where others follow, waits for its slowest worker, and activations
+// come at 64 bytes a cycle behind a latency of 1500.
 struct W4Split {
   int span, cap, wk_log2, ctas;
   double cost;
@@ -847,15 +866,15 @@ W4Split split_of(const W4Params& p, long long blocks) {
   r.ctas = static_cast<int>(tiles < sms ? tiles : sms);
   const double per_cta = static_cast<double>(tiles) / r.ctas;
   const double tokens = std::max(1.0, std::min<double>(S::kTokens, static_cast<double>(entries) / blocks));  // of a block
-  const double windows = 1 + (spans > 1 ? per_cta / row_tiles : std::min<double>(entries, (per_cta / row_tiles + 1) * tokens) / r.cap);
+  const double windows = spans > 1 ? 1 + per_cta / row_tiles : std::ceil(std::min<double>(entries, (per_cta / row_tiles + 1) * tokens) / r.cap);
   const double rows_a_window = std::min<double>(r.cap, std::max<double>(entries < S::kTokens ? entries : S::kTokens, static_cast<double>(entries) / r.ctas));
   const int last_chunks = chunks - (chunks - 1) / span_chunks * span_chunks;  // every warp has a step in every span
   r.cost = -1;
   for (int lg = 0; lg <= 4 && (1 << lg) <= std::min(last_chunks, span_chunks); ++lg) {
-    const double rounds = std::max(std::ceil(per_cta / (kWarps >> lg)), per_cta / (kWarps >> lg) + 0.5 * windows);
+    const double rounds = windows * (std::ceil(per_cta / windows / (kWarps >> lg)) + 1.5 * std::min(1.0, windows - 1));
     const double steps = (spans - 1.0) * ((span_chunks + (1 << lg) - 1) >> lg) + ((last_chunks + (1 << lg) - 1) >> lg);
     const double x_loads = spans > 1 ? rounds * spans : windows;
-    const double cost = rounds * (steps * 1100 * kRB * (1 + 0.4 * (kTB - 1)) + 3000) +
+    const double cost = rounds * (steps * (250 + 600 * kRB) * (1 + 0.2 * (kGpc - 1)) * (1 + 0.5 * (kTB - 1)) + 2200) +
                         x_loads * (1500 + rows_a_window * (kMode == kDown ? 4 : 2) * r.span / 64.0);
     if (r.cost < 0 || cost < r.cost) {
       r.cost = cost;
