@@ -56,7 +56,7 @@ struct W4Params {
   int span;               // columns whose activations are in shared memory at a time, a multiple of kChunk
   int cap;                // token rows whose activations fit
   int whole;              // K is a multiple of kChunk
-  int packed;             // the scales and zero points of a chunk can be read at once
+  int scale_words;        // scales of a row can be read four (2), two (1) or one (0) at a time
   int wk_log2;            // log2 of the warps of a worker
   int row_tiles;
   const void* x;          // dense / gate_up: bf16 [tokens, K]; down: fp32 [slots, K]
@@ -498,55 +498,61 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   };
 
   // ------------------------------------------------------------------ scales and zero points of this lane's rows
-  // Fetched one chunk ahead, and those of a tile's first chunk before the end of the tile in front of it.
-  constexpr int kSWords = kGpc == 4 ? 2 : 1;
+  // Four scales of a row (kUnit chunks) are fetched at a time, where they start on their size with one load: an SM has more rows
+  // under way than its first-level cache has lines, so that every further load of a row would go to the second level again. The
+  // fetch is one unit ahead, that of a tile's first unit in front of the end of the tile before.
+  constexpr int kUnit = 4 / kGpc;
   const __nv_bfloat16* s_src[2 * kRB];
   const uint8_t* z_src = nullptr;
-  int gi = 0;
-  uint32_t s_next[2 * kRB][kSWords], z_next[2 * kRB];
+  int gi = 0, words = 0;
+  uint32_t s_next[2 * kRB][2], z_next[2 * kRB];
   bool fetched = false;
   auto open_scales = [&](const Place& at, int span_i) {
     int begin, n;
     chunks_of(span_i, begin, n);
     gi = (span_i * p.span / kChunk + begin) * kGpc;
+    words = gi % 4 == 0 ? p.scale_words : (gi % 2 == 0 ? min(p.scale_words, 1) : 0);
     const long long s_at = (first_row_of_matrix(at.block) + first_row(at.r) * step_row + row_lo) * groups + gi;
 #pragma unroll
     for (int i = 0; i < 2 * kRB; ++i) s_src[i] = p.w.scale + s_at + s_off[i];
     z_src = p.w.zero + s_at;
   };
-          auto fetch_scales = [&](auto ahead_c) {  // of the chunk so many chunks behind s_src
-            constexpr int kAhead = decltype(ahead_c)::value * kGpc;
-  #pragma unroll
-            for (int i = 0; i < 2 * kRB; ++i) {
-              const __nv_bfloat16* sp = s_src[i] + kAhead;
-              const uint8_t* zp = z_src + s_off[i] + kAhead;
-              if (kGpc == 1) {
-                s_next[i][0] = *reinterpret_cast<const uint16_t*>(sp);
-                if (kZero) z_next[i] = *zp;
-              } else if (p.packed) {
-                if (kGpc == 2) {
-                  s_next[i][0] = *reinterpret_cast<const uint32_t*>(sp);
-                  if (kZero) z_next[i] = *reinterpret_cast<const uint16_t*>(zp);
-                } else {
-                  const uint2 v = *reinterpret_cast<const uint2*>(sp);
-                  s_next[i][0] = v.x;
-                  s_next[i][kSWords - 1] = v.y;
-                  if (kZero) z_next[i] = *reinterpret_cast<const uint32_t*>(zp);
-                }
-              } else {
-                if (kZero) z_next[i] = 0;
-  #pragma unroll
-                for (int q = 0; q < kSWords; ++q) s_next[i][q] = 0;
-  #pragma unroll
-                for (int q = 0; q < kGpc; ++q) {
-                  if (gi + kAhead + q < groups) {
-                    s_next[i][q / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(sp + q)) << (16 * (q & 1));
-                    if (kZero) z_next[i] |= static_cast<uint32_t>(zp[q]) << (8 * q);
-                  }
-                }
-              }
-            }
-          };
+  auto fetch_scales = [&](auto ahead_c) {  // of the unit so many chunks behind s_src
+    constexpr int kAhead = decltype(ahead_c)::value * kGpc;
+    if (words == 2) {
+#pragma unroll
+      for (int i = 0; i < 2 * kRB; ++i) {
+        const uint2 v = *reinterpret_cast<const uint2*>(s_src[i] + kAhead);
+        s_next[i][0] = v.x;
+        s_next[i][1] = v.y;
+        if (kZero) z_next[i] = *reinterpret_cast<const uint32_t*>(z_src + s_off[i] + kAhead);
+      }
+    } else if (words == 1) {
+#pragma unroll
+      for (int i = 0; i < 2 * kRB; ++i) {
+        const bool more = gi + kAhead + 2 < groups;
+        s_next[i][0] = *reinterpret_cast<const uint32_t*>(s_src[i] + kAhead);
+        s_next[i][1] = more ? *reinterpret_cast<const uint32_t*>(s_src[i] + kAhead + 2) : 0;
+        if (kZero) {
+          z_next[i] = *reinterpret_cast<const uint16_t*>(z_src + s_off[i] + kAhead);
+          if (more) z_next[i] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(z_src + s_off[i] + kAhead + 2)) << 16;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2 * kRB; ++i) {
+        s_next[i][0] = s_next[i][1] = 0;
+        if (kZero) z_next[i] = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (gi + kAhead + q < groups) {
+            s_next[i][q / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(s_src[i] + kAhead + q)) << (16 * (q & 1));
+            if (kZero) z_next[i] |= static_cast<uint32_t>(z_src[s_off[i] + kAhead + q]) << (8 * q);
+          }
+        }
+      }
+    }
+  };
 
   open();
   load_chunk(std::integral_constant<int, 0>{});
@@ -619,6 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
           xs_at[tb][0] = xs_lane[tb][0] + begin * (kGpc + 1);
           xs_at[tb][1] = xs_lane[tb][1] + begin * (kGpc + 1);
         }
+        uint32_t s_cur[2 * kRB][2], z_cur[2 * kRB];
         auto chunk = [&](auto slot_c) {  // the products of chunk kSlot of four
           constexpr int kSlot = decltype(slot_c)::value;
           cp_async_wait<kStages - 2>();
@@ -651,14 +658,15 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
             read_row(std::integral_constant<int, 3 % (2 * kRB)>{});
           }
           load_chunk(std::integral_constant<int, (kSlot + 3) % kStages>{});  // into the slot that the previous chunk has left
-          uint32_t s_cur[2 * kRB][kSWords], z_cur[2 * kRB];
+          if (kSlot % kUnit == 0) {
 #pragma unroll
-          for (int i = 0; i < 2 * kRB; ++i) {
-            if (kZero) z_cur[i] = z_next[i];
-#pragma unroll
-            for (int q = 0; q < kSWords; ++q) s_cur[i][q] = s_next[i][q];
+            for (int i = 0; i < 2 * kRB; ++i) {
+              if (kZero) z_cur[i] = z_next[i];
+              s_cur[i][0] = s_next[i][0];
+              s_cur[i][1] = s_next[i][1];
+            }
+            if (left > kSlot + kUnit) fetch_scales(std::integral_constant<int, kSlot + kUnit>{});
           }
-          if (kSlot + 1 < left) fetch_scales(std::integral_constant<int, kSlot + 1>{});
           int high[kRB][kTB][4], low[kRB][kTB][4];
           float part[kRB][kTB][4];  // of the chunk, in units of f
 #pragma unroll
@@ -688,10 +696,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
               float s[2 * kRB], z[2 * kRB];
 #pragma unroll
               for (int i = 0; i < 2 * kRB; ++i) {
-                const uint32_t v = s_cur[i][q / 2];
-                s[i] = __uint_as_float(q & 1 ? v & 0xffff0000u : v << 16);
+                const int at = kSlot % kUnit * kGpc + q;
+                const uint32_t v = s_cur[i][at / 2];
+                s[i] = __uint_as_float(at & 1 ? v & 0xffff0000u : v << 16);
                 // -zero: 0xcb000000 are the bits of -8388608, one less for every unit
-                if (kZero) z[i] = __uint_as_float(((z_cur[i] >> (8 * q)) & 15u) | 0xcb000000u) + 8388608.f;
+                if (kZero) z[i] = __uint_as_float(((z_cur[i] >> (8 * at)) & 15u) | 0xcb000000u) + 8388608.f;
               }
 #pragma unroll
               for (int tb = 0; tb < kTB; ++tb)
@@ -902,7 +911,9 @@ cudaError_t launch_split(W4Params p, const W4Split& s, cudaStream_t stream) {
   p.cap = s.cap;
   p.wk_log2 = s.wk_log2;
   p.whole = p.K % kChunk == 0;
-  p.packed = p.whole && reinterpret_cast<uintptr_t>(p.w.scale) % (2 * kGpc) == 0 && reinterpret_cast<uintptr_t>(p.w.zero) % kGpc == 0;
+  const uintptr_t s_at = reinterpret_cast<uintptr_t>(p.w.scale), z_at = reinterpret_cast<uintptr_t>(p.w.zero);
+  const int groups = p.K / p.w.group;
+  p.scale_words = groups % 4 == 0 && s_at % 8 == 0 && z_at % 4 == 0 ? 2 : (groups % 2 == 0 && s_at % 4 == 0 && z_at % 2 == 0 ? 1 : 0);
   return launch_pdl(kernel, dim3(s.ctas), dim3(kThreads), S::kFixed + s.cap * S::x_row_bytes(s.span, kGpc), stream, p);
 }
 
