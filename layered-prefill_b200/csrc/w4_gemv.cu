@@ -158,10 +158,15 @@ __device__ void build_lists(SlotLists& l, int* first_of, uint16_t* table, const 
     const int e = e0 + t;
     int c = 0;
     if (e < E) {
-      for (int r = 0; r < rows; ++r) {
-        const int n = table[r * E + e];
-        table[r * E + e] = static_cast<uint16_t>(c);
-        c += n;
+      for (int r0 = 0; r0 < rows; r0 += 16) {
+        int n[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) n[r] = r0 + r < rows ? table[(r0 + r) * E + e] : 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (r0 + r < rows) table[(r0 + r) * E + e] = static_cast<uint16_t>(c);
+          c += n[r];
+        }
       }
     }
     const int v = c | (((c + width - 1) / width) << 16);
@@ -465,18 +470,43 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
     // half a warp takes a chunk of a token
     int row = 0, c = warp * 2 + (lane >> 4);
     const int u = lane & 15;
+    if (kMode != kDown && p.xq != nullptr) {
+      // not by cp.async: its wait would be for the codes under way too
+      const int all = (p.K + kChunk - 1) / kChunk;
+      constexpr int kAhead = 4;
+      for (int at = warp * 2; at < n * chunks; at += kAhead * 2 * kWarps) {
+        uint4 v[kAhead];
+        float s[kAhead];
+        int to[kAhead], to_s[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          while (c >= chunks) {
+            c -= chunks;
+            ++row;
+          }
+          const int r = min(row, n - 1);  // behind the last chunk: one of the last token again
+          const long long src = source_row(r) * all + c0 / kChunk + c;
+          v[i] = *reinterpret_cast<const uint4*>(p.xq + src * 256 + u * 16);
+          s[i] = u <= kGpc ? p.xm[src * (kGpc + 1) + u] : 0.f;
+          to[i] = r * x_ld + c * 256 + u * 16;
+          to_s[i] = r * xs_ld + c * (kGpc + 1) + u;
+          c += 2 * kWarps;
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          *reinterpret_cast<uint4*>(x_mem + to[i]) = v[i];
+          if (u <= kGpc) x_sum[to_s[i]] = s[i];
+        }
+      }
+      return;
+    }
     for (int at = warp * 2; at < n * chunks; at += 2 * kWarps) {
       while (c >= chunks) {
         c -= chunks;
         ++row;
       }
-      const int r = min(row, n - 1);  // behind the last chunk: one of the last token again
-      if (kMode != kDown && p.xq != nullptr) {
-        const int all = (p.K + kChunk - 1) / kChunk;
-        const long long src = source_row(r) * all + c0 / kChunk + c;
-        cp_async_16(smem_u32(x_mem + r * x_ld + c * 256 + u * 16), p.xq + src * 256 + u * 16, 16);
-        if (u <= kGpc) x_sum[r * xs_ld + c * (kGpc + 1) + u] = p.xm[src * (kGpc + 1) + u];
-      } else {
+      const int r = min(row, n - 1);
+      {
         const int col = c0 + c * kChunk + col_of<kGpc>(u >> 2, u & 3);
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         using X = std::conditional_t<kMode == kDown, float, __nv_bfloat16>;
@@ -490,10 +520,6 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
         if (u == 0) x_sum[r * xs_ld + c * (kGpc + 1) + kGpc] = f;
       }
       c += 2 * kWarps;
-    }
-    if (kMode != kDown && p.xq != nullptr) {
-      cp_async_commit();
-      cp_async_wait_all();
     }
   };
 
@@ -918,7 +944,18 @@ cudaError_t launch_split(W4Params p, const W4Split& s, cudaStream_t stream) {
 }
 
 template <int kMode, int kTB, int kGpc>
+double least_cost(const W4Params& p, long long blocks) {
+  return std::min(split_of<kMode, 1, kTB, kGpc>(p, blocks).cost, split_of<kMode, 2, kTB, kGpc>(p, blocks).cost);
+}
+
+template <int kMode, int kTB, int kGpc>
 cudaError_t launch_groups(W4Params p, long long blocks, int x_rows, void* xq, cudaStream_t stream) {
+  // More than eight tokens: blocks of sixteen, unless a long K leaves no room for so many activations and the weights
+  // are better read once more (M = 16, N = 4096, K = 8192: 26 us in one block of two halves of K, 24 us in two blocks).
+  if constexpr (kTB == 2) {
+    const long long more = (p.m + 7) / 8;
+    if (least_cost<kMode, 1, kGpc>(p, more) < least_cost<kMode, 2, kGpc>(p, blocks)) return launch_groups<kMode, 1, kGpc>(p, more, x_rows, xq, stream);
+  }
   if (xq != nullptr) {
     const long long chunks = static_cast<long long>(x_rows) * ((p.K + kChunk - 1) / kChunk);
     p.xq = static_cast<uint8_t*>(xq);
