@@ -556,8 +556,8 @@ int moe_b200_fused_experts_w4(const void* x, const void* w13_q, const void* w13_
     return set_error(kStatusInvalidArgument, "fused_experts_w4: null pointer");
   if ((w13_zero == nullptr) != (w2_zero == nullptr))
     return set_error(kStatusInvalidArgument, "fused_experts_w4: zero points for both weights or for none");
-  if (!aligned(x, 16) || !aligned(w13_q, 16) || !aligned(w2_q, 16))
-    return set_error(kStatusInvalidArgument, "fused_experts_w4: x and the codes must start on 16 bytes");
+  if (!aligned(x, 16) || !aligned(w13_q, 16) || !aligned(w2_q, 16) || !aligned(out, 8))
+    return set_error(kStatusInvalidArgument, "fused_experts_w4: x and the codes must start on 16 bytes, out on 8");
   const size_t need = moe_b200_fused_experts_w4_workspace_bytes(T, E, top_k, H, I);
   if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16))
     return set_error(kStatusWorkspaceTooSmall, "fused_experts_w4: workspace of %zu bytes on 16 needed, %zu given", need, workspace_bytes);

@@ -486,7 +486,7 @@ cudaError_t allow_smem(K kernel, size_t bytes) {
 int check_router(const char* what, int T, int E, int k) {
   if (T < 0 || E <= 0 || k <= 0 || k > E) return set_error(kStatusInvalidArgument, "%s: need T >= 0 and 0 < k <= E (T=%d E=%d k=%d)", what, T, E, k);
   if (E > kMaxExperts) return set_error(kStatusInvalidArgument, "%s: more than %d experts", what, kMaxExperts);
-  if (static_cast<long long>(T) * k > 0x7fffffffll) return set_error(kStatusInvalidArgument, "%s: T * k does not fit the int32 counts", what);
+  if (T > 1 << 30 || static_cast<long long>(T) * k > 0x7fffffffll) return set_error(kStatusInvalidArgument, "%s: T * k is too large for the int32 counts", what);
   return kStatusOk;
 }
 

@@ -12,8 +12,8 @@
 // 32 columns instead of 16 at the same rate. Unpacking is what bounds the loop next to the loads.
 //   The activations become 16-bit integers with a power of two f for every token and 128 columns:
 //   x = f * (256 hi + lo), hi signed and lo unsigned bytes, two products a word; f puts the largest |x| of them between 2^14 and 2^15.
-//   A bf16 value has 8 significant bits, so that all within 2^7 of the largest are exact and smaller ones are off by at most
-//   2^-16 of the largest; the intermediate h of the experts (fp32) is off by that everywhere. Integer sums are exact; then
+//   A bf16 value has 8 significant bits, so that all down to 2^-7 of the largest are exact and smaller ones are off by at most
+//   2^-15 of the largest; the intermediate h of the experts (fp32) is off by that everywhere. Integer sums are exact; then
 //   sum (code - zero) x = f * (256 sum code hi + sum code lo - zero * sum x) in fp32, times the group's scale, summed in fp32.
 //   Where a value is not finite f is NaN, so that its token's results are NaN.
 //   A CTA makes these integers itself where they are few; where many CTAs would make many of them (a batch, a long K) a kernel in
@@ -980,8 +980,8 @@ cudaError_t launch_mode(const W4Params& p, long long blocks, int x_rows, void* x
   return launch_groups<kMode, kTB, 4>(p, blocks, x_rows, xq, stream);
 }
 
-// Room for the integers of `rows` activations of K columns, 0 where the CTAs make them themselves: with up to 16 chunks of
-// 128 columns (one turn of half the warps of a CTA) the kernel in front takes longer than it saves.
+// Room for the integers of `rows` activations of K columns, 0 where the CTAs make them themselves: up to kPreparedChunks chunks
+// of 128 columns, two turns of a CTA's warps, for which a launch in front takes longer than it saves.
 size_t prepared_bytes(int rows, int K, int group) {
   const size_t chunks = static_cast<size_t>(rows) * ((K + kChunk - 1) / kChunk);
   return chunks <= kPreparedChunks ? 0 : chunks * (256 + 4 * (kChunk / group + 1));
@@ -998,7 +998,7 @@ int launch_w4_linear(__nv_bfloat16* out, const __nv_bfloat16* x, long long x_ld,
   p.w = w; p.rows = N; p.K = K; p.x = x; p.x_ld = x_ld; p.m = M; p.out = out;
   const int tb = M <= 8 ? 1 : 2;
   const long long blocks = (M + 8 * tb - 1) / (8 * tb);
-  if (blocks * ((N + 15) / 16) > 0x3fffffffll) return set_error(kStatusInvalidArgument, "w4_linear: M x N too large");
+  if (blocks * ((N + 15) / 16) > 0x3fffffffll || K > 1 << 24) return set_error(kStatusInvalidArgument, "w4_linear: M x N or K too large");
   void* xq = prepared_bytes(M, K, w.group) > 0 ? workspace : nullptr;
   const cudaError_t e = tb == 1 ? launch_mode<kDense, 1>(p, blocks, M, xq, stream) : launch_mode<kDense, 2>(p, blocks, M, xq, stream);
   if (int st = check_cuda(e, "w4_linear launch")) return st;

@@ -188,7 +188,8 @@ def w4_linear(out: torch.Tensor, input: torch.Tensor, qweight: torch.Tensor, sca
     """out[.., N] = input[.., K] @ W^T + bias for 4-bit weights W[n, k] = (code - zero) * scale, built for few tokens (any number
     works). qweight uint8 [N, K / 2], two codes a byte, the low nibble is the even k; scales bf16 [N, K / group], groups of 32, 64 or
     128; zeros uint8 0..15 like scales (8 without it); bias bf16 [N]. A two-dimensional input may have rows further than K apart
-    (a multiple of 8 elements). `fused_moe.quant_w4` makes such weights."""
+    (a multiple of 8 elements). The activations enter the products as 16-bit integers times a power of two for every 128 columns (exact
+    down to 2^-7 of their largest, off by at most 2^-15 of it below); sums are fp32. `fused_moe.quant_w4` makes such weights."""
     K = input.size(-1) if input.dim() else 0
     N, groups = (qweight.size(0), scales.size(-1)) if qweight.dim() == 2 and scales.dim() == 2 else (0, 0)
     if N == 0 or groups == 0 or K == 0:

@@ -2,7 +2,11 @@
 
 Tolerances. A sum of K products in fp32, in any order and with a truncating adder, is off by at most (K / 16 + 64) * 2^-23 of
 sum |w x|: products of a tensor instruction are exact and added 16 at a time, and at most 64 further additions (groups, warps) follow.
-The output's rounding adds 2^-8 of the value. The experts' intermediate carries at least 16 significant bits (2^-16)."""
+The output's rounding adds 2^-8 of the value.
+Activations become 16-bit integers times 2^(e - 14), 2^e being the power of two at or below the largest |x| of 128 columns: a step of
+at most 2^-14 of the largest, so half a step is at most 2^-15 of it, which adds 2^-15 * largest * sum |w|. A bf16 value of exponent at
+least e - 7 is a whole number of steps (its last bit is worth 2^(e - 7 - 7)) and adds nothing: only values below 2^-7 * 2^e, which are
+below 2^-7 of the largest, do. The experts' intermediate is fp32 and adds it everywhere."""
 import pytest
 import torch
 
@@ -28,6 +32,18 @@ def _dense64(packed, scale, zp, group):
     return (code - z) * scale.double().repeat_interleave(group, -1)
 
 
+def _step(x):
+    """2^-15 of the largest |x| of every 128 columns, [.., K]."""
+    pad = -x.size(-1) % 128
+    big = torch.nn.functional.pad(x.abs(), (0, pad)).unflatten(-1, (-1, 128)).amax(-1)
+    return 2.0 ** -15 * big.repeat_interleave(128, -1)[..., :x.size(-1)]
+
+
+def _bf16_off(x):
+    """What a bf16 x may be off by as an integer."""
+    return torch.where(x.abs() < 2.0 ** 8 * _step(x), _step(x), torch.zeros_like(x))
+
+
 def _linear(x, packed, scale, zp, bias=None):
     from layered_prefill_b200 import ops
     out = torch.full((*x.shape[:-1], packed.size(0)), float("nan"), dtype=torch.bfloat16, device="cuda")
@@ -39,7 +55,7 @@ def _check_linear(out, x, packed, scale, zp, bias=None):
     group = 2 * packed.size(-1) // scale.size(-1)
     w, x = _dense64(packed, scale, zp, group), x.double()
     y = x @ w.t() + (0 if bias is None else bias.double())
-    bound = BF16 * y.abs() * 1.01 + _gamma(x.size(-1)) * (x.abs() @ w.abs().t() + (0 if bias is None else bias.double().abs()))
+    bound = BF16 * y.abs() * 1.01 + _bf16_off(x) @ w.abs().t() + _gamma(x.size(-1)) * (x.abs() @ w.abs().t() + (0 if bias is None else bias.double().abs()))
     err = (out.double() - y).abs()
     assert (err <= bound).all(), (err / bound).max()
 
@@ -135,15 +151,15 @@ def _experts64(x, w13, w2, b13, b2, tw, ti, group, activation):
         b = _dense64(w2[0][e], w2[1][e], None if w2[2] is None else w2[2][e], group)
         xe = x[t].double()
         gu = xe @ a.t() + (0 if b13 is None else b13[e].double())
-        dgu = _gamma(H) * (xe.abs() @ a.abs().t() + (0 if b13 is None else b13[e].double().abs()))
+        dgu = _bf16_off(xe) @ a.abs().t() + _gamma(H) * (xe.abs() @ a.abs().t() + (0 if b13 is None else b13[e].double().abs()))
         I = gu.size(1) // 2
         cut = (lambda v: (v[:, :I], v[:, I:])) if activation == "silu" else (lambda v: (v[:, 0::2], v[:, 1::2]))
         (gate, up), (dg, du) = cut(gu), cut(dgu)
         h = _act64(gate, up, activation)
         # slopes: |d act/d gate| <= 1.2 |up + 1|, |d act/d up| <= |gate|
-        dh = 1.2 * (up.abs() + 1) * dg + gate.abs() * du + 2.0 ** -16 * h.abs() + 2.0 ** -20 * gate.abs() * (up.abs() + 1)
+        dh = 1.2 * (up.abs() + 1) * dg + gate.abs() * du + 2.0 ** -20 * gate.abs() * (up.abs() + 1)
         y = h @ b.t() + (0 if b2 is None else b2[e].double())
-        dy = dh @ b.abs().t() + _gamma(I) * (h.abs() @ b.abs().t() + (0 if b2 is None else b2[e].double().abs()))
+        dy = (dh + _step(h)) @ b.abs().t() + _gamma(I) * (h.abs() @ b.abs().t() + (0 if b2 is None else b2[e].double().abs()))
         w = tw[t, j].double()[:, None]
         out.index_add_(0, t, w * y)
         bound.index_add_(0, t, w.abs() * dy + 2.0 ** -22 * (w * y).abs())
@@ -280,6 +296,87 @@ def test_quantised_weights_come_near_the_bf16_block():
     ref = fused_moe.fused_experts(hidden, w13.to(torch.bfloat16), w2.to(torch.bfloat16), None, None, tw, ti)
     # each code is off by at most half a step of a range of 15 steps: with random errors 2 * sqrt(1/12) / (15 / 5.6) ~ 0.11 a matrix
     assert (got.float() - ref.float()).norm() / ref.float().norm() < 0.3
+
+
+@pytest.mark.parametrize("M,N,K,group", [(3, 40, 16384, 128), (16, 100, 16384, 64), (24, 70, 8192, 32), (40, 300, 4096, 128)])
+def test_dense_columns_that_do_not_fit_at_once(M, N, K, group):
+    g = torch.Generator().manual_seed(M + K)
+    w = _weights(N, K, group, True, g)
+    x = torch.randn(M, K, generator=g).to(torch.bfloat16).cuda()
+    _check_linear(_linear(x, *w), x, *w)
+
+
+@pytest.mark.parametrize("M", [2, 20])
+def test_outliers_next_to_small_values(M):
+    """A few columns thousands of times larger than the rest, rows of zeros, and the ends of the range of bf16."""
+    g = torch.Generator().manual_seed(12)
+    w = _weights(64, 2048, 64, True, g)
+    x = torch.randn(M, 2048, generator=g)
+    x[:, ::257] *= 3000
+    x[0, 128:256] = 0
+    x[1, 256:384] *= 2.0 ** -100
+    x[1, 384:512] *= 2.0 ** 60
+    x = x.to(torch.bfloat16).cuda()
+    _check_linear(_linear(x, *w), x, *w)
+    assert (_linear(torch.zeros_like(x), *w) == 0).all()
+    tiny = torch.full_like(x, 2.0 ** -130)
+    assert (_linear(tiny, *w).abs() <= 2.0 ** -100).all()
+    huge = torch.zeros_like(x)
+    huge[:, 5] = 2.0 ** 126
+    _check_linear(_linear(huge, *w), huge, *w)
+
+
+@pytest.mark.parametrize("T,H,E,k,I,group", [(300, 256, 16, 8, 64, 32), (1030, 128, 8, 1, 64, 64), (9, 8192, 4, 2, 128, 128),
+                                             (12, 128, 4, 2, 6400, 128), (5, 10240, 3, 2, 96, 32), (64, 256, 200, 6, 64, 32)])
+def test_experts_in_pieces_and_with_long_columns(T, H, E, k, I, group):
+    """More slots than are listed at once, activations that do not fit at once, more experts than slots of a token."""
+    x, w13, w2, tw, ti = _case(T, H, E, k, I, group, True, T + H)
+    _check_experts(_experts(x, w13, w2, tw, ti, group), x, w13, w2, None, None, tw, ti, group, "silu")
+    if T == 300:
+        want = _experts(x, w13, w2, tw, ti, group)
+        y = x.clone()
+        _experts(y, w13, w2, tw, ti, group, inplace=True)
+        assert torch.equal(y, want)
+
+
+def test_on_scales_and_codes_between_the_usual_boundaries():
+    """Scales and zero points two bytes and one byte off: read one at a time. Codes off sixteen bytes are refused."""
+    from layered_prefill_b200._lib import MoeB200Error
+    g = torch.Generator().manual_seed(6)
+    q, s, z = _weights(48, 1024, 32, True, g)
+    x = torch.randn(10, 1024, generator=g).to(torch.bfloat16).cuda()
+    want = _linear(x, q, s, z)
+    s2 = torch.empty(s.numel() + 1, dtype=s.dtype, device="cuda")[1:].view_as(s).copy_(s)
+    z2 = torch.empty(z.numel() + 1, dtype=z.dtype, device="cuda")[1:].view_as(z).copy_(z)
+    assert torch.equal(_linear(x, q, s2, z2), want)
+    q2 = torch.empty(q.numel() + 8, dtype=q.dtype, device="cuda")[8:].view_as(q).copy_(q)
+    with pytest.raises(MoeB200Error):
+        _linear(x, q2, s, z)
+
+
+def test_dense_on_two_streams_at_once_and_in_a_graph():
+    g = torch.Generator().manual_seed(14)
+    w = _weights(2048, 4096, 128, False, g)
+    xs = [torch.randn(m, 4096, generator=g).to(torch.bfloat16).cuda() for m in (1, 16)]
+    want = [_linear(x, *w) for x in xs]
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [None, None]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] = _linear(xs[i], *w)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _linear(xs[1], *w)
+    keep = xs[1].clone()
+    xs[1].zero_()
+    graph.replay()
+    assert (out == 0).all()
+    xs[1].copy_(keep)
+    graph.replay()
+    assert torch.equal(out, want[1])
 
 
 def test_refusals():
