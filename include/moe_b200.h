@@ -223,7 +223,7 @@ int moe_b200_rms_norm_quant_fp8(void* q, float* scales, void* normed_out, void* 
  *   num_tokens int32 [1] = n;  mean_probs fp32 [E] = P
  * Balanced routing gives a balance loss of k. Same bits on every run. E <= 1024.
  */
-size_t moe_b200_router_loss_workspace_bytes(int T, int E);
+size_t moe_b200_router_loss_workspace_bytes(int T, int E); /* 0 up to 128 tokens */
 int moe_b200_router_loss(float* losses, int32_t* counts, int32_t* num_tokens, float* mean_probs, const void* gating,
                          int gating_is_bf16, const int32_t* topk_ids, const uint8_t* token_mask, int T, int E, int k,
                          void* workspace, size_t workspace_bytes, void* stream);
@@ -250,7 +250,8 @@ int moe_b200_router_backward(void* grad_logits, const void* gating, int gating_i
  * group_size 32, 64 or 128 and K % group_size == 0, K <= 2^24; any N. qweight and x on 16 bytes.
  * x enters as 16-bit integers times a power of two for every token and 128 columns: exact down to 2^-7 of the largest of
  * them, off by at most 2^-15 of it below. Integer products, fp32 sums, one rounding of the output. A value that is not finite
- * makes its token's row NaN. workspace: room for those integers where a kernel of its own makes them.
+ * makes its token's row NaN. workspace: room for those integers where a kernel in front makes them once; without it
+ * (NULL) every CTA makes those that it needs, with the same bits.
  */
 size_t moe_b200_w4_linear_workspace_bytes(int M, int K, int group_size); /* 0: none needed */
 int moe_b200_w4_linear(void* out, const void* x, int64_t x_row_stride, const void* qweight, const void* scale,

@@ -529,7 +529,7 @@ int moe_b200_w4_linear(void* out, const void* x, int64_t x_row_stride, const voi
   if (!aligned(x, 16) || !aligned(qweight, 16) || (M > 1 && (x_row_stride % 8 != 0 || x_row_stride < K)))
     return set_error(kStatusInvalidArgument, "w4_linear: x and qweight must start on 16 bytes and the rows of x lie a multiple of 8 elements, at least K, apart");
   const size_t need = w4_linear_workspace_bytes(M, K, group_size);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
+  if (workspace != nullptr && (workspace_bytes < need || !aligned(workspace, 16)))
     return set_error(kStatusWorkspaceTooSmall, "w4_linear: workspace of %zu bytes on 16 needed, %zu given", need, workspace_bytes);
   return launch_w4_linear(static_cast<__nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(x), x_row_stride,
                           w4_matrix(qweight, scale, zero, bias, group_size), M, N, K, workspace, static_cast<cudaStream_t>(stream));

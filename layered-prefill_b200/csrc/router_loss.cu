@@ -250,6 +250,7 @@ router_loss_kernel(const void* __restrict__ logits, const int* __restrict__ ids,
     s_n[warp] = n;
   }
   __syncthreads();
+  if (gridDim.x == 1) w = LossParts{smem, s_counts, s_z, s_n};  // a CTA alone keeps its parts
   for (int e = t; e < E; e += blockDim.x) {
     float s = 0.f;
     for (int i = 0; i < warps; ++i) s += smem[static_cast<size_t>(i) * E + e];
@@ -266,8 +267,7 @@ router_loss_kernel(const void* __restrict__ logits, const int* __restrict__ ids,
     w.z[blockIdx.x] = zs;
     w.n[blockIdx.x] = ns;
   }
-  if (gridDim.x == 1) {  // its own parts, through memory
-    __threadfence_block();
+  if (gridDim.x == 1) {
     __syncthreads();
     finish_losses<1>(w, 1, E, out, 0);
   }
@@ -493,6 +493,7 @@ int check_router(const char* what, int T, int E, int k) {
 }  // namespace
 
 size_t router_loss_workspace_bytes(int T, int E) {
+  if (T <= kOneCta) return 0;
   const size_t b = loss_blocks(T, E);
   return b * E * 8 + b * 8;
 }
@@ -502,7 +503,7 @@ int launch_router_loss(float* losses, int* counts, int* num_tokens, float* mean_
                        size_t workspace_bytes, cudaStream_t stream) {
   if (int st = check_router("router_loss", T, E, k)) return st;
   const size_t need = router_loss_workspace_bytes(T, E);
-  if (workspace == nullptr || workspace_bytes < need)
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 4 != 0))
     return set_error(kStatusWorkspaceTooSmall, "router_loss: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
   const int blocks = loss_blocks(T, E), warps = loss_warps(T);
   LossParts w;

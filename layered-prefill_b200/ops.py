@@ -155,10 +155,10 @@ def _ptr(t) -> int:
 
 
 def _norm_quant(op, out, scales, residual, input, weight, epsilon, group_size, normed_out, residual_out):  # noqa: A002
-    H = input.size(-1) if input.dim() else 0
+    bf16, shape, device = torch.bfloat16, input.shape, input.device
+    H = shape[-1] if shape else 0
     T = input.numel() // H if H else 0
     groups = 1 if group_size == -1 or (group_size == H and H != 128) else H // 128
-    bf16, shape, device = torch.bfloat16, input.shape, input.device
     _check(op, device, "input out weight scales residual residual_out normed_out", (input, bf16, shape),
            (out, torch.float8_e4m3fn, shape), (weight, bf16, (H,)), (scales, torch.float32, (*shape[:-1], groups)),
            (residual, bf16, shape), (residual_out, bf16, shape), (normed_out, bf16, shape))
@@ -190,23 +190,24 @@ def w4_linear(out: torch.Tensor, input: torch.Tensor, qweight: torch.Tensor, sca
     128; zeros uint8 0..15 like scales (8 without it); bias bf16 [N]. A two-dimensional input may have rows further than K apart
     (a multiple of 8 elements). The activations enter the products as 16-bit integers times a power of two for every 128 columns (exact
     down to 2^-7 of their largest, off by at most 2^-15 of it below); sums are fp32. `fused_moe.quant_w4` makes such weights."""
-    K = input.size(-1) if input.dim() else 0
-    N, groups = (qweight.size(0), scales.size(-1)) if qweight.dim() == 2 and scales.dim() == 2 else (0, 0)
-    if N == 0 or groups == 0 or K == 0:
+    shape, q_shape, s_shape = input.shape, qweight.shape, scales.shape
+    if len(q_shape) != 2 or len(s_shape) != 2 or not shape or not shape[-1] or not q_shape[0] or not s_shape[1]:
         raise RuntimeError("w4_linear: qweight must be [N, K / 2], scales [N, K / group] and input [.., K]")
+    K, N, groups = shape[-1], q_shape[0], s_shape[1]
     M = input.numel() // K
-    ld = K
-    if input.dim() == 2 and input.stride(1) == 1 and not input.is_contiguous():
-        ld = input.stride(0)
-    bf16, u8, device, shape = torch.bfloat16, torch.uint8, qweight.device, input.shape
-    checked = (input, bf16, shape) if ld == K else (input[:1], bf16, (min(M, 1), K))
+    bf16, u8, device, ld, checked = torch.bfloat16, torch.uint8, qweight.device, K, (input, torch.bfloat16, shape)
+    if len(shape) == 2 and not input.is_contiguous() and input.stride(1) == 1:
+        ld, checked = input.stride(0), (input[:1], bf16, (min(M, 1), K))
     _check("w4_linear", device, "input out qweight scales zeros bias", checked, (out, bf16, (*shape[:-1], N)),
            (qweight, u8, (N, K // 2)), (scales, bf16, (N, groups)), (zeros, u8, (N, groups)), (bias, bf16, (N,)))
     group = K // groups if K % groups == 0 else -1
-    nbytes = lib.moe_b200_w4_linear_workspace_bytes(M, K, group)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    ws, nbytes = None, 0
+    if M * K > 8192:  # below, no room is ever asked for
+        nbytes = lib.moe_b200_w4_linear_workspace_bytes(M, K, group)
+        ws = torch.empty(nbytes, dtype=u8, device=device) if nbytes else None
     _launch(lib.moe_b200_w4_linear, device, out.data_ptr(), input.data_ptr(), ld, qweight.data_ptr(), scales.data_ptr(),
-            _ptr(zeros), _ptr(bias), M, N, K, group, _ptr(ws), nbytes)
+            zeros.data_ptr() if zeros is not None else 0, bias.data_ptr() if bias is not None else 0, M, N, K, group,
+            ws.data_ptr() if ws is not None else 0, nbytes)
 
 
 def _router_args(op, gating_output, topk_ids, token_mask):
@@ -232,11 +233,13 @@ def router_loss(losses: torch.Tensor, counts: torch.Tensor, num_tokens: torch.Te
     _check("router_loss", dev, "gating_output topk_ids token_mask losses counts num_tokens mean_probs", *specs,
            (losses, torch.float32, (2,)), (counts, torch.int32, (E,)), (num_tokens, torch.int32, (1,)),
            (mean_probs, torch.float32, (E,)))
-    nbytes = lib.moe_b200_router_loss_workspace_bytes(T, E)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws, nbytes = None, 0
+    if T > 128:  # one CTA takes no more, and needs no room
+        nbytes = lib.moe_b200_router_loss_workspace_bytes(T, E)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _launch(lib.moe_b200_router_loss, dev, losses.data_ptr(), counts.data_ptr(), num_tokens.data_ptr(), mean_probs.data_ptr(),
             gating_output.data_ptr(), gating_output.dtype == torch.bfloat16, topk_ids.data_ptr(), _ptr(token_mask), T, E, k,
-            ws.data_ptr(), nbytes)
+            _ptr(ws), nbytes)
 
 
 def router_backward(grad_logits: torch.Tensor, gating_output: torch.Tensor, topk_ids: torch.Tensor, counts: torch.Tensor,

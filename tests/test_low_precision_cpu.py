@@ -45,7 +45,7 @@ def test_w4_linear_refusals():
     need = room(16, 8192, 64)
     assert need > 16 * 8192 * 2 and room(1, 2048, 128) == 0 and room(0, 2048, 128) == 0 and room(64, 8192, 48) == 0
     assert f(P, P, 8192, P, P, None, None, 16, 8, 8192, 64, None, P, need - 1) == 3 and "workspace" in err()
-    assert f(P, P, 8192, P, P, None, None, 16, 8, 8192, 64, None, None, need) == 3
+    assert f(P, P, 8192, P, P, None, None, 16, 8, 8192, 64, None, P + 8, need) == 3
 
 
 def test_w4_experts_refusals():
@@ -67,11 +67,12 @@ def test_w4_experts_refusals():
 def test_router_refusals():
     lib, err = _lib()
     f, b = lib.moe_b200_router_loss, lib.moe_b200_router_backward
-    need = lib.moe_b200_router_loss_workspace_bytes(64, 16)
+    need = lib.moe_b200_router_loss_workspace_bytes(640, 16)
+    assert need > 0 and lib.moe_b200_router_loss_workspace_bytes(128, 16) == 0
     assert f(P, P, P, P, P, 0, P, None, 64, 16, 17, P, need, None) == 1
     assert f(P, P, P, P, P, 0, P, None, 64, 1025, 2, P, 1 << 30, None) == 1 and "experts" in err()
     assert f(P, P, P, P, None, 0, P, None, 64, 16, 2, P, need, None) == 1
-    assert f(P, P, P, P, P, 0, P, None, 64, 16, 2, P, need - 1, None) == 3
+    assert f(P, P, P, P, P, 0, P, None, 640, 16, 2, P, need - 1, None) == 3
     assert b(P, P, 0, P, P, P, P, P, None, 0, 16, 2, 1, None) == 0
     assert b(P, P, 0, P, None, P, P, P, None, 4, 16, 2, 1, None) == 1
     assert b(P, P, 0, None, P, P, P, P, None, 4, 16, 2, 1, None) == 1
