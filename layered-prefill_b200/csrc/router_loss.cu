@@ -92,6 +92,31 @@ __device__ __forceinline__ void exp_row(float (&x)[kN], float& row_max, float& s
   row_max = m;
 }
 
+// The lane's experts in a row of shared memory (on 16 bytes for vectors of four).
+template <int kL, int kW, int kN>
+__device__ __forceinline__ void put_row(float* row, int E, int l, const float (&x)[kN]) {
+#pragma unroll
+  for (int v = 0; v < kN / kW; ++v) {
+    const int e = (v * kL + l) * kW;
+    if (e >= E) continue;
+    if constexpr (kW == 4) *reinterpret_cast<float4*>(row + e) = make_float4(x[4 * v], x[4 * v + 1], x[4 * v + 2], x[4 * v + 3]);
+    else row[e] = x[v];
+  }
+}
+template <int kL, int kW, int kN>
+__device__ __forceinline__ void get_row(const float* row, int E, int l, float (&x)[kN]) {  // 0 past E
+#pragma unroll
+  for (int v = 0; v < kN / kW; ++v) {
+    const int e = (v * kL + l) * kW;
+    if constexpr (kW == 4) {
+      const float4 q = e < E ? *reinterpret_cast<const float4*>(row + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+      x[4 * v] = q.x; x[4 * v + 1] = q.y; x[4 * v + 2] = q.z; x[4 * v + 3] = q.w;
+    } else {
+      x[v] = e < E ? row[e] : 0.f;
+    }
+  }
+}
+
 struct LossOut {
   float* losses;
   int* counts;
@@ -288,27 +313,24 @@ router_backward_kernel(void* __restrict__ grad, const void* __restrict__ logits,
                        const int* __restrict__ counts, const int* __restrict__ num_tokens,
                        const float* __restrict__ grad_losses, const float* __restrict__ grad_w,
                        const uint8_t* __restrict__ mask, int T, int E, int k, int renormalize) {
-  extern __shared__ float smem[];
+  extern __shared__ __align__(16) float smem[];  // [E] g_b * E * c_e / n^2, then a row a token
   grid_dependency_wait();
   grid_dependency_launch();
   constexpr int kTokens = 32 / kL;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int l = lane % kL, group = lane / kL;
-  float* row = smem + static_cast<size_t>(warp * kTokens + group) * E;
-  float g_b = 0.f, g_z = 0.f;  // g_b * E / n^2 (times c_e), g_z * 2 / n (times lse)
-  float base[kN];
-#pragma unroll
-  for (int i = 0; i < kN; ++i) base[i] = 0.f;
+  const int E4 = (E + 3) & ~3;
+  const float* s_base = smem;
+  float* row = smem + E4 + static_cast<size_t>(warp * kTokens + group) * E4;
+  float g_z = 0.f;  // g_z * 2 / n (times lse)
+  float g_b = 0.f;
   if (grad_losses != nullptr) {
     const float n = static_cast<float>(max(*num_tokens, 1));
     g_b = grad_losses[0] * E / n / n;
     g_z = grad_losses[1] * 2.f / n;
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int e = expert_of<kL, kW>(i, l);
-      if (e < E) base[i] = g_b * static_cast<float>(counts[e]);
-    }
   }
+  for (int e = threadIdx.x; e < E; e += blockDim.x) smem[e] = grad_losses != nullptr ? g_b * static_cast<float>(counts[e]) : 0.f;
+  __syncthreads();
   const int stride = gridDim.x * (blockDim.x >> 5) * kTokens;
   float next[kN];
   bool next_live = false;
@@ -340,25 +362,23 @@ router_backward_kernel(void* __restrict__ grad, const void* __restrict__ logits,
     int id = next_id;
     float gw = next_gw;
     fetch(tok + stride);
-    float m, sum, dot = 0.f;
+    float m, sum, dot = 0.f, u[kN];
     exp_row<kL>(x, m, sum);
+    get_row<kL, kW>(s_base, E, l, u);
 #pragma unroll
-    for (int i = 0; i < kN; ++i) dot = fmaf(x[i], base[i], dot);
+    for (int i = 0; i < kN; ++i) dot = fmaf(x[i], u[i], dot);
     sum = lanes_sum<kL>(sum);
     dot = lanes_sum<kL>(dot);
     const float inv = 1.f / sum;
     float add = g_z * (m + logf(sum)) - dot * inv;
     if (grad_w == nullptr) {
 #pragma unroll
-      for (int i = 0; i < kN; ++i) x[i] = x[i] * inv * (base[i] + add);
+      for (int i = 0; i < kN; ++i) x[i] = x[i] * inv * (u[i] + add);
     } else {
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        x[i] *= inv;
-        const int e = expert_of<kL, kW>(i, l);
-        if (e < E) row[e] = x[i];
-      }
+      for (int i = 0; i < kN; ++i) x[i] *= inv;
+      put_row<kL, kW>(row, E, l, x);
       __syncwarp();
       // p of the picked experts, their sum and its product with the gradients; slots past the lanes in further turns
       float s = 0.f, gs = 0.f;
@@ -382,10 +402,8 @@ router_backward_kernel(void* __restrict__ grad, const void* __restrict__ logits,
       if (!renormalize) add -= gs;  // sum p du, which the renormalisation makes zero
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const int e = expert_of<kL, kW>(i, l);
-        if (e < E) row[e] = base[i] + add;  // u - sum p u + g_z 2 lse / n
-      }
+      for (int i = 0; i < kN; ++i) u[i] += add;  // u - sum p u + g_z 2 lse / n
+      put_row<kL, kW>(row, E, l, u);
       __syncwarp();
       for (int j0 = 0; j0 < k; j0 += kL) {
         if (j0 > 0) {
@@ -410,11 +428,9 @@ router_backward_kernel(void* __restrict__ grad, const void* __restrict__ logits,
         if (lead) row[id] += du;
         __syncwarp();
       }
+      get_row<kL, kW>(row, E, l, u);
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const int e = expert_of<kL, kW>(i, l);
-        if (e < E) x[i] *= row[e];
-      }
+      for (int i = 0; i < kN; ++i) x[i] *= u[i];
     }
     if (tok >= T) continue;
     const size_t off = static_cast<size_t>(tok) * E;
@@ -534,7 +550,7 @@ int launch_router_backward(void* grad_logits, const void* gating, int gating_is_
   if (int st = check_router("router_backward", T, E, k)) return st;
   if (T == 0) return kStatusOk;
   const int tokens = 8 * 32 / lanes_of(E);  // of a CTA at a time
-  const size_t smem = grad_topk_weights != nullptr ? static_cast<size_t>(tokens) * E * sizeof(float) : 0;
+  const size_t smem = (grad_topk_weights != nullptr ? tokens + 1ull : 1ull) * ((E + 3) & ~3) * sizeof(float);
   const cudaError_t e = with_lanes(E, on_16(gating) && on_16(grad_logits), [&](auto lc, auto wc, auto nc) {
     constexpr int L = decltype(lc)::value, W = decltype(wc)::value, N = decltype(nc)::value;
     auto kernel = gating_is_bf16 ? router_backward_kernel<true, L, W, N> : router_backward_kernel<false, L, W, N>;
