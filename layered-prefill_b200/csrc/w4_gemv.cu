@@ -22,9 +22,12 @@
 //
 // Work: a tile is 16 * kRB weight rows x one block of up to 8 * kTB tokens; a CTA takes consecutive tiles, so that it
 // meets few token blocks. The activations of a window of them stay in shared memory as the integers above, in the
-// order in which the codes come, next to their group sums. A worker is 1 to 16 warps that split a tile's columns. Every warp streams codes through a
-// FIFO of its own (16-byte cp.async, four 128-column steps deep) that runs on into the next tile, so no warp waits for another
-// inside a window.
+// order in which the codes come, next to their group sums. A worker is 1 to 16 warps that split a tile's columns. Every warp
+// streams codes through a FIFO of its own (16-byte cp.async, four 128-column steps deep) that runs on into the next tile, so
+// no warp waits for another inside a window. What bounds it now: the instructions of a step (about 200 for 32 rows, at two a cycle
+// and SM) and of a tile's end; the same loop without products reads at 5.2 to 5.7 TB/s, with them at 4.1 to 4.6.
+// Measured (graph replay): 64 tokens over 128 experts, H = 2048, I = 768: 82 us, 3.7 TB/s, against 205 us of the bf16 experts;
+// 93 tokens, H = 4096, I = 1536, groups of 64: 335 us, 3.9 TB/s; N = 131075, K = 2048, groups of 32, five tokens: 40 us, 3.8 TB/s.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -506,19 +509,17 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
         ++row;
       }
       const int r = min(row, n - 1);
-      {
-        const int col = c0 + c * kChunk + col_of<kGpc>(u >> 2, u & 3);
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        using X = std::conditional_t<kMode == kDown, float, __nv_bfloat16>;
-        if (col < p.K) load_x8(static_cast<const X*>(p.x) + source_row(r) * p.x_ld + col, v);
-        uint4 ints;
-        int sum;
-        const float f = quant_x<kGpc, kMode == kDown>(v, ints, sum);
-        *reinterpret_cast<uint4*>(x_mem + r * x_ld + c * 256 + u * 16) = ints;
-        constexpr int kUnits = 16 / kGpc;
-        if (u % kUnits == 0) x_sum[r * xs_ld + c * (kGpc + 1) + u / kUnits] = static_cast<float>(sum);
-        if (u == 0) x_sum[r * xs_ld + c * (kGpc + 1) + kGpc] = f;
-      }
+      const int col = c0 + c * kChunk + col_of<kGpc>(u >> 2, u & 3);
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      using X = std::conditional_t<kMode == kDown, float, __nv_bfloat16>;
+      if (col < p.K) load_x8(static_cast<const X*>(p.x) + source_row(r) * p.x_ld + col, v);
+      uint4 ints;
+      int sum;
+      const float f = quant_x<kGpc, kMode == kDown>(v, ints, sum);
+      *reinterpret_cast<uint4*>(x_mem + r * x_ld + c * 256 + u * 16) = ints;
+      constexpr int kUnits = 16 / kGpc;
+      if (u % kUnits == 0) x_sum[r * xs_ld + c * (kGpc + 1) + u / kUnits] = static_cast<float>(sum);
+      if (u == 0) x_sum[r * xs_ld + c * (kGpc + 1) + kGpc] = f;
       c += 2 * kWarps;
     }
   };
@@ -981,7 +982,8 @@ cudaError_t launch_mode(const W4Params& p, long long blocks, int x_rows, void* x
 }
 
 // Room for the integers of `rows` activations of K columns, 0 where the CTAs make them themselves: up to kPreparedChunks chunks
-// of 128 columns, two turns of a CTA's warps, for which a launch in front takes longer than it saves.
+// of 128 columns, two turns of a CTA's warps, for which a launch in front takes longer than it saves (N = 4096: 80 chunks 6.8 us
+// prepared and 7.2 without, 512 chunks 11.3 and 14.6; the experts of one token, 16 chunks, 16.9 and 15.9).
 size_t prepared_bytes(int rows, int K, int group) {
   const size_t chunks = static_cast<size_t>(rows) * ((K + kChunk - 1) / kChunk);
   return chunks <= kPreparedChunks ? 0 : chunks * (256 + 4 * (kChunk / group + 1));

@@ -234,7 +234,7 @@ def router_loss(losses: torch.Tensor, counts: torch.Tensor, num_tokens: torch.Te
            (losses, torch.float32, (2,)), (counts, torch.int32, (E,)), (num_tokens, torch.int32, (1,)),
            (mean_probs, torch.float32, (E,)))
     ws, nbytes = None, 0
-    if T > 128:  # one CTA takes no more, and needs no room
+    if T > 128 or T * E > 16384:  # below, one CTA does it without
         nbytes = lib.moe_b200_router_loss_workspace_bytes(T, E)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _launch(lib.moe_b200_router_loss, dev, losses.data_ptr(), counts.data_ptr(), num_tokens.data_ptr(), mean_probs.data_ptr(),
