@@ -301,6 +301,7 @@ router_loss_kernel(const void* __restrict__ logits, const int* __restrict__ ids,
 }
 
 __global__ void __launch_bounds__(1024) router_loss_finish_kernel(LossParts w, int blocks, int E, LossOut out) {
+  cluster_sync_all();  // every CTA has started: its shared memory may be written from now on
   grid_dependency_wait();
   grid_dependency_launch();
   finish_losses<kFinishCtas>(w, blocks, E, out, static_cast<int>(cluster_ctarank()));
@@ -558,7 +559,7 @@ int launch_router_backward(void* grad_logits, const void* gating, int gating_is_
     constexpr int L = decltype(lc)::value, W = decltype(wc)::value, N = decltype(nc)::value;
     auto kernel = gating_is_bf16 ? router_backward_kernel<true, L, W, N> : router_backward_kernel<false, L, W, N>;
     // as many CTAs as are resident, each with several tokens a lane group in turn, so that the counts are fetched once and
-    // the next logits are on their way (T = 65519, E = 160: 37 us both passes; 42 us with four times the CTAs)
+    // the next logits are on their way (T = 65519, E = 160: 38 us both passes; 42 us with four times the CTAs)
     const int most = device_sm_count() * 2;
     const int want = (T + tokens - 1) / tokens;
     return launch_pdl(kernel, dim3(want < most ? want : most), dim3(256), smem, stream, grad_logits, gating, topk_ids, counts,
