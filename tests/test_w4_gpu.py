@@ -207,6 +207,20 @@ def test_interleaved_activation_and_biases(T):
         _check_experts(_experts(x, w13, w2, tw, ti, 64, b13, b2, act), x, w13, w2, b13, b2, tw, ti, 64, act)
 
 
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("act", ["silu", "swigluoai"])
+def test_values_that_are_not_finite_reach_their_token_through_the_experts(T, act):
+    x, w13, w2, tw, ti = _case(T, 256, 8, 2, 128, 64, True, 12)
+    want = _experts(x, w13, w2, tw, ti, 64, None, None, act)
+    for value in (float("nan"), float("inf"), float("-inf")):
+        bad = x.clone()
+        bad[1, 77] = value
+        out = _experts(bad, w13, w2, tw, ti, 64, None, None, act)
+        assert out[1].isnan().all()
+        rest = [t for t in range(T) if t != 1]
+        assert torch.equal(out[rest], want[rest])
+
+
 def test_one_expert_takes_every_token():
     x, w13, w2, tw, ti = _case(90, 256, 8, 1, 128, 32, False, 2)
     ti[:] = 5
