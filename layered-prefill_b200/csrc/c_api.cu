@@ -521,7 +521,7 @@ size_t moe_b200_w4_linear_workspace_bytes(int M, int K, int group_size) {
 int moe_b200_w4_linear(void* out, const void* x, int64_t x_row_stride, const void* qweight, const void* scale,
                        const void* zero, const void* bias, int M, int N, int K, int group_size, void* workspace,
                        size_t workspace_bytes, void* stream) {
-  if (M < 0 || N <= 0) return set_error(kStatusInvalidArgument, "w4_linear: bad sizes M=%d N=%d", M, N);
+  if (M < 0 || M > 0x3fffffff || N <= 0) return set_error(kStatusInvalidArgument, "w4_linear: bad sizes M=%d N=%d", M, N);
   if (int st = check_w4_group("w4_linear", group_size, K)) return st;
   if (M == 0) return kStatusOk;
   if (out == nullptr || x == nullptr || qweight == nullptr || scale == nullptr)

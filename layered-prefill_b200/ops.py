@@ -114,6 +114,9 @@ def topk_softmax_renorm(topk_weights: torch.Tensor, topk_indices: torch.Tensor, 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(device).cuda_stream, without the Stream object (5 us a call)
 
 
+_MAX_ROWS = 2**30 - 1  # tokens of a call: their number crosses the C interface as an int
+
+
 def _launch(fn, device: torch.device, *args) -> None:
     """check(fn(*args, current stream)) with `device` current."""
     idx = device.index
@@ -158,6 +161,8 @@ def _norm_quant(op, out, scales, residual, input, weight, epsilon, group_size, n
     bf16, shape, device = torch.bfloat16, input.shape, input.device
     H = shape[-1] if shape else 0
     T = input.numel() // H if H else 0
+    if T > _MAX_ROWS:
+        raise RuntimeError(f"{op}: at most {_MAX_ROWS} tokens, got {T}")
     groups = 1 if group_size == -1 or (group_size == H and H != 128) else H // 128
     _check(op, device, "input out weight scales residual residual_out normed_out", (input, bf16, shape),
            (out, torch.float8_e4m3fn, shape), (weight, bf16, (H,)), (scales, torch.float32, (*shape[:-1], groups)),
@@ -195,6 +200,8 @@ def w4_linear(out: torch.Tensor, input: torch.Tensor, qweight: torch.Tensor, sca
         raise RuntimeError("w4_linear: qweight must be [N, K / 2], scales [N, K / group] and input [.., K]")
     K, N, groups = shape[-1], q_shape[0], s_shape[1]
     M = input.numel() // K
+    if M > _MAX_ROWS:
+        raise RuntimeError(f"w4_linear: at most {_MAX_ROWS} tokens, got {M}")
     bf16, u8, device, ld, checked = torch.bfloat16, torch.uint8, qweight.device, K, (input, torch.bfloat16, shape)
     if len(shape) == 2 and not input.is_contiguous() and input.stride(1) == 1:
         ld, checked = input.stride(0), (input[:1], bf16, (min(M, 1), K))
@@ -202,7 +209,7 @@ def w4_linear(out: torch.Tensor, input: torch.Tensor, qweight: torch.Tensor, sca
            (qweight, u8, (N, K // 2)), (scales, bf16, (N, groups)), (zeros, u8, (N, groups)), (bias, bf16, (N,)))
     group = K // groups if K % groups == 0 else -1
     ws, nbytes = None, 0
-    if M * K > 8192:  # below, no room is ever asked for
+    if M * (K + 127) > 8192:  # below, no room is ever asked for
         nbytes = lib.moe_b200_w4_linear_workspace_bytes(M, K, group)
         ws = torch.empty(nbytes, dtype=u8, device=device) if nbytes else None
     _launch(lib.moe_b200_w4_linear, device, out.data_ptr(), input.data_ptr(), ld, qweight.data_ptr(), scales.data_ptr(),
@@ -217,6 +224,8 @@ def _router_args(op, gating_output, topk_ids, token_mask):
         raise RuntimeError(f"{op}: gating_output must be float32 or bfloat16")
     T, E = gating_output.shape
     k = topk_ids.size(1)
+    if T > _MAX_ROWS:
+        raise RuntimeError(f"{op}: at most {_MAX_ROWS} tokens, got {T}")
     specs = ((gating_output, gating_output.dtype, (T, E)), (topk_ids, torch.int32, (T, k)),
              (token_mask, torch.uint8 if token_mask is not None and token_mask.dtype == torch.uint8 else torch.bool, (T,)))
     return T, E, k, specs

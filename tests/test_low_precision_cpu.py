@@ -42,6 +42,7 @@ def test_w4_linear_refusals():
     assert f(P, P + 2, 256, P, P, None, None, 1, 8, 256, 64, None) == 1 and "16 bytes" in err()
     assert f(P, P, 256, P + 8, P, None, None, 1, 8, 256, 64, None) == 1
     assert f(P, P, 256, P, None, None, None, 1, 8, 256, 64, None) == 1 and "null" in err()
+    assert f(P, P, 256, P, P, None, None, 1 << 30, 8, 256, 64, None) == 1 and "sizes" in err()
     need = room(16, 8192, 64)
     assert need > 16 * 8192 * 2 and room(1, 2048, 128) == 0 and room(0, 2048, 128) == 0 and room(64, 8192, 48) == 0
     assert f(P, P, 8192, P, P, None, None, 16, 8, 8192, 64, None, P, need - 1) == 3 and "workspace" in err()
@@ -89,6 +90,23 @@ def test_cpu_tensors_are_refused():
         ops.w4_linear(torch.zeros(2, 8, dtype=torch.bfloat16), x, q, s)
     with pytest.raises(RuntimeError):
         fused_moe.fused_topk_with_loss(torch.zeros(2, 4), 2, True)
+
+
+def test_more_tokens_than_an_int_counts_are_refused():
+    """2^32 + 1 would cross the C interface as 1. The tensors are one row seen many times."""
+    from layered_prefill_b200 import ops
+    T = 2**32 + 1
+    row = lambda n, dtype: torch.zeros(1, n, dtype=dtype).expand(T, n)  # noqa: E731
+    bf16 = torch.bfloat16
+    with pytest.raises(RuntimeError, match="at most"):
+        ops.rms_norm_quant_fp8(row(8, torch.float8_e4m3fn), row(1, torch.float32), row(8, bf16), torch.zeros(8, dtype=bf16), 1e-6, -1)
+    with pytest.raises(RuntimeError, match="at most"):
+        ops.w4_linear(row(8, bf16), row(32, bf16), torch.zeros(8, 16, dtype=torch.uint8), torch.zeros(8, 1, dtype=bf16))
+    one = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="at most"):
+        ops.router_loss(torch.zeros(2), one, one, torch.zeros(1), row(1, torch.float32), row(1, torch.int32))
+    with pytest.raises(RuntimeError, match="at most"):
+        ops.router_backward(row(1, torch.float32), row(1, torch.float32), row(1, torch.int32), one, one, None, None, True)
 
 
 @pytest.mark.parametrize("group", [32, 64, 128])
