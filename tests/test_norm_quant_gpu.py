@@ -126,6 +126,16 @@ def test_rows_past_the_batch_stay_and_leading_dimensions():
     ops.rms_norm_quant_fp8(q[:0], s[:0], x[:0], w, 1e-6)  # no token
 
 
+def test_offsets_past_32_bits():
+    g = torch.Generator(device="cuda").manual_seed(2)
+    T, H = 2**18 + 70, 16384
+    x = torch.randn(T, H, generator=g, device="cuda", dtype=torch.bfloat16)
+    w = (1 + 0.2 * torch.randn(H, generator=g, device="cuda")).to(torch.bfloat16)
+    q, s, n, _ = _run(x, None, w, 128, True)
+    for lo, hi in ((0, 9), (2**17 - 4, 2**17 + 4), (2**18 - 4, 2**18 + 4), (T - 9, T)):
+        _check(q[lo:hi], s[lo:hi], n[lo:hi], x[lo:hi], w, 128)
+
+
 def test_on_another_stream_and_in_a_graph():
     from layered_prefill_b200 import ops
     x, res, w = _inputs(33, 1024, 3)

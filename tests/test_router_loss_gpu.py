@@ -99,6 +99,20 @@ def test_masked_tokens_count_for_nothing_whatever_they_hold(dtype):
     assert all(torch.equal(a, b) for a, b in zip(got, same))
 
 
+def test_offsets_past_32_bits():
+    T, E, k, n = 2**22 + 101, 1024, 2, 60
+    part = _inputs(2 * n, E, k, torch.bfloat16, 11)
+    ends = torch.cat((torch.arange(n), torch.arange(T - n, T))).cuda()
+    logits = torch.full((T, E), float("nan"), dtype=torch.bfloat16, device="cuda")
+    ids = torch.zeros(T, k, dtype=torch.int32, device="cuda")
+    mask = torch.zeros(T, dtype=torch.bool, device="cuda")
+    g_w = torch.zeros(T, k, device="cuda")
+    logits[ends], ids[ends], mask[ends], g_w[ends] = part[0], part[1], True, part[3]
+    losses, counts, live, mean, grad = _run(logits, ids, mask, g_w, part[4])
+    assert not grad[n:-n].any()
+    _check((losses, counts, live, mean, grad[ends]), _oracle(*part), torch.bfloat16)
+
+
 def test_no_token_counts():
     logits, ids, _, g_w, g_l = _inputs(20, 16, 2, torch.float32, 2)
     losses, counts, n, mean, grad = _run(logits, ids, torch.zeros(20, dtype=torch.bool, device="cuda"), g_w, g_l)

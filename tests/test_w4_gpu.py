@@ -368,6 +368,48 @@ def test_on_scales_and_codes_between_the_usual_boundaries():
         _linear(x, q2, s, z)
 
 
+def _big(shape_n, k, group, lead, g):
+    packed = torch.randint(0, 256, (*lead, shape_n, k // 2), generator=g, dtype=torch.uint8, device="cuda")
+    scale = (0.01 + 0.02 * torch.rand(*lead, shape_n, k // group, generator=g, device="cuda")).to(torch.bfloat16)
+    return packed, scale, None
+
+
+def test_dense_codes_past_32_bits():
+    g = torch.Generator(device="cuda").manual_seed(3)
+    N, K = 2**20 + 1003, 8192  # 4096 bytes a row: the last 1003 rows lie past 2^32 bytes
+    packed, scale, _ = _big(N, K, 128, (), g)
+    x = torch.randn(2, K, generator=g, device="cuda").to(torch.bfloat16)
+    out = _linear(x, packed, scale, None)
+    for lo, hi in ((0, 40), (2**19 - 20, 2**19 + 20), (2**20 - 20, 2**20 + 20), (N - 40, N)):
+        _check_linear(out[:, lo:hi], x, packed[lo:hi], scale[lo:hi], None)
+
+
+def test_as_many_experts_as_may_be_with_codes_past_32_bits():
+    g = torch.Generator(device="cuda").manual_seed(6)
+    E, H, I = 1024, 8192, 1024
+    w13, w2 = _big(2 * I, H, 128, (E,), g), _big(H, I, 128, (E,), g)
+    x = torch.randn(3, H, generator=g, device="cuda").to(torch.bfloat16)
+    ti = torch.tensor([[0, 1023, 511, 900], [1023, 512, 1, 700], [1022, 1023, 600, 513]], dtype=torch.int32, device="cuda")
+    tw = torch.rand(3, 4, generator=g, device="cuda")
+    _check_experts(_experts(x, w13, w2, tw, ti, 128), x, w13, w2, None, None, tw, ti, 128, "silu")
+
+
+def test_as_many_slots_a_token_as_may_be():
+    x, w13, w2, _, _ = _case(2, 128, 1024, 1, 32, 32, False, 15)
+    g = torch.Generator().manual_seed(15)
+    ti = torch.stack([torch.randperm(1024, generator=g) for _ in range(2)]).to(torch.int32).cuda()
+    tw = torch.rand(2, 1024, generator=g).cuda()
+    out = _experts(x, w13, w2, tw, ti, 32)
+    want, bound = _experts64(x, w13, w2, None, None, tw, ti, 32, "silu")
+    # 1024 slots in a row of fp32 additions: a rounding each of at most the sum of the magnitudes
+    w13d, w2d = _dense64(*w13, 32), _dense64(*w2, 32)
+    gate, up = torch.einsum("th,enh->ten", x.double(), w13d).chunk(2, -1)
+    y = torch.einsum("ten,ehn->teh", _act64(gate, up, "silu"), w2d)
+    sizes = (y.abs() * tw.double().gather(1, ti.long().argsort(1))[..., None]).sum(1)
+    err = (out.double() - want).abs()
+    assert (err <= bound + 1024 * 2.0 ** -24 * sizes).all()
+
+
 def test_dense_on_two_streams_at_once_and_in_a_graph():
     g = torch.Generator().manual_seed(14)
     w = _weights(2048, 4096, 128, False, g)
