@@ -77,6 +77,14 @@ def test_one_scale_a_token(T, H, residual):
     _check(q, s, n, r, w, -1)
 
 
+@pytest.mark.parametrize("H", [12288, 12296, 32768])
+def test_where_a_thread_takes_more_vectors(H):
+    x, res, w = _inputs(3, H, H)
+    for group in (128, -1) if H % 128 == 0 else (-1,):
+        q, s, n, r = _run(x, res, w, group, True)
+        _check(q, s, n, r, w, group)
+
+
 def test_residual_in_place_and_the_same_bits_twice():
     x, res, w = _inputs(40, 2048, 5)
     a, b = _run(x, res, w, 128, True), _run(x, res, w, 128, True, in_place=True)

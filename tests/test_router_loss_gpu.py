@@ -84,6 +84,14 @@ def test_losses_counts_and_gradients(T, E, k, dtype):
         _check(_run(*args, renorm), _oracle(*args, renorm), dtype)
 
 
+@pytest.mark.parametrize("T,E,k", [(5, 1024, 8), (16, 1024, 1024), (16, 1001, 3), (128, 128, 128), (129, 127, 9), (17, 1023, 200)])
+def test_sizes_at_the_edges_of_the_shapes(T, E, k):
+    for dtype in (torch.bfloat16, torch.float32):
+        args = _inputs(T, E, k, dtype, T * E, masked=0.2)
+        for renorm in (True, False):
+            _check(_run(*args, renorm), _oracle(*args, renorm), dtype)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_masked_tokens_count_for_nothing_whatever_they_hold(dtype):
     logits, ids, mask, g_w, g_l = _inputs(300, 96, 4, dtype, 1, masked=0.4)
