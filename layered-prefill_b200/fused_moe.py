@@ -329,16 +329,27 @@ def quant_w4(weight: torch.Tensor, group_size: int = 128, zero_points: bool = Fa
     return code[..., 0::2] | (code[..., 1::2] << 4), scale, zero.to(torch.uint8) if zero_points else None
 
 
-def shard_w4_expert_weights(w13, w2, tp_rank: int, tp_size: int, group_size: int):
+def shard_w4_expert_weights(w13, w2, tp_rank: int, tp_size: int, group_size: int, activation: str = "silu"):
     """Slices 4-bit expert weights over the intermediate dimension the way FusedMoE.weight_loader slices bf16 ones
-    (nanovllm/layers/fused_moe.py:400-470). w13 and w2 are quant_w4's (codes, scales, zeros) of [E, 2I, H] and [E, H, I];
-    a rank's share of I has to be a whole number of groups. Returns the two triples of this rank. Works on any device."""
+    (nanovllm/layers/fused_moe.py:400-470): for silu, whose w13 holds the gate rows and then the up rows, this rank's part of
+    each; for swigluoai, whose gate and up rows alternate, the rows between. w13 and w2 are quant_w4's (codes, scales, zeros) of
+    [E, 2I, H] and [E, H, I]; a rank's share of I has to be a whole number of groups. Returns the two triples of this rank. Works
+    on any device."""
+    if activation not in ACT_CODES:
+        raise ValueError(f"Unsupported FusedMoe activation: {activation}")
     inter = w13[0].size(1) // 2
     if inter % tp_size or (inter // tp_size) % group_size:
         raise ValueError(f"a rank's share of I={inter} over {tp_size} ranks must be a whole number of groups of {group_size}")
     ip = inter // tp_size
     lo, hi = tp_rank * ip, (tp_rank + 1) * ip
-    rows = lambda t: None if t is None else torch.cat([t[:, lo:hi], t[:, inter + lo:inter + hi]], dim=1)  # noqa: E731
+
+    def rows(t):
+        if t is None:
+            return None
+        if activation == "swigluoai":
+            return t[:, 2 * lo:2 * hi].contiguous()
+        return torch.cat([t[:, lo:hi], t[:, inter + lo:inter + hi]], dim=1)
+
     cols = lambda t, per: None if t is None else t[:, :, lo // per:hi // per].contiguous()  # noqa: E731
     return tuple(rows(t) for t in w13), tuple(cols(t, per) for t, per in zip(w2, (2, group_size, group_size)))
 

@@ -160,3 +160,37 @@ def test_w4_row_parallel_linear_loads_and_refuses():
     assert torch.equal(layer.qweight, q2[:, 128:]) and torch.equal(layer.scales, s2[:, 4:])
     with pytest.raises(ValueError):
         linear.W4RowParallelLinear(192, 8, group_size=128)
+
+
+@pytest.mark.parametrize("activation", ["silu", "swigluoai"])
+@pytest.mark.parametrize("tp", [2, 4])
+def test_expert_shards_add_up_to_the_whole(activation, tp):
+    """The partial results of the ranks, each from its own shard, sum to the unsharded experts' result."""
+    from layered_prefill_b200 import fused_moe
+    E, I, H, g = 3, 128, 64, 32
+    gen = torch.Generator().manual_seed(tp)
+    w13, w2 = (fused_moe.quant_w4(torch.randn(*s, generator=gen) * 0.2, g, True) for s in ((E, 2 * I, H), (E, H, I)))
+    x = torch.randn(5, H, generator=gen, dtype=torch.float64)
+
+    def dense(w):
+        codes, scale, zero = w
+        code = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).double()
+        return (code - zero.double().repeat_interleave(g, -1)) * scale.double().repeat_interleave(g, -1)
+
+    def experts(a, b):  # [E, T, H]: every token through every expert
+        gu = torch.einsum("th,enh->etn", x, dense(a))
+        if activation == "silu":
+            gate, up = gu.chunk(2, -1)
+            h = gate * torch.sigmoid(gate) * up
+        else:  # gate and up rows alternate
+            gate, up = gu[..., 0::2].clamp(max=7), gu[..., 1::2].clamp(-7, 7)
+            h = gate * torch.sigmoid(1.702 * gate) * (up + 1)
+        return torch.einsum("eti,ehi->eth", h, dense(b))
+
+    whole = experts(w13, w2)
+    parts = [fused_moe.shard_w4_expert_weights(w13, w2, r, tp, g, activation) for r in range(tp)]
+    assert all(t.is_contiguous() for p in parts for triple in p for t in triple)
+    # 64-bit sums of I + H terms in another order
+    assert (sum(experts(*p) for p in parts) - whole).abs().max() <= (I + H) * 2.0 ** -52 * whole.abs().max() * 16
+    with pytest.raises(ValueError):
+        fused_moe.shard_w4_expert_weights(w13, w2, 0, tp, g, "gelu")
