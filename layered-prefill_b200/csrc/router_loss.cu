@@ -136,14 +136,17 @@ struct LossParts {
 
 constexpr int kFinishCtas = 8;
 
+struct FinishShared {
+  double red[32], s_p[1024], s_bal[kFinishCtas], s_z;
+  int s_c[1024], s_n;
+};
+
 // The sums over `blocks` rows of parts, and the outputs. Called by all threads of a CTA (rank 0 of 1) or of a cluster of
 // kFinishCtas, whose CTAs take E / ranks experts each; several threads share an expert's rows. Fixed orders throughout.
 template <int kRanks>
 __device__ void finish_losses(const LossParts& w, int blocks, int E, const LossOut& out, int rank) {
-  __shared__ double red[32], s_p[1024], s_bal[kFinishCtas];
-  __shared__ int s_c[1024];
-  __shared__ int s_n;
-  __shared__ double s_z;
+  __shared__ FinishShared sh;
+  auto& [red, s_p, s_bal, s_z, s_c, s_n] = sh;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int per = (E + kRanks - 1) / kRanks, e0 = rank * per, mine = max(0, min(per, E - e0));
   const int parts = static_cast<int>(blockDim.x) / per;  // blockDim.x >= per
@@ -498,9 +501,14 @@ cudaError_t with_lanes(int E, bool vectors, F&& f) {
 
 bool on_16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// What the kernel holds in fixed arrays counts against the 48 KB that it may have without asking, too. It asks for the most that
+// any call needs, so that calls of two host threads ask for the same.
+constexpr size_t kLossFixedSmem = sizeof(FinishShared) + kOneWarps * (sizeof(float) + sizeof(int));
+constexpr size_t kLossMostSmem = (kOneWarps + 1) * kMaxExperts * sizeof(float);
 template <typename K>
-cudaError_t allow_smem(K kernel, size_t bytes) {
-  return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) : cudaSuccess;
+cudaError_t allow_loss_smem(K kernel, size_t dynamic) {
+  if (dynamic + kLossFixedSmem <= 48 * 1024) return cudaSuccess;
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLossMostSmem));
 }
 
 int check_router(const char* what, int T, int E, int k) {
@@ -536,7 +544,7 @@ int launch_router_loss(float* losses, int* counts, int* num_tokens, float* mean_
   const cudaError_t e = with_lanes(E, on_16(gating), [&](auto lc, auto wc, auto nc) {
     constexpr int L = decltype(lc)::value, W = decltype(wc)::value, N = decltype(nc)::value;
     auto kernel = gating_is_bf16 ? router_loss_kernel<true, L, W, N> : router_loss_kernel<false, L, W, N>;
-    const cudaError_t a = allow_smem(kernel, smem);
+    const cudaError_t a = allow_loss_smem(kernel, smem);
     if (a != cudaSuccess) return a;
     return launch_pdl(kernel, dim3(blocks), dim3(warps * 32), smem, stream, gating, topk_ids, token_mask, T, E, k, static_cast<int>(one_cta(T, E)), w, out);
   });
@@ -554,7 +562,7 @@ int launch_router_backward(void* grad_logits, const void* gating, int gating_is_
   if (int st = check_router("router_backward", T, E, k)) return st;
   if (T == 0) return kStatusOk;
   const int tokens = 8 * 32 / lanes_of(E);  // of a CTA at a time
-  const size_t smem = (grad_topk_weights != nullptr ? tokens + 1ull : 1ull) * ((E + 3) & ~3) * sizeof(float);
+  const size_t smem = (grad_topk_weights != nullptr ? tokens + 1ull : 1ull) * ((E + 3) & ~3) * sizeof(float);  // at most 36 KB, and no fixed arrays
   const cudaError_t e = with_lanes(E, on_16(gating) && on_16(grad_logits), [&](auto lc, auto wc, auto nc) {
     constexpr int L = decltype(lc)::value, W = decltype(wc)::value, N = decltype(nc)::value;
     auto kernel = gating_is_bf16 ? router_backward_kernel<true, L, W, N> : router_backward_kernel<false, L, W, N>;

@@ -260,3 +260,34 @@ def test_refusals():
                         torch.empty(1025, device="cuda"), big, ids[:2])
     with pytest.raises(RuntimeError):
         ops.router_backward(torch.empty_like(logits).bfloat16(), logits, ids, o["counts"], o["num_tokens"], g_l, g_w, True)
+
+
+_FRESH = """
+import sys
+sys.path.insert(0, {root!r})
+import torch
+from tests.test_router_loss_gpu import _check, _inputs, _oracle, _run
+failed = []
+for T, E in {shapes!r}:
+    for dtype in (torch.bfloat16, torch.float32):
+        args = _inputs(T, E, 3, dtype, T + E)
+        try:
+            _check(_run(*args), _oracle(*args), dtype)
+        except Exception as e:
+            failed.append((T, E, str(dtype), str(e)[:200]))
+assert not failed, failed
+print("OK")
+"""
+
+
+@pytest.mark.parametrize("shapes", [((50, 288), (32, 320), (16, 372), (300, 576), (300, 640), (300, 720)),
+                                    ((50, 277), (16, 371), (300, 577), (300, 721))])
+def test_shared_memory_just_below_48_kb_in_a_process_of_its_own(shapes):
+    """132 E bytes (one CTA) or 68 E (several) of dynamic shared memory below 48 KB that pass it with the kernel's own arrays. What
+    a kernel may take stays set in a process, so no larger call may come before: sizes ascend, E in vectors and not."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _FRESH.format(root=root, shapes=shapes)], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0 and "OK" in r.stdout, r.stderr[-2000:]
