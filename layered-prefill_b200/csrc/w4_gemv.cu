@@ -735,13 +735,12 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
 #pragma unroll
                 for (int o = 0; o < 2; ++o) {
                   const float xs = xs_at[tb][o][kSlot * (kGpc + 1) + q];
-                  const float off = fmaf(8.f, xs, kFloatBias);
 #pragma unroll
                   for (int i = 0; i < 2 * kRB; ++i) {
-                    // 256 times the high sum, exactly; the low sum still has its bias, which leaves with the zero point's share
-                    const float sum = fmaf(__int_as_float(high[i >> 1][tb][2 * (i & 1) + o]), 256.f, -256.f * kFloatBias) +
-                                      __int_as_float(low[i >> 1][tb][2 * (i & 1) + o]);
-                    const float v = kZero ? fmaf(z[i], xs, sum - kFloatBias) : sum - off;
+                    // 256 times the high sum and the zero point's share meet first, with the low sum's bias taken off: where the
+                    // weights cancel, what is left is below 2^24 and every step exact (weights of zero give zero)
+                    const float high_sum = fmaf(__int_as_float(high[i >> 1][tb][2 * (i & 1) + o]), 256.f, -257.f * kFloatBias);
+                    const float v = fmaf(kZero ? z[i] : -8.f, xs, high_sum) + __int_as_float(low[i >> 1][tb][2 * (i & 1) + o]);
                     float& acc = part[i >> 1][tb][2 * (i & 1) + o];
                     acc = q == 0 ? s[i] * v : fmaf(s[i], v, acc);
                   }

@@ -464,3 +464,26 @@ def test_refusals():
             fused_moe.fused_experts(x, w13[0], w2[0], None, None, tw, ti, **{**good, **bad})
     with pytest.raises(RuntimeError):
         fused_moe.fused_experts(x.float(), w13[0], w2[0], None, None, tw, ti, **good)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_weights_of_zero_give_zero(group, zeros):
+    """Codes equal to their zero points, scales that are not zero, activations of one sign and of many magnitudes."""
+    g = torch.Generator().manual_seed(group)
+    N, K = 48, 640
+    zp = torch.randint(9, 16, (N, K // group), generator=g, dtype=torch.uint8) if zeros else torch.full((N, K // group), 8, dtype=torch.uint8)
+    code = zp.repeat_interleave(group, 1)
+    packed = (code[:, 0::2] | (code[:, 1::2] << 4)).cuda()
+    scale = torch.rand(N, K // group, generator=g).add(0.5).to(torch.bfloat16).cuda()
+    for M in (1, 7, 16, 40):
+        x = (torch.rand(M, K, generator=g) * 2.0 ** torch.randint(-6, 1, (M, K), generator=g)).to(torch.bfloat16).cuda()
+        assert (_linear(x, packed, scale, zp.cuda() if zeros else None) == 0).all()
+    I = 128
+    x, w13, _, tw, ti = _case(9, 128, 4, 2, I, group, zeros, 3)
+    zp = zp[:, :1].repeat(3, I // group)[:128]
+    code = zp.repeat_interleave(group, 1)
+    w2 = (code[:, 0::2] | (code[:, 1::2] << 4)).expand(4, 128, I // 2).contiguous().cuda()
+    s2 = torch.ones(4, 128, I // group, dtype=torch.bfloat16, device="cuda")
+    z2 = zp.expand(4, 128, I // group).contiguous().cuda() if zeros else None
+    assert (_experts(x, w13, (w2, s2, z2), tw, ti, group) == 0).all()
