@@ -38,13 +38,22 @@ class RowParallelLinear(nn.Module):
         self.tp_size = dist.get_world_size() if initialised else 1
         self.input_size_per_partition = divide(input_size, self.tp_size)
         self.output_size_per_partition = output_size
-        self.weight = nn.Parameter(torch.empty(self.output_size, self.input_size_per_partition), requires_grad=False)
-        self.weight.weight_loader = self.weight_loader
-        if bias:
-            self.bias = nn.Parameter(torch.empty(self.output_size), requires_grad=False)
-            self.bias.weight_loader = self.weight_loader
-        else:
-            self.register_parameter("bias", None)
+        self._make_weights()
+        self._add_parameter("bias", torch.empty(self.output_size, dtype=self._bias_dtype()) if bias else None)
+
+    def _make_weights(self) -> None:
+        self._add_parameter("weight", torch.empty(self.output_size, self.input_size_per_partition))
+
+    def _bias_dtype(self) -> torch.dtype:
+        return self.weight.dtype
+
+    def _add_parameter(self, name: str, data: Optional[torch.Tensor]) -> None:
+        if data is None:
+            self.register_parameter(name, None)
+            return
+        p = nn.Parameter(data, requires_grad=False)
+        p.weight_loader = self.weight_loader
+        setattr(self, name, p)
 
     def weight_loader(self, param: nn.Parameter, loaded_weight: torch.Tensor) -> None:
         """linear.py:176-186."""
@@ -102,25 +111,23 @@ class RowParallelLinear(nn.Module):
 class W4RowParallelLinear(RowParallelLinear):
     """RowParallelLinear with 4-bit weights and group scales (fused_moe.quant_w4's layout; the product is ops.w4_linear, built for
     decode batches): qweight uint8 [output_size, input_size / tp / 2], scales bf16 [output_size, input_size / tp / group], zeros
-    uint8 like scales or None. weight_loader takes the unsharded codes, scales and zeros and keeps this rank's columns, so
-    a rank's share of the input has to be a whole number of groups."""
+    uint8 like scales or None, the bias bf16. weight_loader takes the unsharded codes, scales and zeros and keeps this rank's
+    columns, so a rank's share of the input has to be a whole number of groups."""
 
     def __init__(self, input_size: int, output_size: int, bias: bool = False, group_size: int = 128, zero_points: bool = False):
+        self.group_size, self._zero_points = group_size, zero_points
         super().__init__(input_size, output_size, bias)
-        k = self.input_size_per_partition
-        if group_size not in (32, 64, 128) or k % group_size:
+
+    def _make_weights(self) -> None:
+        k, group = self.input_size_per_partition, self.group_size
+        if group not in (32, 64, 128) or k % group:
             raise ValueError(f"group_size must be 32, 64 or 128 and divide this rank's {k} input columns")
-        del self.weight
-        self.group_size = group_size
-        shapes = {"qweight": (k // 2, torch.uint8), "scales": (k // group_size, torch.bfloat16),
-                  "zeros": (k // group_size, torch.uint8) if zero_points else None}
-        for name, spec in shapes.items():
-            if spec is None:
-                self.register_parameter(name, None)
-                continue
-            p = nn.Parameter(torch.empty(output_size, spec[0], dtype=spec[1]), requires_grad=False)
-            p.weight_loader = self.weight_loader
-            setattr(self, name, p)
+        self._add_parameter("qweight", torch.empty(self.output_size, k // 2, dtype=torch.uint8))
+        self._add_parameter("scales", torch.empty(self.output_size, k // group, dtype=torch.bfloat16))
+        self._add_parameter("zeros", torch.empty(self.output_size, k // group, dtype=torch.uint8) if self._zero_points else None)
+
+    def _bias_dtype(self) -> torch.dtype:
+        return torch.bfloat16  # what ops.w4_linear takes, whatever the default type is
 
     def _product(self, x: torch.Tensor, out: torch.Tensor) -> None:
         ops.w4_linear(out, x, self.qweight, self.scales, self.zeros, self.bias if self.tp_rank == 0 else None)

@@ -194,3 +194,18 @@ def test_expert_shards_add_up_to_the_whole(activation, tp):
     assert (sum(experts(*p) for p in parts) - whole).abs().max() <= (I + H) * 2.0 ** -52 * whole.abs().max() * 16
     with pytest.raises(ValueError):
         fused_moe.shard_w4_expert_weights(w13, w2, 0, tp, g, "gelu")
+
+
+def test_w4_row_parallel_linear_has_a_bf16_bias_and_no_dense_weight(monkeypatch):
+    from layered_prefill_b200 import linear
+    assert torch.get_default_dtype() == torch.float32
+    sizes, empty = [], torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: sizes.append(empty(*a, **k).nbytes) or empty(*a, **k))
+    layer = linear.W4RowParallelLinear(256, 24, bias=True, group_size=64, zero_points=True)
+    assert layer.bias.dtype == torch.bfloat16 and not layer.bias.requires_grad and not hasattr(layer, "weight")
+    assert max(sizes) == 24 * 128  # the codes
+    assert [n for n, _ in layer.named_parameters()] == ["qweight", "scales", "zeros", "bias"]
+    assert all(callable(p.weight_loader) for p in layer.parameters())
+    assert linear.W4RowParallelLinear(256, 24, group_size=64).bias is None
+    dense = linear.RowParallelLinear(256, 24, bias=True)  # as it was: both in the default type
+    assert dense.weight.shape == (24, 256) and dense.weight.dtype == dense.bias.dtype == torch.float32

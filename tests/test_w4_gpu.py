@@ -487,3 +487,26 @@ def test_weights_of_zero_give_zero(group, zeros):
     s2 = torch.ones(4, 128, I // group, dtype=torch.bfloat16, device="cuda")
     z2 = zp.expand(4, 128, I // group).contiguous().cuda() if zeros else None
     assert (_experts(x, w13, (w2, s2, z2), tw, ti, group) == 0).all()
+
+
+@pytest.mark.parametrize("M", [1, 19])
+def test_row_parallel_linear_with_a_bias_under_the_default_type(M):
+    from layered_prefill_b200 import fused_moe, linear, ops
+    assert torch.get_default_dtype() == torch.float32
+    g = torch.Generator().manual_seed(M)
+    N, K = 256, 512
+    layer = linear.W4RowParallelLinear(K, N, bias=True, group_size=64)
+    for name, value in zip(("qweight", "scales"), fused_moe.quant_w4(torch.randn(N, K, generator=g) * 0.05, 64)):
+        p = getattr(layer, name)
+        p.weight_loader(p, value)
+    layer.bias.weight_loader(layer.bias, torch.randn(N, generator=g))
+    layer = layer.cuda()
+    x = torch.randn(M, K, generator=g).to(torch.bfloat16).cuda()
+    y = layer(x)
+    _check_linear(y, x, layer.qweight, layer.scales, None, layer.bias)
+    residual = torch.randn(M, N, generator=g).to(torch.bfloat16).cuda()
+    norm_w = torch.rand(N, generator=g).to(torch.bfloat16).cuda()
+    normed, res = layer.forward_reduce_norm(x, residual.clone(), norm_w, 1e-6)
+    want = torch.empty_like(y)
+    ops.add_rms_norm(want, residual, y, norm_w, 1e-6)
+    assert torch.equal(normed, want) and torch.equal(res, residual)
