@@ -222,8 +222,10 @@ __device__ __forceinline__ uint32_t cluster_ctarank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-// Barrier over all threads of all CTAs of the cluster; orders shared-memory accesses across the cluster.
+// Barrier over all threads of all CTAs of the cluster; orders shared-memory accesses across the cluster. The aligned forms want the
+// warp's lanes together, which nothing promises behind a branch that some of them took.
 __device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Store one float into the same shared-memory location of CTA `rank` of the cluster.
