@@ -10,8 +10,8 @@
 // Both passes read the logits once and recompute the softmax in registers: writing p and reading it back would cost
 // more than the exponentials. Eight lanes take a token of up to 256 experts (32 lanes one of more), so that a warp works on four
 // at once and a reduction costs three shuffles for all of them (with a warp a token the reductions were most of the work). Sums over the
-// tokens are fp32 over at most a few hundred terms a warp, then fixed-order sums over warps and CTAs (double in the last
-// step), so that two runs give the same bits; counts are integers. Bound: HBM (logits in, gradient out) for large batches,
+// tokens are fp32 over short runs of a lane group (loss_run), then over its runs and over warps, then over CTAs (double), all in
+// fixed orders, so that two runs give the same bits; counts are integers. Bound: HBM (logits in, gradient out) for large batches,
 // launches for small ones: one CTA does the whole first pass of a small batch.
 #include <type_traits>
 
@@ -219,7 +219,7 @@ __device__ void finish_losses(const LossParts& w, int blocks, int E, const LossO
 template <bool kBf16, int kL, int kW, int kN>
 __global__ void __launch_bounds__(kOneWarps * 32)
 router_loss_kernel(const void* __restrict__ logits, const int* __restrict__ ids, const uint8_t* __restrict__ mask, int T, int E,
-                   int k, int alone, LossParts w, LossOut out) {
+                   int k, int run, int alone, LossParts w, LossOut out) {
   extern __shared__ float smem[];  // [warps][E] sums of p, then [E] counts
   __shared__ float s_z[kOneWarps];
   __shared__ int s_n[kOneWarps];
@@ -231,52 +231,62 @@ router_loss_kernel(const void* __restrict__ logits, const int* __restrict__ ids,
   int* s_counts = reinterpret_cast<int*>(smem + static_cast<size_t>(warps) * E);
   for (int e = t; e < E; e += blockDim.x) s_counts[e] = 0;
   __syncthreads();
-  float acc[kN];
-#pragma unroll
-  for (int i = 0; i < kN; ++i) acc[i] = 0.f;
-  float z = 0.f;
+  float z_all = 0.f;
   int n = 0;
   const int stride = gridDim.x * warps * kTokens;
-  for (int tok0 = (blockIdx.x * warps + warp) * kTokens; tok0 < T; tok0 += stride) {
-    const int tok = tok0 + lane / kL;
-    const bool live = tok < T && (mask == nullptr || mask[tok] != 0);
-    float x[kN];
+  int tok0 = (blockIdx.x * warps + warp) * kTokens;
+  bool first = true;
+  do {  // `run` tokens a lane group, then its sums join the warp's
+    float acc[kN];
 #pragma unroll
-    for (int i = 0; i < kN; ++i) x[i] = 0.f;
-    if (live) {
-      load_row<kBf16, kL, kW>(logits, static_cast<size_t>(tok) * E, E, l, x);
-      for (int j = l; j < k; j += kL) {
-        const int id = ids[static_cast<size_t>(tok) * k + j];
-        if (id >= 0 && id < E) atomicAdd(&s_counts[id], 1);
+    for (int i = 0; i < kN; ++i) acc[i] = 0.f;
+    float z = 0.f;
+    for (int turn = 0; turn < run && tok0 < T; ++turn, tok0 += stride) {
+      const int tok = tok0 + lane / kL;
+      const bool live = tok < T && (mask == nullptr || mask[tok] != 0);
+      float x[kN];
+#pragma unroll
+      for (int i = 0; i < kN; ++i) x[i] = 0.f;
+      if (live) {
+        load_row<kBf16, kL, kW>(logits, static_cast<size_t>(tok) * E, E, l, x);
+        for (int j = l; j < k; j += kL) {
+          const int id = ids[static_cast<size_t>(tok) * k + j];
+          if (id >= 0 && id < E) atomicAdd(&s_counts[id], 1);
+        }
+      }
+      float m, sum;
+      exp_row<kL>(x, m, sum);
+      sum = lanes_sum<kL>(sum);
+      if (live) {
+        const float inv = 1.f / sum, lse = m + logf(sum);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) acc[i] = fmaf(x[i], inv, acc[i]);
+        z = fmaf(lse, lse, z);
+        ++n;
       }
     }
-    float m, sum;
-    exp_row<kL>(x, m, sum);
-    sum = lanes_sum<kL>(sum);
-    if (live) {
-      const float inv = 1.f / sum, lse = m + logf(sum);
 #pragma unroll
-      for (int i = 0; i < kN; ++i) acc[i] = fmaf(x[i], inv, acc[i]);
-      z = fmaf(lse, lse, z);
-      ++n;
+    for (int s = 16; s >= kL; s >>= 1) {  // the tokens of the warp
+#pragma unroll
+      for (int i = 0; i < kN; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], s);
+      z += __shfl_xor_sync(0xffffffffu, z, s);
     }
-  }
+    z_all += z;
+    if (lane < kL) {
 #pragma unroll
-  for (int s = 16; s >= kL; s >>= 1) {  // the tokens of the warp
-#pragma unroll
-    for (int i = 0; i < kN; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], s);
-    z += __shfl_xor_sync(0xffffffffu, z, s);
-    n += __shfl_xor_sync(0xffffffffu, n, s);
-  }
-  if (lane < kL) {
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int e = expert_of<kL, kW>(i, l);
-      if (e < E) smem[static_cast<size_t>(warp) * E + e] = acc[i];
+      for (int i = 0; i < kN; ++i) {
+        const int e = expert_of<kL, kW>(i, l);
+        if (e >= E) continue;
+        float& row = smem[static_cast<size_t>(warp) * E + e];
+        row = first ? acc[i] : row + acc[i];
+      }
     }
-  }
+    first = false;
+  } while (tok0 < T);
+#pragma unroll
+  for (int s = 16; s >= kL; s >>= 1) n += __shfl_xor_sync(0xffffffffu, n, s);
   if (lane == 0) {
-    s_z[warp] = z;
+    s_z[warp] = z_all;
     s_n[warp] = n;
   }
   __syncthreads();
@@ -501,6 +511,16 @@ cudaError_t with_lanes(int E, bool vectors, F&& f) {
 
 bool on_16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// Tokens that a lane group adds up in a row before their sum joins the others', itself one addition of many: 64, or the root of
+// their number where that is more, so that neither chain is longer than max(64, root) + 1 additions (up to 4096 tokens a group, that
+// is 19 million tokens of many experts, a chain is off by at most 2^-17 in all; of 2^30 tokens 476 + 476 additions follow each other).
+int loss_run(int T, int E, int blocks, int warps) {
+  const long long at_once = static_cast<long long>(blocks) * warps * (32 / lanes_of(E)), turns = (T + at_once - 1) / at_once;
+  int run = 64;
+  while (static_cast<long long>(run) * run < turns) ++run;
+  return run;
+}
+
 // What the kernel holds in fixed arrays counts against the 48 KB that it may have without asking, too. It asks for the most that
 // any call needs, so that calls of two host threads ask for the same.
 constexpr size_t kLossFixedSmem = sizeof(FinishShared) + kOneWarps * (sizeof(float) + sizeof(int));
@@ -546,7 +566,8 @@ int launch_router_loss(float* losses, int* counts, int* num_tokens, float* mean_
     auto kernel = gating_is_bf16 ? router_loss_kernel<true, L, W, N> : router_loss_kernel<false, L, W, N>;
     const cudaError_t a = allow_loss_smem(kernel, smem);
     if (a != cudaSuccess) return a;
-    return launch_pdl(kernel, dim3(blocks), dim3(warps * 32), smem, stream, gating, topk_ids, token_mask, T, E, k, static_cast<int>(one_cta(T, E)), w, out);
+    return launch_pdl(kernel, dim3(blocks), dim3(warps * 32), smem, stream, gating, topk_ids, token_mask, T, E, k, loss_run(T, E, blocks, warps),
+                      static_cast<int>(one_cta(T, E)), w, out);
   });
   if (int st = check_cuda(e, "router_loss launch")) return st;
   if (!one_cta(T, E)) {

@@ -291,3 +291,22 @@ def test_shared_memory_just_below_48_kb_in_a_process_of_its_own(shapes):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", _FRESH.format(root=root, shapes=shapes)], capture_output=True, text=True, timeout=300, cwd=root)
     assert r.returncode == 0 and "OK" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("T,E", [(2**27, 8), (2**23, 260)])
+def test_long_batches_keep_their_precision(T, E):
+    """Millions of equal tokens: every addition rounds the same way, so that one chain of fp32 additions over all of a lane's tokens
+    (7085 and 1772 of them) is off by more than 2^-17. All tokens being equal, mean_probs is the softmax of one of them."""
+    from layered_prefill_b200 import ops
+    g = torch.Generator().manual_seed(E)
+    row = torch.randn(E, generator=g).to(torch.bfloat16).cuda()
+    logits = row.expand(T, E).contiguous()
+    ids = torch.full((T, 1), 3, dtype=torch.int32, device="cuda")
+    losses, mean = torch.empty(2, device="cuda"), torch.empty(E, device="cuda")
+    counts, n = torch.empty(E, dtype=torch.int32, device="cuda"), torch.empty(1, dtype=torch.int32, device="cuda")
+    ops.router_loss(losses, counts, n, mean, logits, ids)
+    p, lse = torch.softmax(row.double(), -1), torch.logsumexp(row.double(), -1)
+    assert int(n) == T and int(counts[3]) == T and int(counts.sum()) == T
+    assert ((mean.double() - p).abs() <= 2.0 ** -17 * p).all(), ((mean.double() - p).abs() / p).max()
+    want = torch.stack((E * p[3], lse.square()))
+    assert ((losses.double() - want).abs() <= 2.0 ** -17 * want).all(), (losses, want)
