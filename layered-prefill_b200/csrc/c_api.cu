@@ -24,6 +24,7 @@ int set_error(int status, const char* fmt, ...) {
 
 int check_cuda(cudaError_t e, const char* what) {
   if (e == cudaSuccess) return kStatusOk;
+  cudaGetLastError();  // reported here: the runtime would hand it to the next launch's check as well, this library's or another's
   return set_error(kStatusCudaError, "%s: %s", what, cudaGetErrorString(e));
 }
 

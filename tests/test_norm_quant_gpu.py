@@ -212,3 +212,20 @@ def test_refusals():
     off = torch.empty(4 * 256 + 8, dtype=torch.bfloat16, device="cuda")[1:1025].view(4, 256)  # two bytes off the boundary
     with pytest.raises(MoeB200Error):
         ops.rms_norm_quant_fp8(q, s, off, w, 1e-6)
+
+
+def test_an_error_of_one_call_is_not_reported_by_the_next():
+    """A refused allocation (64 TB) leaves the runtime's last error behind; the launches that follow are not to find it."""
+    from layered_prefill_b200 import ops
+    from layered_prefill_b200._lib import MoeB200Error
+    x, w = torch.randn(4, 256).to(torch.bfloat16).cuda(), torch.ones(256, dtype=torch.bfloat16, device="cuda")
+    out = torch.empty_like(x)
+    ops.rms_norm(out, x, w, 1e-6)
+    want = out.clone()
+    with pytest.raises(MoeB200Error):
+        ops.allocate_shared_buffer_and_handle(1 << 46)
+    ops.rms_norm(out.zero_(), x, w, 1e-6)
+    assert torch.equal(out, want)
+    with pytest.raises(MoeB200Error):
+        ops.allocate_shared_buffer_and_handle(1 << 46)
+    assert float((x + x).float().abs().sum()) > 0  # torch checks its launches the same way
