@@ -125,6 +125,11 @@ int check_block_shapes(int T, int E, int top_k, int H, int I) {
 
 bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
+bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  const uintptr_t u = reinterpret_cast<uintptr_t>(a), v = reinterpret_cast<uintptr_t>(b);
+  return u < v + b_bytes && v < u + a_bytes;
+}
+
 int check_w4_group(const char* what, int group_size, int K) {
   if (group_size != 32 && group_size != 64 && group_size != 128)
     return set_error(kStatusInvalidArgument, "%s: group_size must be 32, 64 or 128 (got %d)", what, group_size);
@@ -510,6 +515,10 @@ int moe_b200_router_backward(void* grad_logits, const void* gating, int gating_i
   if (T > 0 && (grad_logits == nullptr || gating == nullptr || (grad_topk_weights != nullptr && topk_ids == nullptr) ||
                 (grad_losses != nullptr && (counts == nullptr || num_tokens == nullptr))))
     return set_error(kStatusInvalidArgument, "router_backward: null pointer");
+  if (T > 0 && E > 0) {
+    const size_t bytes = static_cast<size_t>(T) * E * (gating_is_bf16 ? 2 : 4);
+    if (overlap(grad_logits, bytes, gating, bytes)) return set_error(kStatusInvalidArgument, "router_backward: grad_logits must not overlap gating");
+  }
   return launch_router_backward(grad_logits, gating, gating_is_bf16, topk_ids, counts, num_tokens, grad_losses,
                                 grad_topk_weights, token_mask, T, E, k, renormalize, static_cast<cudaStream_t>(stream));
 }
@@ -532,6 +541,8 @@ int moe_b200_w4_linear(void* out, const void* x, int64_t x_row_stride, const voi
   const size_t need = w4_linear_workspace_bytes(M, K, group_size);
   if (workspace != nullptr && (workspace_bytes < need || !aligned(workspace, 16)))
     return set_error(kStatusWorkspaceTooSmall, "w4_linear: workspace of %zu bytes on 16 needed, %zu given", need, workspace_bytes);
+  if (overlap(out, static_cast<size_t>(M) * N * 2, x, (static_cast<size_t>(M - 1) * x_row_stride + K) * 2))
+    return set_error(kStatusInvalidArgument, "w4_linear: out must not overlap x, which is still read when the first results are written");
   return launch_w4_linear(static_cast<__nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(x), x_row_stride,
                           w4_matrix(qweight, scale, zero, bias, group_size), M, N, K, workspace, static_cast<cudaStream_t>(stream));
 }
@@ -562,6 +573,9 @@ int moe_b200_fused_experts_w4(const void* x, const void* w13_q, const void* w13_
   const size_t need = moe_b200_fused_experts_w4_workspace_bytes(T, E, top_k, H, I);
   if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16))
     return set_error(kStatusWorkspaceTooSmall, "fused_experts_w4: workspace of %zu bytes on 16 needed, %zu given", need, workspace_bytes);
+  const size_t io_bytes = static_cast<size_t>(T) * H * 2;
+  if (out != x && overlap(out, io_bytes, x, io_bytes))
+    return set_error(kStatusInvalidArgument, "fused_experts_w4: out may be x, but not overlap it in part");
   return launch_w4_experts(static_cast<__nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(x),
                            w4_matrix(w13_q, w13_scale, w13_zero, w13_bias, group_size),
                            w4_matrix(w2_q, w2_scale, w2_zero, w2_bias, group_size), topk_weights, topk_ids, T, E, top_k, H, I,

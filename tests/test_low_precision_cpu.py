@@ -209,3 +209,22 @@ def test_w4_row_parallel_linear_has_a_bf16_bias_and_no_dense_weight(monkeypatch)
     assert linear.W4RowParallelLinear(256, 24, group_size=64).bias is None
     dense = linear.RowParallelLinear(256, 24, bias=True)  # as it was: both in the default type
     assert dense.weight.shape == (24, 256) and dense.weight.dtype == dense.bias.dtype == torch.float32
+
+
+def test_outputs_over_inputs_are_refused():
+    """Inputs are read while outputs are written: a result over its input would depend on which block comes first."""
+    lib, err = _lib()
+    far = P + (1 << 20)  # never dereferenced either
+
+    def linear(out, x, M, ld, N=128, K=128):
+        return lib.moe_b200_w4_linear(out, x, ld, P, P, None, None, M, N, K, 64, None, 0, None)
+
+    for out, x, M, ld in ((far, far, 1, 128), (far, far, 4, 128), (far + 3 * 256, far, 4, 128), (far, far + 4 * 256 - 16, 4, 128),
+                          (far + 256, far, 2, 512)):
+        assert linear(out, x, M, ld) == 1 and "overlap" in err(), (out - far, x - far, M, ld)
+    for x, grad, bf16 in ((far, far, 0), (far + 4 * 64 - 4, far, 0), (far, far + 4 * 32 - 2, 1)):
+        assert lib.moe_b200_router_backward(grad, x, bf16, P, P, P, P, P, None, 4, 16, 2, 1, None) == 1 and "overlap" in err()
+    need = lib.moe_b200_fused_experts_w4_workspace_bytes(4, 8, 2, 256, 128)
+    for out in (far + 512, far - 512, far + 8):
+        assert lib.moe_b200_fused_experts_w4(far, P, P, None, None, P, P, None, None, P, P, out, 4, 8, 2, 256, 128, 64, 0, P, need,
+                                             None) == 1 and "overlap" in err()
