@@ -249,8 +249,11 @@ int moe_b200_router_backward(void* grad_logits, const void* gating, int gating_i
  *   out bf16 [M, N] = x @ W^T + bias;  x bf16, rows x_row_stride elements apart (a multiple of 8)
  * group_size 32, 64 or 128 and K % group_size == 0, K <= 2^24; any N. qweight and x on 16 bytes.
  * x enters as 16-bit integers times a power of two for every token and 128 columns: exact down to 2^-7 of the largest of
- * them, off by at most 2^-15 of it below. Integer products, fp32 sums, one rounding of the output. A value that is not finite
- * makes its token's row NaN. out must not overlap x. workspace: room for those integers where a kernel in front makes them
+ * them, off by at most 2^-15 of it below. Where a few columns stand out so far that this would show in rows without a weight
+ * for them (sum of min(|x|, 2^10 steps)^2 below 2^24 steps^2, a step being 2^-14 of the power of two at or below the largest),
+ * 16 bits more are taken and x is off by at most 2^-29 of the largest; such columns cost two to five times the others.
+ * Integer products, fp32 sums, one rounding of the output. A value that is not finite makes its token's row NaN. out must
+ * not overlap x. workspace: room for those integers where a kernel in front makes them
  * once; without it (NULL) every CTA makes those that it needs, with the same bits.
  */
 size_t moe_b200_w4_linear_workspace_bytes(int M, int K, int group_size); /* 0: none needed */
@@ -261,8 +264,8 @@ int moe_b200_w4_linear(void* out, const void* x, int64_t x_row_stride, const voi
  * fused_experts with such weights: w13 codes [E, 2*I, H/2] (gate rows then up rows, interleaved for
  * MOE_B200_ACT_SWIGLUOAI), w2 codes [E, H, I/2], scales [E, 2*I, H/g] and [E, H, I/g], zeros alike or NULL, biases bf16
  * [E, 2*I] and [E, H] or NULL. H % group_size == 0, I % group_size == 0. Slots whose id is outside [0, E) add
- * nothing. The intermediate enters the second product as x does the first (off by at most 2^-15 of the largest of 128
- * columns), the slots' results are fp32. out may be x, but not overlap it in part. E <= 1024, top_k <= 1024, I * H < 2^32.
+ * nothing. The intermediate, which is fp32, enters the second product as x does the first (off by at most 2^-15 of the
+ * largest of 128 columns, or 2^-29 where a few stand out), the slots' results are fp32. out may be x, but not overlap it in part. E <= 1024, top_k <= 1024, I * H < 2^32.
  */
 size_t moe_b200_fused_experts_w4_workspace_bytes(int T, int E, int top_k, int H, int I);
 int moe_b200_fused_experts_w4(const void* x, const void* w13_q, const void* w13_scale, const void* w13_zero,

@@ -13,7 +13,9 @@
 //   The activations become 16-bit integers with a power of two f for every token and 128 columns:
 //   x = f * (256 hi + lo), hi signed and lo unsigned bytes, two products a word; f puts the largest |x| of them between 2^14 and 2^15.
 //   A bf16 value has 8 significant bits, so that all down to 2^-7 of the largest are exact and smaller ones are off by at most
-//   2^-15 of the largest; the intermediate h of the experts (fp32) is off by that everywhere. Integer sums are exact; then
+//   2^-15 of the largest; the intermediate h of the experts (fp32) is off by that everywhere. Where a few columns stand out so far that this
+//   would show in rows which have no weight for them (see kMarkBelow), what is cut off is added as 16 bits more: off by 2^-29 of the
+//   largest then. Integer sums are exact; then
 //   sum (code - zero) x = f * (256 sum code hi + sum code lo - zero * sum x) in fp32, times the group's scale, summed in fp32.
 //   Where a value is not finite f is NaN, so that its token's results are NaN.
 //   A CTA makes these integers itself where they are few; where many CTAs would make many of them (a batch, a long K) a kernel in
@@ -95,6 +97,17 @@ __device__ __forceinline__ void mma_codes(int (&d)[4], const uint32_t (&a)[4], u
     asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+}
+
+// The same of signed bytes (what the zero point has left already).
+template <bool kSigned>
+__device__ __forceinline__ void mma_weights(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (kSigned)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 constexpr int kFloatBits = 0x4b400000;    // bits of 12582912.f, one more for every unit up to 2^22
@@ -231,8 +244,35 @@ __device__ __forceinline__ int col_of(int j, int t) {
   return kGpc == 1 ? 32 * t + 8 * j : (kGpc == 2 ? 64 * (j >> 1) + 16 * t + 8 * (j & 1) : 32 * j + 8 * t);
 }
 
+// v: integers in their low 16 bits. Bytes 1 (high) of columns 0, 2, 4, 6 and of 1, 3, 5, 7, then bytes 0.
+__device__ __forceinline__ uint4 pack_ints(const uint32_t (&v)[8]) {
+  uint32_t o[4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t a02 = __byte_perm(v[h], v[2 + h], 0x5410), a46 = __byte_perm(v[4 + h], v[6 + h], 0x5410);
+    o[h] = __byte_perm(a02, a46, 0x7531);
+    o[2 + h] = __byte_perm(a02, a46, 0x6420);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// The float whose low 16 bits are x / f rounded to nearest. An fp32 value may lie past 32767.5, a bf16 one does not.
+template <bool kFp32>
+__device__ __forceinline__ float int_of(float x, float to_int) {
+  return kFp32 ? fminf(x * to_int, 32767.f) + kFloatBias : fmaf(x, to_int, kFloatBias);
+}
+
+// A chunk of a token whose integers cut off too much of it is marked in the last bit of its f (which moves its products by 2^-23, no more
+// than one of the additions that follow), and what they cut off is added behind the loop. An integer is off by at most 1/2, all 128 together by at most 5.7 and as a rule by 3.3 (their norm).
+// With every magnitude counted as 1024 at most (2^-4 to 2^-5 of the largest), a chunk below kMarkBelow, that is of a norm
+// below 4096, is marked: in the others the columns left next to any eight have a norm of 2896, so that what is cut off stays
+// below 2^-9 of them, a rounding of the output, also in rows whose weights for those eight are zero. Of normally distributed values none
+// are marked, of those with a column of 100 times the rest all.
+constexpr float kMarkCap = 1024.f, kMarkBelow = 16.f * kMarkCap * kMarkCap;
+constexpr uint32_t kMark = 1;
+
 // The integers of 128 columns of a token by sixteen neighbouring lanes, lane u holding the eight columns from col_of(u / 4, u % 4) on.
-// ints: bytes 1 (high) of columns 0, 2, 4, 6 and of 1, 3, 5, 7, then bytes 0; sum: of its group; returns f.
+// ints: see pack_ints; sum: of its group; returns f, marked or not.
 template <int kGpc, bool kFp32>
 __device__ __forceinline__ float quant_x(const float (&x)[8], uint4& ints, int& sum) {
   uint32_t big = 0;  // the largest magnitude as bits, which order like the values, NaN last
@@ -245,26 +285,28 @@ __device__ __forceinline__ float quant_x(const float (&x)[8], uint4& ints, int& 
   const float to_int = __uint_as_float(static_cast<uint32_t>(254 + 14 - e) << 23);  // 2^(14 - exponent)
   uint32_t v[8];
   sum = 0;
+  float norm = 0.f;  // its square
+  bool cut = false;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    // the integer in the low bits, rounded to nearest; an fp32 value may lie past 32767.5, a bf16 one does not
-    v[k] = __float_as_uint(kFp32 ? fminf(x[k] * to_int, 32767.f) + kFloatBias : fmaf(x[k], to_int, kFloatBias));
+    const float i = int_of<kFp32>(x[k], to_int), scaled = x[k] * to_int;
+    v[k] = __float_as_uint(i);
     sum += static_cast<int>(v[k]) - kFloatBits;
+    const float m = fminf(fabsf(scaled), kMarkCap);
+    norm = fmaf(m, m, norm);
+    cut |= i - kFloatBias != scaled;
   }
-  uint32_t o[4];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t a02 = __byte_perm(v[h], v[2 + h], 0x5410), a46 = __byte_perm(v[4 + h], v[6 + h], 0x5410);
-    o[h] = __byte_perm(a02, a46, 0x7531);
-    o[2 + h] = __byte_perm(a02, a46, 0x6420);
-  }
-  ints = make_uint4(o[0], o[1], o[2], o[3]);
+  ints = pack_ints(v);
   if (!finite) sum = 0;
   sum += __shfl_xor_sync(0xffffffffu, sum, 1);
   sum += __shfl_xor_sync(0xffffffffu, sum, 2);
   if (kGpc < 4) sum += __shfl_xor_sync(0xffffffffu, sum, 4);
   if (kGpc < 2) sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-  return finite ? __uint_as_float(static_cast<uint32_t>(e - 14) << 23) : __uint_as_float(0x7fffffffu);
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) norm += __shfl_xor_sync(0xffffffffu, norm, m);
+  const uint32_t cuts = __ballot_sync(0xffffffffu, cut) >> (threadIdx.x & 16) & 0xffffu;
+  if (!finite) return __uint_as_float(0x7fc00000u);
+  return __uint_as_float(static_cast<uint32_t>(e - 14) << 23 | (norm < kMarkBelow && cuts != 0 ? kMark : 0));
 }
 
 __device__ __forceinline__ void load_x8(const __nv_bfloat16* src, float (&x)[8]) {
@@ -464,13 +506,15 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   };
 
   // ------------------------------------------------------------------ activations of entries and a span of columns
-  auto load_x = [&](int base, int n, int span_i) {
+  using X = std::conditional_t<kMode == kDown, float, __nv_bfloat16>;
+  auto source_row = [&](int entry) -> long long {
+    if (kMode == kDense) return entry;
+    return kMode == kGateUp ? lists.slots[entry] / p.top_k : lists.slots[entry];
+  };
+  auto load_x = [&](int base, int n, int span_i) -> bool {  // whether this thread has met a marked chunk
     const int c0 = span_i * p.span;
     const int chunks = (min(p.span, p.K - c0) + kChunk - 1) / kChunk;
-    auto source_row = [&](int row) -> long long {
-      if (kMode == kDense) return base + row;
-      return kMode == kGateUp ? lists.slots[base + row] / p.top_k : lists.slots[base + row];
-    };
+    uint32_t marks = 0;
     // half a warp takes a chunk of a token
     int row = 0, c = warp * 2 + (lane >> 4);
     const int u = lane & 15;
@@ -489,11 +533,12 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
             ++row;
           }
           const int r = min(row, n - 1);  // behind the last chunk: one of the last token again
-          const long long src = source_row(r) * all + c0 / kChunk + c;
+          const long long src = source_row(base + r) * all + c0 / kChunk + c;
           v[i] = *reinterpret_cast<const uint4*>(p.xq + src * 256 + u * 16);
           s[i] = u <= kGpc ? p.xm[src * (kGpc + 1) + u] : 0.f;
           to[i] = r * x_ld + c * 256 + u * 16;
           to_s[i] = r * xs_ld + c * (kGpc + 1) + u;
+          if (u == kGpc) marks |= __float_as_uint(s[i]);
           c += 2 * kWarps;
         }
 #pragma unroll
@@ -502,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
           if (u <= kGpc) x_sum[to_s[i]] = s[i];
         }
       }
-      return;
+      return (marks & kMark) != 0;
     }
     for (int at = warp * 2; at < n * chunks; at += 2 * kWarps) {
       while (c >= chunks) {
@@ -512,8 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
       const int r = min(row, n - 1);
       const int col = c0 + c * kChunk + col_of<kGpc>(u >> 2, u & 3);
       float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      using X = std::conditional_t<kMode == kDown, float, __nv_bfloat16>;
-      if (col < p.K) load_x8(static_cast<const X*>(p.x) + source_row(r) * p.x_ld + col, v);
+      if (col < p.K) load_x8(static_cast<const X*>(p.x) + source_row(base + r) * p.x_ld + col, v);
       uint4 ints;
       int sum;
       const float f = quant_x<kGpc, kMode == kDown>(v, ints, sum);
@@ -521,8 +565,10 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
       constexpr int kUnits = 16 / kGpc;
       if (u % kUnits == 0) x_sum[r * xs_ld + c * (kGpc + 1) + u / kUnits] = static_cast<float>(sum);
       if (u == 0) x_sum[r * xs_ld + c * (kGpc + 1) + kGpc] = f;
+      marks |= __float_as_uint(f);
       c += 2 * kWarps;
     }
+    return (marks & kMark) != 0;
   };
 
   // ------------------------------------------------------------------ scales and zero points of this lane's rows
@@ -594,6 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
   // ------------------------------------------------------------------ products
   const int start[4] = {kFloatBits, kFloatBits, kFloatBits, kFloatBits};
   const uint32_t fifo_lane = smem_u32(fifo) + g * 64;
+  int marked = 0;  // whether a chunk of the activations in shared memory is
   for (int block0 = first_block; block0 <= last_block;) {
     const int block1 = window_end(block0);
     Place at{first, first_block, first - first_block * p.row_tiles};
@@ -634,8 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
       for (int span_i = 0; span_i < spans; ++span_i) {
         if (spans > 1 || round == 0) {
           __syncthreads();  // the last readers of the previous activations are done
-          load_x(win_base, win_n, span_i);
-          __syncthreads();
+          marked = __syncthreads_or(load_x(win_base, win_n, span_i));
         }
         if (!active) continue;
         int begin, left;
@@ -775,6 +821,75 @@ __global__ void __launch_bounds__(kThreads, 1) w4_mma_kernel(const W4Params p) {
           for (int i = 0; i < 2 * kRB; ++i) s_src[i] += kStages * kGpc;
           z_src += kStages * kGpc;
           gi += kStages * kGpc;
+        }
+        // What the integers of marked chunks cut off: once more through these chunks, with (x / f - integer) * 2^15 as integers against
+        // code - zero. Behind the loop and in as few registers as it can be, because the loop above has none to spare; codes and
+        // activations come from the second level cache. A marked chunk costs as much as two to five others: 64 tokens over 128
+        // experts, H = 2048, I = 768: 85 us without one, 114 us with two of the 16 chunks of every token, 290 us with all.
+        if (__builtin_expect(marked, 0)) {
+          int entry0, tokens, window0, unused, chunks;  // found anew rather than kept over the loop
+          entries_of(block, entry0, tokens);
+          entries_of(block0, window0, unused);
+          chunks_of(span_i, begin, chunks);
+          const long long first = first_row_of_matrix(block) + first_row(here.r) * step_row + row_lo;
+          const float* const f_at = x_sum + (entry0 - window0) * xs_ld + kGpc;
+#pragma unroll 1
+          for (int c = begin; c < begin + chunks; ++c) {
+#pragma unroll
+            for (int tb = 0; tb < kTB; ++tb) {
+              const int mine = min(tb * 8 + g, tokens - 1);  // token whose activations this lane brings
+              const uint32_t f_mine = __float_as_uint(f_at[mine * xs_ld + c * (kGpc + 1)]);
+              if (!__any_sync(0xffffffffu, f_mine & kMark)) continue;
+              const float to_int = __uint_as_float((254u << 23) - (f_mine & ~kMark));
+              const int c0 = span_i * p.span + c * kChunk;
+              const X* const x_at = static_cast<const X*>(p.x) + source_row(entry0 + mine) * p.x_ld;
+#pragma unroll 1
+              for (int q = 0; q < kGpc; ++q) {
+                const int group = c0 / (kChunk / kGpc) + q;
+                if (group >= groups) continue;
+                int high[kRB][4] = {}, low[kRB][4] = {};
+#pragma unroll 1
+                for (int j = q * (4 / kGpc); j < (q + 1) * (4 / kGpc); ++j) {
+                  const int col = c0 + col_of<kGpc>(j, t);
+                  const bool in = col < p.K;
+                  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                  if (in && (f_mine & kMark)) load_x8(x_at + col, x);
+                  uint32_t v[8];
+#pragma unroll
+                  for (int k = 0; k < 8; ++k) {
+                    const float cut = x[k] * to_int - (int_of<kMode == kDown>(x[k], to_int) - kFloatBias);  // exact, -1/2 to 1
+                    v[k] = __float_as_uint(fminf(cut * 32768.f, 32767.f) + kFloatBias);
+                  }
+                  const uint4 b = pack_ints(v);
+#pragma unroll
+                  for (int rb = 0; rb < kRB; ++rb) {
+                    uint32_t w[2], z[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                      w[h] = in ? *reinterpret_cast<const uint32_t*>(p.w.q + first * row_bytes + (col >> 1) + q_off[2 * rb + h]) : 0u;
+                      z[h] = (kZero ? p.w.zero[first * groups + group + s_off[2 * rb + h]] & 15u : 8u) * 0x01010101u;
+                    }
+                    const uint32_t a[4] = {__vsub4(w[0] & 0x0f0f0f0fu, z[0]), __vsub4(w[1] & 0x0f0f0f0fu, z[1]),
+                                           __vsub4((w[0] >> 4) & 0x0f0f0f0fu, z[0]), __vsub4((w[1] >> 4) & 0x0f0f0f0fu, z[1])};
+                    mma_weights<true>(high[rb], a, b.x, b.y);
+                    mma_weights<false>(low[rb], a, b.z, b.w);
+                  }
+                }
+#pragma unroll
+                for (int o = 0; o < 2; ++o) {
+                  const uint32_t f = __float_as_uint(f_at[min(tb * 8 + 2 * t + o, tokens - 1) * xs_ld + c * (kGpc + 1)]);
+                  const float unit = __uint_as_float(f & ~kMark) * 0x1p-15f;
+#pragma unroll
+                  for (int i = 0; i < 2 * kRB; ++i) {
+                    const float s = __bfloat162float(p.w.scale[first * groups + group + s_off[i]]);
+                    const int r = 2 * (i & 1) + o;
+                    float& sum = tot[i >> 1][tb][r];
+                    sum = fmaf(unit * s, static_cast<float>(high[i >> 1][r] * 256 + low[i >> 1][r]), sum);
+                  }
+                }
+              }
+            }
+          }
         }
       }
 

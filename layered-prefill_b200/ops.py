@@ -193,8 +193,10 @@ def w4_linear(out: torch.Tensor, input: torch.Tensor, qweight: torch.Tensor, sca
     """out[.., N] = input[.., K] @ W^T + bias for 4-bit weights W[n, k] = (code - zero) * scale, built for few tokens (any number
     works). qweight uint8 [N, K / 2], two codes a byte, the low nibble is the even k; scales bf16 [N, K / group], groups of 32, 64 or
     128; zeros uint8 0..15 like scales (8 without it); bias bf16 [N]. A two-dimensional input may have rows further than K apart
-    (a multiple of 8 elements); out must not share memory with it. The activations enter the products as 16-bit integers times a power of two for every 128 columns (exact
-    down to 2^-7 of their largest, off by at most 2^-15 of it below); sums are fp32. `fused_moe.quant_w4` makes such weights."""
+    (a multiple of 8 elements); out must not share memory with it. The activations enter the products as 16-bit integers times a
+    power of two for every 128 columns: exact down to 2^-7 of their largest, off by at most 2^-15 of it below; where a few columns stand
+    out so far that this would show in rows without a weight for them (one of 100 times the rest, say), 16 bits more are taken. Sums
+    are fp32. `fused_moe.quant_w4` makes such weights."""
     shape, q_shape, s_shape = input.shape, qweight.shape, scales.shape
     if len(q_shape) != 2 or len(s_shape) != 2 or not shape or not shape[-1] or not q_shape[0] or not s_shape[1]:
         raise RuntimeError("w4_linear: qweight must be [N, K / 2], scales [N, K / group] and input [.., K]")

@@ -510,3 +510,100 @@ def test_row_parallel_linear_with_a_bias_under_the_default_type(M):
     want = torch.empty_like(y)
     ops.add_rms_norm(want, residual, y, norm_w, 1e-6)
     assert torch.equal(normed, want) and torch.equal(res, residual)
+
+
+# ------------------------------------------------------------------------- small values next to large ones
+# Where the integers would cut off too much of 128 columns (the sum of min(|x| / f, 1024)^2 is below 2^24, f being the step, 2^-14 of the power
+# of two at or below the largest) what they cut off is added as further integers in steps of 2^-15 f: off by half of one, or by a whole one where the
+# largest rounds up, so by at most 2^-15 f <= 2^-29 of the largest. The step of such columns carries a mark in its last bit, which moves
+# their products by 2^-23, as one more of the 64 further additions does.
+def _cut(x, unmarked):
+    """What x [.., K] may be off by: 2^-29 of the largest in marked columns, unmarked(x) in the others."""
+    K = x.size(-1)
+    v = torch.nn.functional.pad(x.double(), (0, -K % 128)).unflatten(-1, (-1, 128))
+    big = v.abs().amax(-1, keepdim=True)
+    f = torch.where(big > 0, torch.exp2(torch.floor(torch.log2(big.clamp(min=2.0 ** -120))) - 14), torch.ones_like(big))
+    few = ((v / f).abs().clamp(max=1024).square().sum(-1, keepdim=True) < 2.0 ** 24).expand_as(v).flatten(-2)[..., :K]
+    return torch.where(few, 2.0 ** -29 * big.expand_as(v).flatten(-2)[..., :K], unmarked(x.double()))
+
+
+def _ignoring(packed, zp, group, columns):
+    """The codes with those of some columns equal to their zero points."""
+    code = torch.stack((packed & 15, packed >> 4), -1).flatten(-2)
+    z = torch.full_like(code, 8) if zp is None else zp.repeat_interleave(group, -1)
+    code[..., columns] = z[..., columns]
+    return code[..., 0::2] | (code[..., 1::2] << 4)
+
+
+@pytest.mark.parametrize("factor", [100.0, 3000.0, 1e6])
+@pytest.mark.parametrize("M,N,K,group,zeros", [(1, 64, 2048, 128, False), (3, 70, 640, 32, True), (8, 33, 1024, 64, True), (16, 128, 2048, 128, True),
+                                               (20, 64, 8192, 64, False), (7, 2400, 2048, 32, False), (16, 100, 16384, 64, True),
+                                               (5, 17, 96, 32, True), (40, 4096, 512, 128, False)])
+def test_small_values_next_to_large_ones_that_a_row_ignores(M, N, K, group, zeros, factor):
+    """A few columns far larger than the rest; half of the rows have no weight for them."""
+    g = torch.Generator().manual_seed(M + N + K)
+    packed, scale, zp = _weights(N, K, group, zeros, g)
+    large = torch.arange(5, K, 64)
+    packed[: N // 2] = _ignoring(packed[: N // 2].clone(), None if zp is None else zp[: N // 2], group, large.cuda())
+    x = torch.randn(M, K, generator=g)
+    x[:, large] = factor * (1 + torch.rand(M, large.numel(), generator=g))
+    x = x.to(torch.bfloat16).cuda()
+    out = _linear(x, packed, scale, zp)
+    w, xd = _dense64(packed, scale, zp, group), x.double()
+    y = xd @ w.t()
+    bound = 1.01 * BF16 * y.abs() + _cut(x, _bf16_off) @ w.abs().t() + _gamma(K) * (xd.abs() @ w.abs().t())
+    err = (out.double() - y).abs()
+    assert (err <= bound).all(), (err / bound).max()
+
+
+@pytest.mark.parametrize("T,act,zeros", [(1, "silu", True), (6, "silu", False), (21, "swigluoai", True)])
+def test_small_intermediates_next_to_large_ones_that_a_row_ignores(T, act, zeros):
+    """The same in both products of the experts: hidden states and the activations between, which are fp32."""
+    g = torch.Generator().manual_seed(T)
+    H, I, group = 512, 256, 64
+    w13, w2 = _weights(2 * I, H, group, zeros, g, (1,)), _weights(H, I, group, zeros, g, (1,))
+    large_x, large_h = torch.arange(7, H, 128).cuda(), torch.arange(3, I, 128).cuda()
+    keep = w13[0].clone()
+    w13 = (_ignoring(w13[0].clone(), w13[2], group, large_x), w13[1], w13[2])
+    for i in large_h.tolist():  # these columns between the products do see the large hidden states: they come out large
+        rows = [i, I + i] if act == "silu" else [2 * i + 1]
+        w13[0][:, rows] = keep[:, rows]
+    w2 = (_ignoring(w2[0].clone(), w2[2], group, large_h), w2[1], w2[2])
+    x = torch.randn(T, H, generator=g)
+    x[:, large_x.cpu()] = 2000.0
+    x = x.to(torch.bfloat16).cuda()
+    tw, ti = torch.ones(T, 1, device="cuda"), torch.zeros(T, 1, dtype=torch.int32, device="cuda")
+    out = _experts(x, w13, w2, tw, ti, group, activation=act)
+    a, b, xd = _dense64(*(t if t is None else t[0] for t in w13), group), _dense64(*(t if t is None else t[0] for t in w2), group), x.double()
+    gu, dgu = xd @ a.t(), _cut(x, _bf16_off) @ a.abs().t() + _gamma(H) * (xd.abs() @ a.abs().t())
+    cut = (lambda v: (v[:, :I], v[:, I:])) if act == "silu" else (lambda v: (v[:, 0::2], v[:, 1::2]))
+    (gate, up), (dg, du) = cut(gu), cut(dgu)
+    h = _act64(gate, up, act)
+    dh = 1.2 * (up.abs() + 1) * dg + gate.abs() * du + 2.0 ** -20 * gate.abs() * (up.abs() + 1)
+    y = h @ b.t()
+    bound = 1.01 * BF16 * y.abs() + (dh + _cut(h, _step)) @ b.abs().t() + _gamma(I) * (h.abs() @ b.abs().t())
+    err = (out.double() - y).abs()
+    assert (err <= bound).all(), (err / bound).max()
+
+
+def test_marked_activations_prepared_in_front_or_by_each_block_give_the_same_bits():
+    from layered_prefill_b200 import ops
+    from layered_prefill_b200._lib import lib
+    g = torch.Generator().manual_seed(5)
+    M, N, K, group = 13, 200, 2048, 64
+    packed, scale, zp = _weights(N, K, group, True, g)
+    x = torch.randn(M, K, generator=g)
+    x[:, 9::200] = 900.0
+    x[4] = torch.randn(K, generator=g)  # a token without large columns between those with
+    x = x.to(torch.bfloat16).cuda()
+    with_room = _linear(x, packed, scale, zp)
+    assert lib.moe_b200_w4_linear_workspace_bytes(M, K, group) > 0
+    out = torch.empty_like(with_room)
+    ops._launch(lib.moe_b200_w4_linear, out.device, out.data_ptr(), x.data_ptr(), K, packed.data_ptr(), scale.data_ptr(), zp.data_ptr(), 0, M, N,
+                K, group, 0, 0)
+    assert torch.equal(out, with_room)
+    bad = x.clone()
+    bad[2, 9], bad[5, 0], bad[7, 700] = float("inf"), float("nan"), float("-inf")
+    out = _linear(bad, packed, scale, zp)
+    rest = [i for i in range(M) if i not in (2, 5, 7)]
+    assert out[[2, 5, 7]].isnan().all() and torch.equal(out[rest], with_room[rest])
