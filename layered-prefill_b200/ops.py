@@ -115,6 +115,10 @@ _raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(device).cuda_
 
 
 _MAX_ROWS = 2**30 - 1  # tokens of a call: their number crosses the C interface as an int
+# Below these the library asks for no workspace, and asking it is saved; its own numbers are kOneCta, kOneCtaLogits (router_loss.cu)
+# and kPreparedChunks (w4_gemv.cu), and a test compares the two.
+_LOSS_ALONE_TOKENS, _LOSS_ALONE_LOGITS = 128, 16384
+_W4_SMALL = 8192
 
 
 def _launch(fn, device: torch.device, *args) -> None:
@@ -211,7 +215,7 @@ def w4_linear(out: torch.Tensor, input: torch.Tensor, qweight: torch.Tensor, sca
            (qweight, u8, (N, K // 2)), (scales, bf16, (N, groups)), (zeros, u8, (N, groups)), (bias, bf16, (N,)))
     group = K // groups if K % groups == 0 else -1
     ws, nbytes = None, 0
-    if M * (K + 127) > 8192:  # below, no room is ever asked for
+    if M * (K + 127) > _W4_SMALL:
         nbytes = lib.moe_b200_w4_linear_workspace_bytes(M, K, group)
         ws = torch.empty(nbytes, dtype=u8, device=device) if nbytes else None
     _launch(lib.moe_b200_w4_linear, device, out.data_ptr(), input.data_ptr(), ld, qweight.data_ptr(), scales.data_ptr(),
@@ -245,7 +249,7 @@ def router_loss(losses: torch.Tensor, counts: torch.Tensor, num_tokens: torch.Te
            (losses, torch.float32, (2,)), (counts, torch.int32, (E,)), (num_tokens, torch.int32, (1,)),
            (mean_probs, torch.float32, (E,)))
     ws, nbytes = None, 0
-    if T > 128 or T * E > 16384:  # below, one CTA does it without
+    if T > _LOSS_ALONE_TOKENS or T * E > _LOSS_ALONE_LOGITS:
         nbytes = lib.moe_b200_router_loss_workspace_bytes(T, E)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _launch(lib.moe_b200_router_loss, dev, losses.data_ptr(), counts.data_ptr(), num_tokens.data_ptr(), mean_probs.data_ptr(),

@@ -228,3 +228,18 @@ def test_outputs_over_inputs_are_refused():
     for out in (far + 512, far - 512, far + 8):
         assert lib.moe_b200_fused_experts_w4(far, P, P, None, None, P, P, None, None, P, P, out, 4, 8, 2, 256, 128, 64, 0, P, need,
                                              None) == 1 and "overlap" in err()
+
+
+def test_where_the_library_asks_for_no_workspace():
+    """ops.py does not ask the library below these sizes: nothing may be needed there, and the losses' rule is exact."""
+    from layered_prefill_b200 import ops
+    lib, _ = _lib()
+    for T in (0, 1, 2, 63, 127, 128, 129, 200, 5000):
+        for E in (1, 8, 100, 127, 128, 129, 160, 256, 1023, 1024):
+            room = lib.moe_b200_router_loss_workspace_bytes(T, E) > 0
+            assert room == (T > ops._LOSS_ALONE_TOKENS or T * E > ops._LOSS_ALONE_LOGITS), (T, E)
+    for group in (32, 64, 128):
+        for K in (group, 128, 256, 384, 1024, 2048, 4096, 7936, 8064, 8192, 16384):
+            for M in range(1, 66):
+                if M * (K + 127) <= ops._W4_SMALL:
+                    assert lib.moe_b200_w4_linear_workspace_bytes(M, K, group) == 0, (M, K, group)
