@@ -3,6 +3,11 @@
 // and then block in grid_dependency_wait() until that kernel's results are complete and visible.
 // Every kernel launched this way calls grid_dependency_wait() before it reads or writes anything another
 // kernel touches, so "previous kernel finished" stays transitive along the stream.
+// One exception: w4_mma_kernel (w4_gemv.cu), as the down pass or behind quant_x_kernel, reads topk_ids and the codes before
+// its wait. That is sound because the kernel in front of it, always one of the same call, lets it start only after its own wait
+// (grid_dependency_launch() behind grid_dependency_wait() in every CTA): whatever wrote the ids and the codes has finished by
+// then. What the kernel in front itself writes is read behind the wait. A kernel that lets its successor start first, as most
+// here do, may not stand in front of one that reads early.
 // MOE_B200_PDL=0 in the environment switches back to plain stream-ordered launches (debugging aid).
 #pragma once
 

@@ -27,9 +27,13 @@
 // order in which the codes come, next to their group sums. A worker is 1 to 16 warps that split a tile's columns. Every warp
 // streams codes through a FIFO of its own (16-byte cp.async, four 128-column steps deep) that runs on into the next tile, so
 // no warp waits for another inside a window. What bounds it now: the instructions of a step (about 200 for 32 rows, at two a cycle
-// and SM) and of a tile's end; the same loop without products reads at 5.2 to 5.7 TB/s, with them at 4.1 to 4.6.
+// and SM, and the latency of its chain of codes, products and sums) and of a tile's end; the same loop without products reads at 5.2 to
+// 5.7 TB/s, the cases below at 3.6 to 3.9. The sixteen warps and their rings leave 128 registers a thread, and two row blocks do not
+// quite fit them: ptxas spills 44 to 100 bytes a thread there without zero points, 52 to 336 with them, 152 to 668 with two
+// token blocks as well; one row block spills 0 to 48.
 // Measured (graph replay): 64 tokens over 128 experts, H = 2048, I = 768: 84 us, 3.7 TB/s, against 205 us of the bf16 experts;
-// 93 tokens, H = 4096, I = 1536, groups of 64: 335 us, 3.9 TB/s; N = 131075, K = 2048, groups of 32, five tokens: 40 us, 3.8 TB/s.
+// 93 tokens, H = 4096, I = 1536, groups of 64: 335 us, 3.9 TB/s, as long as the card stays below its power limit, 368 us at 1.7 GHz
+// when it has run into it (after 0.07 s of nothing else); N = 131075, K = 2048, groups of 32, five tokens: 42 us, 3.7 TB/s.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -992,7 +996,11 @@ int expected_blocks(int slots, int E) {
 // How a launch is split, and a guess of its time in cycles; the shape with the least is taken. What it weighs: a chunk of a
 // warp takes about 850 cycles for 16 rows with all warps at work (1450 for 32), more with small groups and two token blocks, a
 // tile's end 2200, a window is a whole number of rounds and, where others follow, waits for its slowest worker, and activations
-// come at 64 bytes a cycle behind a latency of 1500.
+// come at 64 bytes a cycle behind a latency of 1500. It does not know what a shape spills and is off by tens of percent where shapes
+// lie close. Measured with the row blocks forced (calls, us; what is taken first): N = 131075, K = 2048, groups of 32, M = 5 two 42.0, one
+// 46.3; 64 tokens over 128 experts (H = 2048, I = 768) two 85.2, one 83; 93 tokens (H = 4096, I = 1536, groups of 64 with zero points) one in
+// gate_up and two in down 357, two in both 375, one in both 356; M = 16, N = 4096, K = 8192, groups of 64 with zero points two
+// 22.1, one 17.1: there it takes the slower.
 struct W4Split {
   int span, cap, wk_log2, ctas;
   double cost;
