@@ -266,12 +266,12 @@ __device__ __forceinline__ float int_of(float x, float to_int) {
   return kFp32 ? fminf(x * to_int, 32767.f) + kFloatBias : fmaf(x, to_int, kFloatBias);
 }
 
-// A chunk of a token whose integers cut off too much of it is marked in the last bit of its f (which moves its products by 2^-23, no more
-// than one of the additions that follow), and what they cut off is added behind the loop. An integer is off by at most 1/2, all 128 together by at most 5.7 and as a rule by 3.3 (their norm).
-// With every magnitude counted as 1024 at most (2^-4 to 2^-5 of the largest), a chunk below kMarkBelow, that is of a norm
-// below 4096, is marked: in the others the columns left next to any eight have a norm of 2896, so that what is cut off stays
-// below 2^-9 of them, a rounding of the output, also in rows whose weights for those eight are zero. Of normally distributed values none
-// are marked, of those with a column of 100 times the rest all.
+// A chunk of a token whose integers cut off too much of it is marked in the last bit of its f (which moves its products by 2^-23, no
+// more than one of the additions that follow), and what they cut off is added behind the loop. An integer is off by at most 1/2,
+// all 128 together by at most 5.7 and as a rule by 3.3 (their norm). With every magnitude counted as 1024 at most (2^-4 to 2^-5 of the
+// largest), a chunk below kMarkBelow, that is of a norm below 4096, is marked: in the others the columns left next to any eight
+// have a norm of 2896, so that what is cut off stays below 2^-9 of them, a rounding of the output, also in rows whose weights for
+// those eight are zero. Of normally distributed values none are marked, of those with a column of 100 times the rest all.
 constexpr float kMarkCap = 1024.f, kMarkBelow = 16.f * kMarkCap * kMarkCap;
 constexpr uint32_t kMark = 1;
 

@@ -310,3 +310,29 @@ def test_long_batches_keep_their_precision(T, E):
     assert ((mean.double() - p).abs() <= 2.0 ** -17 * p).all(), ((mean.double() - p).abs() / p).max()
     want = torch.stack((E * p[3], lse.square()))
     assert ((losses.double() - want).abs() <= 2.0 ** -17 * want).all(), (losses, want)
+
+
+def test_two_host_threads_with_different_numbers_of_experts():
+    """Each on its own stream; the amounts of shared memory differ, the same bits come back every time."""
+    import threading
+    cases = [_inputs(16, 1000, 3, torch.float32, 1), _inputs(40, 300, 3, torch.float32, 2), _inputs(900, 600, 3, torch.float32, 3)]
+    want = [_run(*c) for c in cases]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    got = _run(*cases[i])
+                    torch.cuda.current_stream().synchronize()
+                    assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+        except BaseException as e:  # noqa: BLE001
+            failed.append((i, e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed

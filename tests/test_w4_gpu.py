@@ -556,7 +556,7 @@ def test_small_values_next_to_large_ones_that_a_row_ignores(M, N, K, group, zero
     assert (err <= bound).all(), (err / bound).max()
 
 
-@pytest.mark.parametrize("T,act,zeros", [(1, "silu", True), (6, "silu", False), (21, "swigluoai", True)])
+@pytest.mark.parametrize("T,act,zeros", [(1, "silu", True), (6, "silu", False), (21, "swigluoai", True), (1030, "silu", True)])
 def test_small_intermediates_next_to_large_ones_that_a_row_ignores(T, act, zeros):
     """The same in both products of the experts: hidden states and the activations between, which are fp32."""
     g = torch.Generator().manual_seed(T)
@@ -607,3 +607,25 @@ def test_marked_activations_prepared_in_front_or_by_each_block_give_the_same_bit
     out = _linear(bad, packed, scale, zp)
     rest = [i for i in range(M) if i not in (2, 5, 7)]
     assert out[[2, 5, 7]].isnan().all() and torch.equal(out[rest], with_room[rest])
+
+
+def test_marked_activations_of_strided_rows_and_in_a_graph():
+    g = torch.Generator().manual_seed(9)
+    N, K, group = 96, 1024, 32
+    packed, scale, zp = _weights(N, K, group, True, g)
+    wide = torch.randn(9, 2 * K, generator=g)
+    wide[:, K + 3::170] = 4000.0
+    wide = wide.to(torch.bfloat16).cuda()
+    part = wide[:, K:]
+    want = _linear(part.contiguous(), packed, scale, zp)
+    assert torch.equal(_linear(part, packed, scale, zp), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _linear(part, packed, scale, zp)
+    keep = wide.clone()
+    wide.copy_(torch.randn(9, 2 * K, generator=g))  # nothing stands out: no marks
+    graph.replay()
+    assert torch.equal(out, _linear(part.contiguous(), packed, scale, zp)) and not torch.equal(out, want)
+    wide.copy_(keep)
+    graph.replay()
+    assert torch.equal(out, want)
