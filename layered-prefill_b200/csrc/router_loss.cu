@@ -487,11 +487,11 @@ int loss_blocks(int T, int E) {
 template <int N>
 using Int = std::integral_constant<int, N>;
 
-// Calls f(kL, kW, kN): vectors of four where they start on their own size, else single experts. kN is the next of a few widths
-// above E, columns past E being empty work. Both passes of 65519 tokens, fp32: E = 64 28.4 us, 96 (in the width of 128) 36.4, 128 38.0, 160 in
-// a width of its own 35.2 and in that of 256 54.2, 192 57.3 and 224 59.7 in that of 256, 256 60.6. Widths of their own would take
-// 96 to 31.9 and 192 to 40.7; 160 has one because the measured training batch has 160 experts, the others wait for a user. The first
-// pass has 64 registers a thread, as one CTA of a small batch has 1024 threads: in the widths of 32 experts a lane it spills 192 to 240 bytes.
+// Calls f(kL, kW, kN): vectors of four where they start on their own size, else single experts. Up to 256 experts in vectors, the
+// usual form, a lane holds just as many vectors as E needs: what is past E would be empty work (both passes of 65519 tokens, fp32: E = 96 31.9
+// us, and 36.3 in the width of 128; 192 40.7, and 56.4 in that of 256; 160 35.0, and 54.2). Elsewhere kN is the next of two to four
+// widths. The first pass has 64 registers a thread, as one CTA of a small batch has 1024 threads: from 24 experts a lane on it spills, 64 to
+// 240 bytes.
 template <typename F>
 cudaError_t with_lanes(int E, bool vectors, F&& f) {
   if (lanes_of(E) == 32) {
@@ -499,12 +499,16 @@ cudaError_t with_lanes(int E, bool vectors, F&& f) {
     return E <= 512 ? f(Int<32>{}, Int<1>{}, Int<16>{}) : f(Int<32>{}, Int<1>{}, Int<32>{});
   }
   if (vectors && E % 4 == 0) {
-    const int v = (E + 31) / 32;
-    if (v <= 1) return f(Int<8>{}, Int<4>{}, Int<4>{});
-    if (v <= 2) return f(Int<8>{}, Int<4>{}, Int<8>{});
-    if (v <= 4) return f(Int<8>{}, Int<4>{}, Int<16>{});
-    if (v <= 5) return f(Int<8>{}, Int<4>{}, Int<20>{});
-    return f(Int<8>{}, Int<4>{}, Int<32>{});
+    switch ((E + 31) / 32) {
+      case 1: return f(Int<8>{}, Int<4>{}, Int<4>{});
+      case 2: return f(Int<8>{}, Int<4>{}, Int<8>{});
+      case 3: return f(Int<8>{}, Int<4>{}, Int<12>{});
+      case 4: return f(Int<8>{}, Int<4>{}, Int<16>{});
+      case 5: return f(Int<8>{}, Int<4>{}, Int<20>{});
+      case 6: return f(Int<8>{}, Int<4>{}, Int<24>{});
+      case 7: return f(Int<8>{}, Int<4>{}, Int<28>{});
+      default: return f(Int<8>{}, Int<4>{}, Int<32>{});
+    }
   }
   const int n = (E + 7) / 8;
   if (n <= 2) return f(Int<8>{}, Int<1>{}, Int<2>{});

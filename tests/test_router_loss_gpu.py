@@ -336,3 +336,11 @@ def test_two_host_threads_with_different_numbers_of_experts():
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+@pytest.mark.parametrize("E", [4, 28, 32, 36, 64, 68, 92, 96, 100, 132, 164, 188, 192, 196, 220, 224, 228, 252, 256])
+def test_every_number_of_vectors_a_lane(E):
+    for T, dtype in ((45, torch.bfloat16), (700, torch.float32)):
+        args = _inputs(T, E, min(E, 6), dtype, T + E, masked=0.1)
+        _check(_run(*args), _oracle(*args), dtype)
+        _check(_run(args[0], args[1], args[2], None, args[4]), _oracle(args[0], args[1], args[2], None, args[4]), dtype)
